@@ -200,6 +200,19 @@ int srt_sgd_momentum(float* p, const float* g, float* m, void* p_bf16, int64_t n
 int srt_adamw(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, float lr,
               float beta1, float beta2, float eps, float wd, int step, void* stream);
 /* acc += g ; g = 0  (GradAccumulator.accumulate). */
+/* Clipping by the norm of all gradients together (torch.nn.utils.clip_grad_norm_): clip[0] = sqrt(sum of squares, in 64 bits)
+ * over `tensors` device arrays of one dtype, clip[1] = min(1, max_norm / (clip[0] + 1e-6)). srt_clip_grad_norm also multiplies
+ * the arrays by clip[1] in place; the clipped optimizer steps take it from `clip` instead, which saves that pass. grads and
+ * counts are host arrays and are read before the call returns. No array may overlap another. */
+size_t srt_grad_norm_scratch_bytes(int tensors);
+int srt_grad_norm(int dtype, int tensors, const void* const* grads, const int64_t* counts, float max_norm, float* clip, void* scratch,
+                  size_t scratch_bytes, void* stream);
+int srt_clip_grad_norm(int dtype, int tensors, void* const* grads, const int64_t* counts, float max_norm, float* clip, void* scratch,
+                       size_t scratch_bytes, void* stream);
+int srt_adamw_clipped(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, double lr, double beta1, double beta2,
+                      double eps, double wd, int step, const float* clip, void* stream);
+int srt_sgd_momentum_clipped(float* p, const float* g, float* m, void* p_bf16, int64_t n, float lr, float mu, float wd, int first_step,
+                             const float* clip, void* stream);
 int srt_grad_accumulate(float* acc, float* g, int64_t n, void* stream);
 
 /* ---- layout / dtype helpers ---------------------------------------------------------------- */
@@ -494,6 +507,38 @@ int srt_batched_transpose(const void* in, void* out, int R, int C, int64_t ld_in
                           int Z2, void* stream);
 int srt_lm_cross_entropy(void* logits, const int32_t* labels, int64_t rows, int V, int ld, float grad_scale,
                          float* row_loss, void* stream);
+
+/* Root-mean-square norm of rows of C elements (C a multiple of 8, at most 32 KB a row), dtype SRT_F32 or SRT_BF16:
+ *   h = x + residual (residual may be null), rstd = 1 / sqrt(mean(h^2) + eps), y = gamma h rstd.
+ * h and rstd may be null; h may be x or residual. y is formed from the fp32 sum and rounded once. The e4m3 form writes q and
+ * one scale a row instead of y: scale = max(max |y| / 448, 2^-126), q = e4m3(y / scale); srt_quantize_rows_e4m3 does the same
+ * to rows as they are (weights). Backward: dx = dh + the norm's gradient (the gradient of x and of residual alike; dh, the
+ * gradient that reaches h by other ways, may be null; dx may be dy or dh), dgamma = sum over the rows in a fixed order,
+ * overwritten. Operands are 16-byte aligned. Without rows nothing is written but dgamma = 0. */
+int srt_rmsnorm_fwd(int dtype, const void* x, const void* residual, const float* gamma, void* h, void* y, float* rstd, int64_t rows,
+                    int C, float eps, void* stream);
+int srt_rmsnorm_fwd_e4m3(int dtype, const void* x, const void* residual, const float* gamma, void* h, void* q, float* scale, float* rstd,
+                         int64_t rows, int C, float eps, void* stream);
+int srt_quantize_rows_e4m3(int dtype, const void* x, void* q, float* scale, int64_t rows, int C, void* stream);
+size_t srt_rmsnorm_bwd_scratch_bytes(int C);
+int srt_rmsnorm_bwd(int dtype, const void* dy, const void* h, const float* gamma, const float* rstd, const void* dh, void* dx,
+                    float* dgamma, int64_t rows, int C, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Gated feed-forward block: act = silu(x Wg^T) * (x Wu^T), y = residual + act Wd^T, for x [tokens][width],
+ * w_gate_up = Wg over Wu [2 hidden][width], w_down = Wd [width][hidden], all bf16, fp32 accumulation; width and hidden are
+ * multiples of 8, operands 16-byte aligned, matrices below 2^31 elements. residual may be null. act [tokens][hidden] (bf16) is
+ * written on the way; the gate and up projections never reach memory. Backward forms them again from x: dx, dw_gate_up and
+ * dw_down (each may be null; the weights' gradients are of type grad_dtype and overwritten) with
+ * srt_gated_ffn_bwd_scratch_bytes of scratch, 256-byte aligned or better. The e4m3 form takes x and w_gate_up in 8 bits with
+ * one fp32 scale a row (srt_rmsnorm_fwd_e4m3, srt_quantize_rows_e4m3); width is then a multiple of 16. */
+typedef struct srt_gated_ffn_desc { int tokens, width, hidden; } srt_gated_ffn_desc;
+int srt_gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const void* w_gate_up, const void* w_down, const void* residual,
+                      void* act, void* y, void* stream);
+int srt_gated_ffn_fwd_e4m3(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gate_up,
+                           const float* w_scale, const void* w_down, const void* residual, void* act, void* y, void* stream);
+size_t srt_gated_ffn_bwd_scratch_bytes(const srt_gated_ffn_desc* d, int grad_dtype);
+int srt_gated_ffn_bwd(const srt_gated_ffn_desc* d, const void* dy, const void* x, const void* w_gate_up, const void* w_down,
+                      int grad_dtype, void* dx, void* dw_gate_up, void* dw_down, void* scratch, size_t scratch_bytes, void* stream);
 
 /* ---- Swin transformer step -------------------------------------------------------------------------------
  * torchvision.models.swin_b as the reference trains it (train/swin_b.py:38,83-95; AdamW in the DDP config).

@@ -36,7 +36,15 @@ class ConvEpilogue(C.Structure):
 
 
 _vp, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
+
+
+class GatedFfnDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("tokens", "width", "hidden")]
+
+
+_d = C.c_double
 _PD = C.POINTER(ConvDesc)
+_PF = C.POINTER(GatedFfnDesc)
 _PE = C.POINTER(ConvEpilogue)
 
 # name -> (restype, argtypes); restype None means "int status"
@@ -73,6 +81,20 @@ _SIGNATURES = {
     "srt_colsum": (None, [_i, _vp, _i64, _i, _vp, _vp]),
     "srt_sgd_momentum": (None, [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _i, _vp]),
     "srt_adamw": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _i, _vp]),
+    "srt_grad_norm_scratch_bytes": (_sz, [_i]),
+    "srt_grad_norm": (None, [_i, _i, C.POINTER(_vp), C.POINTER(_i64), _f, _vp, _vp, _sz, _vp]),
+    "srt_clip_grad_norm": (None, [_i, _i, C.POINTER(_vp), C.POINTER(_i64), _f, _vp, _vp, _sz, _vp]),
+    "srt_adamw_clipped": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _d, _d, _d, _d, _d, _i, _vp, _vp]),
+    "srt_sgd_momentum_clipped": (None, [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _i, _vp, _vp]),
+    "srt_rmsnorm_fwd": (None, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _f, _vp]),
+    "srt_rmsnorm_fwd_e4m3": (None, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _f, _vp]),
+    "srt_quantize_rows_e4m3": (None, [_i, _vp, _vp, _vp, _i64, _i, _vp]),
+    "srt_rmsnorm_bwd_scratch_bytes": (_sz, [_i]),
+    "srt_rmsnorm_bwd": (None, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp, _sz, _vp]),
+    "srt_gated_ffn_fwd": (None, [_PF, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "srt_gated_ffn_fwd_e4m3": (None, [_PF, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "srt_gated_ffn_bwd_scratch_bytes": (_sz, [_PF, _i]),
+    "srt_gated_ffn_bwd": (None, [_PF, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "srt_grad_accumulate": (None, [_vp, _vp, _i64, _vp]),
     "srt_nchw_to_nhwc": (None, [_i, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "srt_cast_f32_to_bf16": (None, [_vp, _vp, _i64, _vp]),

@@ -275,8 +275,9 @@ __global__ void colsum_kernel(const T* __restrict__ dy, int64_t rows, int K, flo
 __global__ void sgd_momentum_kernel(float* __restrict__ p, const float* __restrict__ g,
                                     float* __restrict__ m, __nv_bfloat16* __restrict__ pb,
                                     int64_t n4, int64_t n, float lr, float mu, float wd,
-                                    int first_step) {
+                                    int first_step, const float* __restrict__ coefficient) {
   pdl_enter();
+  const float k = coefficient ? *coefficient : 1.f;
   int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   for (; i < n4; i += stride) {
@@ -284,7 +285,7 @@ __global__ void sgd_momentum_kernel(float* __restrict__ p, const float* __restri
     const float4 gv = reinterpret_cast<const float4*>(g)[i];
     float4 mv = first_step ? make_float4(0.f, 0.f, 0.f, 0.f) : reinterpret_cast<float4*>(m)[i];
     float pp[4] = {pv.x, pv.y, pv.z, pv.w};
-    const float gg[4] = {gv.x, gv.y, gv.z, gv.w};
+    const float gg[4] = {__fmul_rn(gv.x, k), __fmul_rn(gv.y, k), __fmul_rn(gv.z, k), __fmul_rn(gv.w, k)};
     float mm[4] = {mv.x, mv.y, mv.z, mv.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -305,7 +306,7 @@ __global__ void sgd_momentum_kernel(float* __restrict__ p, const float* __restri
   // scalar tail
   if (blockIdx.x == 0) {
     for (int64_t j = n4 * 4 + threadIdx.x; j < n; j += blockDim.x) {
-      const float d = fmaf(wd, p[j], g[j]);
+      const float d = fmaf(wd, p[j], __fmul_rn(g[j], k));
       const float mj = first_step ? d : fmaf(mu, m[j], d);
       m[j] = mj;
       p[j] = fmaf(-lr, mj, p[j]);
@@ -315,11 +316,11 @@ __global__ void sgd_momentum_kernel(float* __restrict__ p, const float* __restri
 }
 
 // One AdamW element (decoupled decay, bias corrections folded into step_size and bc2_sqrt).
-__device__ inline float adamw_element(float pi, float gi, float& m, float& v, float lr, float b1, float b2, float eps, float wd,
-                                      float step_size, float bc2_sqrt) {
+__device__ inline float adamw_element(float pi, float gi, float& m, float& v, float lr, float b1, float b2, float c1, float c2,
+                                      float eps, float wd, float step_size, float bc2_sqrt) {
   pi = pi * (1.f - lr * wd);
-  m = b1 * m + (1.f - b1) * gi;
-  v = b2 * v + (1.f - b2) * gi * gi;
+  m = b1 * m + c1 * gi;
+  v = b2 * v + c2 * gi * gi;
   const float denom = sqrtf(v) / bc2_sqrt + eps;
   return pi - step_size * (m / denom);
 }
@@ -327,9 +328,10 @@ __device__ inline float adamw_element(float pi, float gi, float& m, float& v, fl
 // elements the loads in flight did not cover the latency (30 bytes x 124 M elements in 904 us, 4.1 TB/s; now 616 us, 6.0 TB/s).
 __global__ void __launch_bounds__(NT)
 adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
-             __nv_bfloat16* __restrict__ pb, int64_t n4, int64_t n, float lr, float b1, float b2, float eps, float wd,
-             float bc1, float bc2_sqrt) {
+             __nv_bfloat16* __restrict__ pb, int64_t n4, int64_t n, float lr, float b1, float b2, float c1, float c2, float eps,
+             float wd, float bc1, float bc2_sqrt, const float* __restrict__ coefficient) {
   pdl_enter();
+  const float k_g = coefficient ? *coefficient : 1.f;  // of clipping; the product with one changes no bit
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   const float step_size = lr / bc1;
   int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -349,10 +351,10 @@ adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restri
     for (int k = 0; k < 2; ++k) {
       if (k && !two) break;
       const int64_t a = i + k * stride;
-      pv[k].x = adamw_element(pv[k].x, gv[k].x, mv[k].x, vv[k].x, lr, b1, b2, eps, wd, step_size, bc2_sqrt);
-      pv[k].y = adamw_element(pv[k].y, gv[k].y, mv[k].y, vv[k].y, lr, b1, b2, eps, wd, step_size, bc2_sqrt);
-      pv[k].z = adamw_element(pv[k].z, gv[k].z, mv[k].z, vv[k].z, lr, b1, b2, eps, wd, step_size, bc2_sqrt);
-      pv[k].w = adamw_element(pv[k].w, gv[k].w, mv[k].w, vv[k].w, lr, b1, b2, eps, wd, step_size, bc2_sqrt);
+      pv[k].x = adamw_element(pv[k].x, __fmul_rn(gv[k].x, k_g), mv[k].x, vv[k].x, lr, b1, b2, c1, c2, eps, wd, step_size, bc2_sqrt);
+      pv[k].y = adamw_element(pv[k].y, __fmul_rn(gv[k].y, k_g), mv[k].y, vv[k].y, lr, b1, b2, c1, c2, eps, wd, step_size, bc2_sqrt);
+      pv[k].z = adamw_element(pv[k].z, __fmul_rn(gv[k].z, k_g), mv[k].z, vv[k].z, lr, b1, b2, c1, c2, eps, wd, step_size, bc2_sqrt);
+      pv[k].w = adamw_element(pv[k].w, __fmul_rn(gv[k].w, k_g), mv[k].w, vv[k].w, lr, b1, b2, c1, c2, eps, wd, step_size, bc2_sqrt);
       reinterpret_cast<float4*>(p)[a] = pv[k];
       reinterpret_cast<float4*>(m)[a] = mv[k];
       reinterpret_cast<float4*>(v)[a] = vv[k];
@@ -367,7 +369,7 @@ adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restri
   }
   // what is left over, or everything when a buffer is not aligned for the vectors (n4 = 0)
   for (i = n4 * 4 + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
-    p[i] = adamw_element(p[i], g[i], m[i], v[i], lr, b1, b2, eps, wd, step_size, bc2_sqrt);
+    p[i] = adamw_element(p[i], __fmul_rn(g[i], k_g), m[i], v[i], lr, b1, b2, c1, c2, eps, wd, step_size, bc2_sqrt);
     if (pb) pb[i] = __float2bfloat16_rn(p[i]);
   }
 }
@@ -575,27 +577,39 @@ int colsum(int dtype, const void* dy, int64_t rows, int K, float* out, cudaStrea
 }
 
 int sgd_momentum(float* p, const float* g, float* m, void* pb, int64_t n, float lr, float mu,
-                 float wd, int first_step, cudaStream_t st) {
+                 float wd, int first_step, cudaStream_t st, const float* coefficient) {
   if (n == 0) return SRT_OK;
   const int64_t n4 = n / 4;
   launch_pdl(sgd_momentum_kernel, dim3(stream_grid(n4 > 0 ? n4 : 1, 8)), dim3(NT), 0, st, 
-      p, g, m, (__nv_bfloat16*)pb, n4, n, lr, mu, wd, first_step);
+      p, g, m, (__nv_bfloat16*)pb, n4, n, lr, mu, wd, first_step, coefficient);
   SRT_LAUNCH_CHECK();
   return SRT_OK;
 }
 
+static int launch_adamw(float* p, const float* g, float* m, float* v, void* pb, int64_t n, float lr, float b1, float b2, float c1, float c2,
+                        float eps, float wd, float bc1, float bc2_sqrt, const float* coefficient, cudaStream_t st) {
+  const bool vectors = ((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) | ((uintptr_t)pb & 7)) == 0;
+  const int64_t n4 = vectors ? n / 4 : 0;
+  launch_pdl(adamw_kernel, dim3(stream_grid(vectors && n4 > 0 ? n4 : n, 8)), dim3(NT), 0, st, p, g, m, v, (__nv_bfloat16*)pb, n4, n,
+             lr, b1, b2, c1, c2, eps, wd, bc1, bc2_sqrt, coefficient);
+  SRT_LAUNCH_CHECK();
+  return SRT_OK;
+}
 int adamw(float* p, const float* g, float* m, float* v, void* pb, int64_t n, float lr, float b1,
-          float b2, float eps, float wd, int step, cudaStream_t st) {
+          float b2, float eps, float wd, int step, cudaStream_t st, const float* coefficient) {
   if (n == 0) return SRT_OK;
   SRT_REQUIRE(step >= 1, "adamw: step counts from 1");
   const float bc1 = 1.f - powf(b1, (float)step);
   const float bc2 = 1.f - powf(b2, (float)step);
-  const bool vectors = ((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) | ((uintptr_t)pb & 7)) == 0;
-  const int64_t n4 = vectors ? n / 4 : 0;
-  launch_pdl(adamw_kernel, dim3(stream_grid(vectors && n4 > 0 ? n4 : n, 8)), dim3(NT), 0, st, p, g, m, v, (__nv_bfloat16*)pb, n4, n,
-             lr, b1, b2, eps, wd, bc1, sqrtf(bc2));
-  SRT_LAUNCH_CHECK();
-  return SRT_OK;
+  return launch_adamw(p, g, m, v, pb, n, lr, b1, b2, 1.f - b1, 1.f - b2, eps, wd, bc1, sqrtf(bc2), coefficient, st);
+}
+// The constants in 64 bits: 1 - beta2 of a beta2 that was rounded to fp32 first is off by 1e-5.
+int adamw_clipped(float* p, const float* g, float* m, float* v, void* pb, int64_t n, double lr, double b1, double b2, double eps, double wd,
+                  int step, const float* clip, cudaStream_t st) {
+  if (n == 0) return SRT_OK;
+  SRT_REQUIRE(step >= 1, "adamw_clipped: step counts from 1");
+  return launch_adamw(p, g, m, v, pb, n, (float)lr, (float)b1, (float)b2, (float)(1.0 - b1), (float)(1.0 - b2), (float)eps, (float)wd,
+                      (float)(1.0 - pow(b1, (double)step)), (float)sqrt(1.0 - pow(b2, (double)step)), clip + 1, st);
 }
 
 int grad_accumulate(float* acc, float* g, int64_t n, cudaStream_t st) {

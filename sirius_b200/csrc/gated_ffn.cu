@@ -1,0 +1,573 @@
+// Gated feed-forward block on the sm_100a tensor cores, without its projections in memory.
+//
+//   forward    act = silu(x Wg^T) * (x Wu^T),   y = residual + act Wd^T
+//   backward   da = dy Wd,  s = 1 / (1 + e^-gate),  silu = gate s
+//              dgate = da up (s + silu (1 - s)),  dup = da silu,  act again
+//              dx = dgate Wg + dup Wu,  dWg = dgate^T x,  dWu = dup^T x,  dWd = dy^T act
+//
+// x [tokens][width], Wg over Wu in one [2 hidden][width] matrix, Wd [width][hidden], all bf16; in 8 bits x and Wg, Wu are
+// e4m3 with one fp32 scale a row, which the epilogue applies (a product of rows scales as its rows do).
+//
+// gated_ffn_kernel<PAIR, BWD, E4M3> makes everything above the line dx: the gate and the up projection of a tile are two
+// halves of one accumulator, so the epilogue holds both factors of the product in fp32 and rounds it once; the backward
+// instance forms both again, and da beside them in a third accumulator, instead of reading what forward would have had to
+// store (4 bytes per token and hidden channel, and twice that to read it: a layer of 8192 x 4864 keeps 240 MB less). What
+// leaves is act and, in backward, dgate and dup, which the plain products of the block read.
+// No sum is shared between CTAs and none depends on the order in which tiles finish: a call repeats bit for bit.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "conv_geom.cuh"
+#include "gated_ffn.cuh"
+#include "ops.cuh"
+#include "ptx.cuh"
+
+namespace srt {
+
+int* tc_status_device_ptr();  // igemm_tcgen05.cu
+// igemm_tcgen05.cu: tensor map of a row-major matrix of 1- or 2-byte elements, boxes of 128 bytes x box_rows, 128-byte swizzle
+int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_rows);
+
+namespace {
+
+using namespace ptx;
+using bf16 = __nv_bfloat16;
+
+constexpr int FM = 128;                  // rows of a CTA's tile (tensor-memory lanes)
+constexpr int F_THREADS = 320;           // warp 0 TMA, warp 1 MMA, warps 2-9 two epilogue groups
+constexpr int F_MAX_STAGES = 8;
+constexpr int F_A_BYTES = FM * 128;      // one 128-byte swizzle row of the reduction a tile row
+constexpr int F_SLAB_BYTES = FM * 128;   // 128 x 64 bf16 on the way out
+enum { W_FFN_LOAD = 0x31, W_FFN_FULL = 0x32, W_FFN_ACC = 0x33, W_FFN_EPI = 0x34, W_FFN_DRAIN = 0x35 };
+
+struct FfnParams {
+  int T, F, k_blocks;
+  int m_units, n_tiles;        // tiles of 128 (256 for a pair) tokens, and of g hidden channels
+  int g;                       // hidden channels of a tile; a pair has 128
+  int cols;                    // tensor-memory columns: a power of two, at least 4 g
+  int stages, stage_bytes;
+  uint32_t gu_bytes, da_bytes; // what one CTA loads a k-block in either phase
+  bf16 *act, *dgu;             // outputs without a tensor map (single CTAs)
+  const float *x_scale, *w_scale;
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
+// Tiles in bands of eight row units, rows fastest: the CTAs at work at one time read about as many rows of x as of the
+// weights, both out of L2.
+__device__ __forceinline__ void tile_of(const FfnParams& p, int t, int& m, int& n) {
+  constexpr int BAND = 8;
+  const int band = t / (BAND * p.n_tiles), first = band * BAND;
+  const int size = min(BAND, p.m_units - first), r = t - first * p.n_tiles;
+  n = r / size;
+  m = first + r - n * size;
+}
+
+// PAIR: cta_group::2, 256 tokens x 128 hidden channels; rank 0 stages the gate rows of the weights and rank 1 the up rows,
+// both halves of the B operand of one 256 x 256 product. Otherwise one CTA has 128 tokens x g channels.
+// Tensor memory, in quarters of `cols`: forward two accumulators of two quarters; backward da of even tiles | gate and up |
+// da of odd tiles, so that the da product of the next tile runs beside the epilogue of the current one.
+template <bool PAIR, bool BWD, bool E4M3>
+__global__ void __launch_bounds__(F_THREADS, PAIR ? 1 : 2)
+gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+                 const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap twd,
+                 const __grid_constant__ CUtensorMap tact, const __grid_constant__ CUtensorMap tgate,
+                 const __grid_constant__ CUtensorMap tup) {
+  constexpr int NCTA = PAIR ? 2 : 1;
+  constexpr int BKE = E4M3 ? 128 : 64;  // reduction elements of a k-block
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int NS = p.stages;
+  uint8_t* sOut = base + NS * p.stage_bytes;  // two slabs, pairs only
+  uint64_t* bars = (uint64_t*)(sOut + (PAIR ? 2 * F_SLAB_BYTES : 0));
+  const uint32_t full = smem_u32(bars), empty = full + 8 * F_MAX_STAGES, acc_full = empty + 8 * F_MAX_STAGES, acc_empty = acc_full + 16;
+  uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * F_MAX_STAGES + 4);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const int unit = (int)blockIdx.x / NCTA, nunits = (int)gridDim.x / NCTA;
+  const int total = p.m_units * p.n_tiles, nkb = p.k_blocks, g = p.g;
+  const int quarter = p.cols / 4;
+  const uint32_t s0 = smem_u32(base);
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + 8 * b, 1); mbar_init(acc_empty + 8 * b, 8 * NCTA); }
+    mbar_fence_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tx);
+    tma_prefetch_desc(&tw);
+    if (BWD) { tma_prefetch_desc(&tdy); tma_prefetch_desc(&twd); }
+  }
+  if (warp == 1) {
+    if (PAIR) { tmem_alloc_pair(smem_u32(tmem_ptr), p.cols); tmem_relinquish_pair(); }
+    else { tmem_alloc(smem_u32(tmem_ptr), p.cols); tmem_relinquish(); }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // the peer's barriers and tensor memory exist before anything refers to them
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_ptr;
+  pdl_enter();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0, s = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      // one k-block: `a` and the B rows of this phase into stage s
+      auto next = [&](uint32_t bytes) -> uint32_t {
+        ok = ok && mbar_wait(empty + 8 * s, ph, p.status, W_FFN_LOAD);
+        if (!ok) return 0u;
+        if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, bytes * NCTA);
+        return PAIR ? map_to_cta(full + 8 * s, 0u) : full + 8 * s;
+      };
+      auto advance = [&]() {
+        ++it;
+        if (++s == NS) { s = 0; ph ^= 1u; }
+      };
+      for (int t = unit; t < total && ok; t += nunits) {
+        int m, n;
+        tile_of(p, t, m, n);
+        const int m0 = (m * NCTA + (int)rank) * FM, n0 = n * g;
+        if (BWD) {
+          for (int kb = 0; kb < nkb; ++kb) {
+            const uint32_t bar = next(p.da_bytes);
+            if (!ok) break;
+            const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + F_A_BYTES;
+            if (PAIR) {
+              tma_load_2d_pair(a, &tdy, bar, kb * 64, m0);
+              tma_load_2d_pair(b, &twd, bar, n0 + (int)rank * 64, kb * 64);
+            } else {
+              tma_load_2d(a, &tdy, bar, kb * 64, m0);
+              for (int c = 0; c < g; c += 64) tma_load_2d(b + c * 128, &twd, bar, n0 + c, kb * 64);
+            }
+            advance();
+          }
+        }
+        for (int kb = 0; kb < nkb && ok; ++kb) {
+          const uint32_t bar = next(p.gu_bytes);
+          if (!ok) break;
+          const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + F_A_BYTES;
+          if (PAIR) {
+            tma_load_2d_pair(a, &tx, bar, kb * BKE, m0);
+            tma_load_2d_pair(b, &tw, bar, kb * BKE, (int)rank * p.F + n0);
+          } else {
+            tma_load_2d(a, &tx, bar, kb * BKE, m0);
+            tma_load_2d(b, &tw, bar, kb * BKE, n0);
+            tma_load_2d(b + g * 128, &tw, bar, kb * BKE, p.F + n0);
+          }
+          advance();
+        }
+      }
+      // a wait that gave up: the copies in flight land before the CTA's memory is given back
+      if (!ok && rank == 0)
+        for (int k = it > NS ? it - NS : 0; k < it; ++k) mbar_wait(full + 8 * (k % NS), (uint32_t)(k / NS) & 1u, p.status, W_FFN_DRAIN);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t i_gu = E4M3 ? make_idesc_e4m3(FM * NCTA, PAIR ? 256 : 2 * g) : make_idesc_bf16(FM * NCTA, PAIR ? 256 : 2 * g, 0, 0);
+      const uint32_t i_da = make_idesc_bf16(FM * NCTA, g, 0, 1);
+      int s = 0, i = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        ok = ok && (PAIR ? mbar_wait_cluster(bar, parity, p.status, code) : mbar_wait(bar, parity, p.status, code));
+        if (ok) tc_fence_after_sync();
+        return ok;
+      };
+      // b_mn: the B rows of this phase lie along the reduction (MN-major)
+      auto product = [&](uint32_t acc, uint32_t idesc, bool b_mn) {
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!wait(full + 8 * s, ph, W_FFN_FULL)) return;
+          const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + F_A_BYTES;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t ad = make_smem_desc_sw128(a + k * 32, 0, 1024);
+            const uint64_t bd = b_mn ? make_smem_desc_sw128(b + k * 2048, 8192, 1024) : make_smem_desc_sw128(b + k * 32, 0, 1024);
+            const uint32_t add = (kb | k) != 0 ? 1u : 0u;
+            if (E4M3) {
+              if (PAIR) umma_e4m3_pair(acc, ad, bd, idesc, add);
+              else umma_e4m3(acc, ad, bd, idesc, add);
+            } else {
+              if (PAIR) umma_bf16_pair(acc, ad, bd, idesc, add);
+              else umma_bf16(acc, ad, bd, idesc, add);
+            }
+          }
+          if (PAIR) umma_commit_pair(empty + 8 * s, (uint16_t)3);
+          else umma_commit(empty + 8 * s);
+          if (++s == NS) { s = 0; ph ^= 1u; }
+        }
+      };
+      for (int t = unit; t < total && ok; t += nunits, ++i) {
+        const uint32_t b = (uint32_t)i & 1u;
+        // tile i - 2 has been read (parity starts so that the first two waits pass)
+        if (!wait(acc_empty + 8 * b, ((uint32_t)(i >> 1) & 1u) ^ 1u, W_FFN_ACC)) break;
+        if (BWD) {
+          product(tmem + (b ? 3u * quarter : 0u), i_da, true);
+          // gate and up have one accumulator: tile i - 1 has been read
+          if (i > 0 && !wait(acc_empty + 8 * (b ^ 1u), (uint32_t)((i - 1) >> 1) & 1u, W_FFN_ACC)) break;
+          product(tmem + quarter, i_gu, false);
+        } else {
+          product(tmem + b * 2u * quarter, i_gu, false);
+        }
+        if (!ok) break;
+        if (PAIR) umma_commit_pair(acc_full + 8 * b, (uint16_t)3);
+        else umma_commit(acc_full + 8 * b);
+      }
+    }
+  } else {
+    const int grp = (warp - 2) >> 2, q = warp & 3, row = q * 32 + lane;
+    const bool issuer = ((warp - 2) & 3) == 0 && lane == 0;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    bool ok = true;
+    int i = 0;
+    for (int t = unit; t < total; t += nunits, ++i) {
+      int m, n;
+      tile_of(p, t, m, n);
+      const int m0 = (m * NCTA + (int)rank) * FM, n0 = n * g;
+      const uint32_t b = (uint32_t)i & 1u;
+      const uint32_t t_gu = tmem + lanes + (BWD ? (uint32_t)quarter : b * 2u * quarter);
+      const uint32_t t_da = tmem + lanes + (b ? 3u * quarter : 0u);
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b, (uint32_t)(i >> 1) & 1u, p.status, W_FFN_EPI));
+      tc_fence_after_sync();
+      const int mrow = m0 + row;
+      const float xs = E4M3 && mrow < p.T ? p.x_scale[mrow] : 1.f;
+      auto done = [&]() {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty + 8 * b, 0u));
+          else mbar_arrive(acc_empty + 8 * b);
+        }
+      };
+      if constexpr (PAIR) {
+        const int c0 = grp * 64;
+        const bool live = m0 < p.T && n0 + c0 < p.F;  // the same for the whole group
+        uint32_t w[BWD ? 3 : 1][32];
+        if (live) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t gv[32], uv[32], dv[BWD ? 32 : 1];
+            tmem_ld_32x32b_x32(t_gu + (uint32_t)(c0 + h * 32), gv);
+            tmem_ld_32x32b_x32(t_gu + 128u + (uint32_t)(c0 + h * 32), uv);
+            if constexpr (BWD) tmem_ld_32x32b_x32(t_da + (uint32_t)(c0 + h * 32), dv);
+            tmem_ld_wait();
+            const int col = n0 + c0 + h * 32;
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float a[2], dg[2], du[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float gt = __uint_as_float(gv[c + e]), up = __uint_as_float(uv[c + e]);
+                if (E4M3) {
+                  const int f = min(col + c + e, p.F - 1);
+                  gt *= xs * p.w_scale[f];
+                  up *= xs * p.w_scale[p.F + f];
+                }
+                const float sg = sigmoid_f(gt), silu = gt * sg;
+                a[e] = silu * up;
+                if constexpr (BWD) {
+                  const float da = __uint_as_float(dv[c + e]);
+                  dg[e] = da * up * (sg + silu * (1.f - sg));
+                  du[e] = da * silu;
+                }
+              }
+              w[0][h * 16 + c / 2] = pack_bf16(a[0], a[1]);
+              if constexpr (BWD) {
+                w[1][h * 16 + c / 2] = pack_bf16(dg[0], dg[1]);
+                w[2][h * 16 + c / 2] = pack_bf16(du[0], du[1]);
+              }
+            }
+          }
+        }
+        done();
+        if (live) {
+          const uint32_t slab = smem_u32(sOut) + (uint32_t)grp * F_SLAB_BYTES, mine = slab + (uint32_t)row * 128u;
+#pragma unroll
+          for (int o = 0; o < (BWD ? 3 : 1); ++o) {
+            if (issuer) bulk_wait_group_read<0>();  // the store before has read the slab
+            named_bar_sync(1 + grp, 128);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              st_shared_v4(mine + (uint32_t)((c ^ (row & 7)) << 4), w[o][c * 4], w[o][c * 4 + 1], w[o][c * 4 + 2], w[o][c * 4 + 3]);
+            fence_proxy_async_smem();
+            named_bar_sync(1 + grp, 128);
+            if (issuer) {
+              tma_store_2d(o == 0 ? &tact : o == 1 ? &tgate : &tup, slab, n0 + c0, m0);
+              bulk_commit_group();
+            }
+          }
+        }
+      } else {
+        // eight channels at a time, dealt to the two groups in turn
+        if (m0 < p.T)
+          for (int c = grp * 8; c < g; c += 16) {
+            uint32_t gv[8], uv[8], dv[8];
+            tmem_ld_32x32b_x8(t_gu + (uint32_t)c, gv);
+            tmem_ld_32x32b_x8(t_gu + (uint32_t)(g + c), uv);
+            if constexpr (BWD) tmem_ld_32x32b_x8(t_da + (uint32_t)c, dv);
+            tmem_ld_wait();
+            const int f = n0 + c;
+            if (mrow < p.T && f < p.F) {
+              float a[8], dg[8], du[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float gt = __uint_as_float(gv[e]), up = __uint_as_float(uv[e]);
+                if (E4M3) {
+                  gt *= xs * p.w_scale[f + e];
+                  up *= xs * p.w_scale[p.F + f + e];
+                }
+                const float sg = sigmoid_f(gt), silu = gt * sg;
+                a[e] = silu * up;
+                if constexpr (BWD) {
+                  const float da = __uint_as_float(dv[e]);
+                  dg[e] = da * up * (sg + silu * (1.f - sg));
+                  du[e] = da * silu;
+                }
+              }
+              Vec16<bf16> o;
+              o.pack(a);
+              o.store(p.act + (size_t)mrow * p.F + f);
+              if constexpr (BWD) {
+                o.pack(dg);
+                o.store(p.dgu + (size_t)mrow * 2 * p.F + f);
+                o.pack(du);
+                o.store(p.dgu + (size_t)mrow * 2 * p.F + p.F + f);
+              }
+            }
+          }
+        done();
+      }
+    }
+    if (PAIR && issuer) bulk_wait_group_read<0>();  // the slab outlives the last store's read
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // neither CTA leaves while the other can signal its barriers or read its operands
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after_sync();
+    if (PAIR) tmem_dealloc_pair(tmem, p.cols);
+    else tmem_dealloc(tmem, p.cols);
+  }
+}
+
+constexpr size_t ffn_tail_bytes() { return (2 * F_MAX_STAGES + 4) * 8 + 16; }
+
+// How a call is cut. Clocks a k-block and SM are those of the operand stream out of L2 (about 50 bytes a clock and SM), which
+// bounds either form before the tensor cores do; the form and the tile width with the shorter longest SM win.
+struct FfnPlan {
+  bool pair;
+  int g;
+};
+FfnPlan plan_ffn(int T, int F, bool bwd) {
+  const int sms = sm_count();
+  const int a_rows = T < FM ? (T + 7) / 8 * 8 : FM;
+  FfnPlan best = {false, 16};
+  double best_cost = 1e30;
+  for (int g = 16; g <= 128; g += bwd ? 16 : 8) {
+    const long long tiles = (long long)ceil_div(T, FM) * ceil_div(F, g);
+    const double bytes = 128.0 * a_rows * (bwd ? 2 : 1) + 256.0 * g + (bwd ? 8192.0 * ceil_div(g, 64) : 0.0);
+    const double cost = (double)ceil_div_ll(tiles, sms) * bytes;
+    if (cost < best_cost) { best_cost = cost; best = {false, g}; }
+  }
+  if (sms >= 2) {
+    const long long tiles = (long long)ceil_div(T, 2 * FM) * ceil_div(F, 128);
+    const double cost = (double)ceil_div_ll(tiles, sms / 2) * (32768.0 + (bwd ? 24576.0 : 0.0));
+    if (cost < best_cost) best = {true, 128};
+  }
+  return best;
+}
+
+template <bool PAIR, bool BWD, bool E4M3>
+int launch_ffn(FfnParams& p, const CUtensorMap (&tm)[7], cudaStream_t st) {
+  const size_t budget = PAIR || p.cols > 256 ? 232448 : 113 * 1024;  // two single CTAs share an SM where tensor memory allows
+  const size_t fixed = 1024 + (PAIR ? 2 * F_SLAB_BYTES : 0) + ffn_tail_bytes();
+  p.stages = (int)((budget - fixed) / p.stage_bytes);
+  if (p.stages > F_MAX_STAGES) p.stages = F_MAX_STAGES;
+  const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
+  SRT_CHECK_CUDA(cudaFuncSetAttribute(gated_ffn_kernel<PAIR, BWD, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+  const int room = PAIR ? sm_count() / 2 : sm_count() * (p.cols > 256 ? 1 : 2);
+  const long long total = (long long)p.m_units * p.n_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((total < room ? total : room) * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(F_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = (pdl_big_kernels() && (pdl_classes() & PDL_GEMM) != 0) ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (PAIR) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  SRT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gated_ffn_kernel<PAIR, BWD, E4M3>, p, tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6]));
+  SRT_LAUNCH_CHECK();
+  return SRT_OK;
+}
+
+// act, and with dy also dgu = (dgate, dup), from x and the weights.
+int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_scale, const void* w_gu, const float* w_scale,
+                   const void* dy, const void* w_down, void* act, void* dgu, cudaStream_t st) {
+  const bool bwd = dy != nullptr, e4m3 = x_scale != nullptr;
+  const int T = d.tokens, C = d.width, F = d.hidden, esz = e4m3 ? 1 : 2;
+  const FfnPlan plan = plan_ffn(T, F, bwd);
+  FfnParams p = {};
+  p.T = T;
+  p.F = F;
+  p.g = plan.g;
+  p.k_blocks = ceil_div(C, 128 / esz);
+  p.m_units = ceil_div(T, plan.pair ? 2 * FM : FM);
+  p.n_tiles = ceil_div(F, plan.g);
+  p.cols = 32;
+  while (p.cols < 4 * plan.g) p.cols *= 2;
+  const int a_rows = plan.pair || T >= FM ? FM : (T + 7) / 8 * 8;
+  const int b_rows = plan.pair ? 128 : plan.g;  // of the gate or of the up matrix, a CTA and k-block
+  const int da_blocks = plan.pair ? 1 : ceil_div(plan.g, 64);
+  p.gu_bytes = (uint32_t)(a_rows + (plan.pair ? 1 : 2) * b_rows) * 128u;
+  p.da_bytes = (uint32_t)a_rows * 128u + (uint32_t)da_blocks * 8192u;
+  int b_bytes = (plan.pair ? 1 : 2) * b_rows * 128;
+  if (bwd && da_blocks * 8192 > b_bytes) b_bytes = da_blocks * 8192;
+  p.stage_bytes = F_A_BYTES + b_bytes;
+  p.act = (bf16*)act;
+  p.dgu = (bf16*)dgu;
+  p.x_scale = x_scale;
+  p.w_scale = w_scale;
+  p.status = tc_status_device_ptr();
+  SRT_REQUIRE(p.status != nullptr, "tcgen05 status word unavailable");
+  CUtensorMap tm[7];
+  int rc;
+  if ((rc = tmap_rows_128b(&tm[0], x, T, C, C, esz, a_rows)) || (rc = tmap_rows_128b(&tm[1], w_gu, 2ull * F, C, C, esz, b_rows))) return rc;
+  for (int i = 2; i < 7; ++i) tm[i] = tm[0];
+  if (bwd && ((rc = tmap_rows_128b(&tm[2], dy, T, C, C, 2, a_rows)) || (rc = tmap_rows_128b(&tm[3], w_down, C, F, F, 2, 64)))) return rc;
+  if (plan.pair && (rc = tmap_rows_128b(&tm[4], act, T, F, F, 2, FM))) return rc;
+  // the two halves of dgu have maps of their own: a store that reaches beyond `hidden` is clipped in either
+  if (plan.pair && bwd && ((rc = tmap_rows_128b(&tm[5], dgu, T, F, 2ull * F, 2, FM)) ||
+                           (rc = tmap_rows_128b(&tm[6], (bf16*)dgu + F, T, F, 2ull * F, 2, FM))))
+    return rc;
+  if (bwd) return plan.pair ? launch_ffn<true, true, false>(p, tm, st) : launch_ffn<false, true, false>(p, tm, st);
+  if (e4m3) return plan.pair ? launch_ffn<true, false, true>(p, tm, st) : launch_ffn<false, false, true>(p, tm, st);
+  return plan.pair ? launch_ffn<true, false, false>(p, tm, st) : launch_ffn<false, false, false>(p, tm, st);
+}
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+srt_conv_desc linear(int rows, int in, int out) { return {rows, 1, 1, in, out, 1, 1, 1, 0, 1, 1}; }
+
+int check_ffn(const srt_gated_ffn_desc* d, int width_unit) {
+  SRT_REQUIRE(d, "gated_ffn: null descriptor");
+  SRT_REQUIRE(d->tokens >= 0 && d->width > 0 && d->hidden > 0, "gated_ffn: sizes %d, %d, %d out of range", d->tokens, d->width, d->hidden);
+  SRT_REQUIRE(d->width % width_unit == 0 && d->hidden % 8 == 0, "gated_ffn: width (%d) must be a multiple of %d and hidden (%d) of 8",
+              d->width, width_unit, d->hidden);
+  SRT_REQUIRE((long long)d->tokens * 2 * d->hidden < (1ll << 31) && (long long)d->tokens * d->width < (1ll << 31) &&
+                  2ll * d->hidden * d->width < (1ll << 31),
+              "gated_ffn: a matrix of %d tokens x (%d, 2 x %d) exceeds 2^31 elements", d->tokens, d->width, d->hidden);
+  return SRT_OK;
+}
+#define FFN_ALIGNED(...) ffn_aligned({__VA_ARGS__})
+int ffn_aligned(std::initializer_list<const void*> ps) {
+  for (const void* q : ps) SRT_REQUIRE(((uintptr_t)q & 15) == 0, "gated_ffn: operands must be 16-byte aligned");
+  return SRT_OK;
+}
+
+// y = residual + act Wd^T
+int down_product(const srt_gated_ffn_desc& d, const void* act, const void* w_down, const void* residual, void* y, cudaStream_t st) {
+  return conv_fprop_infer(linear(d.tokens, d.hidden, d.width), SRT_BF16, SRT_IMPL_AUTO, act, w_down, y, {nullptr, nullptr, residual, ACT_NONE}, st);
+}
+
+}  // namespace
+
+int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gu, const float* w_scale,
+                  const void* w_down, const void* residual, void* act, void* y, bool e4m3, cudaStream_t st) {
+  int rc = check_ffn(d, e4m3 ? 16 : 8);
+  if (rc || d->tokens == 0) return rc;
+  SRT_REQUIRE(x && w_gu && w_down && act && y && (!e4m3 || (x_scale && w_scale)), "gated_ffn_fwd: null operand");
+  if ((rc = FFN_ALIGNED(x, w_gu, w_down, residual, act, y))) return rc;
+  if ((rc = gated_products(*d, x, x_scale, w_gu, w_scale, nullptr, nullptr, act, nullptr, st))) return rc;
+  return down_product(*d, act, w_down, residual, y, st);
+}
+
+GatedFfnScratch gated_ffn_scratch(const srt_gated_ffn_desc& d, int grad_dtype) {
+  GatedFfnScratch s;
+  const size_t TF = (size_t)d.tokens * d.hidden, CF = (size_t)d.width * d.hidden;
+  s.dgu = up256(TF * 2);
+  s.grad = s.dgu + up256(TF * 4);
+  s.wgrad = s.grad + (grad_dtype == SRT_BF16 ? up256(CF * 8) : 0);  // the larger of the two gradients before it is rounded
+  size_t w = 0;
+  if (d.tokens > 0) {
+    const size_t a = conv_wgrad_scratch_bytes(linear(d.tokens, d.width, 2 * d.hidden), SRT_BF16, SRT_IMPL_AUTO);
+    const size_t b = conv_wgrad_scratch_bytes(linear(d.tokens, d.hidden, d.width), SRT_BF16, SRT_IMPL_AUTO);
+    w = a > b ? a : b;
+  }
+  s.wgrad_bytes = w;
+  s.total = s.wgrad + up256(w);
+  return s;
+}
+
+int gated_ffn_bwd(const srt_gated_ffn_desc* d, const void* dy, const void* x, const void* w_gu, const void* w_down, int grad_dtype,
+                  void* dx, void* dw_gu, void* dw_down, void* scratch, size_t scratch_bytes, cudaStream_t st) {
+  int rc = check_ffn(d, 8);
+  if (rc) return rc;
+  SRT_REQUIRE(grad_dtype == SRT_F32 || grad_dtype == SRT_BF16, "gated_ffn_bwd: gradient type %d is neither SRT_F32 nor SRT_BF16", grad_dtype);
+  const int T = d->tokens, C = d->width, F = d->hidden;
+  const size_t CF = (size_t)C * F, gsz = grad_dtype == SRT_F32 ? 4 : 2;
+  if (T == 0) {
+    if (dw_gu) SRT_CHECK_CUDA(cudaMemsetAsync(dw_gu, 0, 2 * CF * gsz, st));
+    if (dw_down) SRT_CHECK_CUDA(cudaMemsetAsync(dw_down, 0, CF * gsz, st));
+    return SRT_OK;
+  }
+  SRT_REQUIRE(dy && x && w_gu && w_down, "gated_ffn_bwd: null operand");
+  const GatedFfnScratch s = gated_ffn_scratch(*d, grad_dtype);
+  SRT_REQUIRE(scratch && scratch_bytes >= s.total, "gated_ffn_bwd: scratch too small (%zu < %zu)", scratch_bytes, s.total);
+  if ((rc = FFN_ALIGNED(dy, x, w_gu, w_down, dx, dw_gu, dw_down, scratch))) return rc;
+  char* base = (char*)scratch;
+  void *act = base, *dgu = base + s.dgu, *wscratch = base + s.wgrad;
+  if ((rc = gated_products(*d, x, nullptr, w_gu, nullptr, dy, w_down, act, dgu, st))) return rc;
+  if (dx && (rc = conv_dgrad_direct(linear(T, C, 2 * F), SRT_BF16, SRT_IMPL_AUTO, dgu, w_gu, dx, nullptr, st))) return rc;
+  auto weights = [&](const srt_conv_desc& c, const void* g, const void* in, void* out, size_t n) -> int {
+    float* f = grad_dtype == SRT_F32 ? (float*)out : (float*)(base + s.grad);
+    int r = conv_wgrad(c, SRT_BF16, SRT_IMPL_AUTO, g, in, f, wscratch, s.wgrad_bytes, st);
+    return r || grad_dtype == SRT_F32 ? r : cast_f32_to_bf16(f, out, (int64_t)n, st);
+  };
+  if (dw_gu && (rc = weights(linear(T, C, 2 * F), dgu, x, dw_gu, 2 * CF))) return rc;
+  if (dw_down && (rc = weights(linear(T, F, C), dy, act, dw_down, CF))) return rc;
+  return SRT_OK;
+}
+
+}  // namespace srt
+
+using namespace srt;
+
+extern "C" {
+
+int srt_gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const void* w_gate_up, const void* w_down, const void* residual,
+                      void* act, void* y, void* stream) {
+  return gated_ffn_fwd(d, x, nullptr, w_gate_up, nullptr, w_down, residual, act, y, false, (cudaStream_t)stream);
+}
+
+int srt_gated_ffn_fwd_e4m3(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gate_up,
+                           const float* w_scale, const void* w_down, const void* residual, void* act, void* y, void* stream) {
+  return gated_ffn_fwd(d, x, x_scale, w_gate_up, w_scale, w_down, residual, act, y, true, (cudaStream_t)stream);
+}
+
+size_t srt_gated_ffn_bwd_scratch_bytes(const srt_gated_ffn_desc* d, int grad_dtype) {
+  return check_ffn(d, 8) ? 0 : gated_ffn_scratch(*d, grad_dtype).total;
+}
+
+int srt_gated_ffn_bwd(const srt_gated_ffn_desc* d, const void* dy, const void* x, const void* w_gate_up, const void* w_down,
+                      int grad_dtype, void* dx, void* dw_gate_up, void* dw_down, void* scratch, size_t scratch_bytes, void* stream) {
+  return gated_ffn_bwd(d, dy, x, w_gate_up, w_down, grad_dtype, dx, dw_gate_up, dw_down, scratch, scratch_bytes, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -1744,6 +1744,28 @@ int tmap_batched_bf16(CUtensorMap* tm, const void* base, uint64_t kdim, uint64_t
   return make_tmap_4d(tm, base, kdim, rows, z1, z2, ld, s1, s2, box_rows);
 }
 
+// Row-major matrix of 1- or 2-byte elements, rows `pitch` elements apart, boxes of 128 bytes x box_rows, 128B swizzle.
+int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return SRT_ERR_CUDA;
+  }
+  SRT_REQUIRE(((uintptr_t)base & 15) == 0 && pitch * elem_bytes % 16 == 0, "TMA operand must be 16-byte aligned with a 16-byte multiple row pitch");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch * elem_bytes};
+  cuuint32_t box[2] = {128u / (uint32_t)elem_bytes, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(tm, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return SRT_ERR_CUDA;
+  }
+  return SRT_OK;
+}
+
 int bgemm_bf16(const BgemmDesc& d, const void* A, const void* B, void* D, cudaStream_t st) {
   SRT_REQUIRE(d.M > 0 && d.N > 0 && d.K > 0 && d.Z1 > 0 && d.Z2 > 0, "bgemm: empty problem");
   SRT_REQUIRE(d.K % 8 == 0 && d.N % 8 == 0 && d.ldd % 8 == 0 && d.d_s1 % 8 == 0 && d.d_s2 % 8 == 0 &&

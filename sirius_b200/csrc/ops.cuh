@@ -55,10 +55,14 @@ int softmax_ce(int dtype, const void* logits, const int64_t* labels, int B, int 
                float grad_scale, float* row_loss, void* dlogits, cudaStream_t st);
 int sum_f32(const float* v, int n, float* out, int accumulate, cudaStream_t st);
 int colsum(int dtype, const void* dy, int64_t rows, int K, float* out, cudaStream_t st);
+// coefficient: a device value that every gradient is multiplied by (clipping), or null.
 int sgd_momentum(float* p, const float* g, float* m, void* pb, int64_t n, float lr, float mu,
-                 float wd, int first_step, cudaStream_t st);
+                 float wd, int first_step, cudaStream_t st, const float* coefficient = nullptr);
 int adamw(float* p, const float* g, float* m, float* v, void* pb, int64_t n, float lr, float b1,
-          float b2, float eps, float wd, int step, cudaStream_t st);
+          float b2, float eps, float wd, int step, cudaStream_t st, const float* coefficient = nullptr);
+// clip: the two results of grad_norm.
+int adamw_clipped(float* p, const float* g, float* m, float* v, void* pb, int64_t n, double lr, double b1, double b2, double eps, double wd,
+                  int step, const float* clip, cudaStream_t st);
 int grad_accumulate(float* acc, float* g, int64_t n, cudaStream_t st);
 int nchw_to_nhwc(int dtype, const float* src, void* dst, int N, int C, int H, int W, int Cpad,
                  cudaStream_t st);

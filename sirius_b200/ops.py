@@ -29,6 +29,28 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def _check(what, shape, dtype, device, **tensors):
+    """Each of `tensors` is a contiguous CUDA tensor on the current device (whose stream the call goes to), beside `device`,
+    of this shape and type. None passes; a shape or type of None is not looked at."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous CUDA tensor")
+        if t.device != device or t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{what}: {name} is on {t.device}; operands are on the current device, cuda:{torch.cuda.current_device()}")
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"{what}: {name} is {t.dtype}, not {dtype}")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+
+
+def _device(what, t):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: tensors are wanted")
+    return t.device
+
+
 def _ep(bias, addend, addend_bits=None):
     if bias is None and addend is None:
         return None
@@ -226,12 +248,166 @@ def colsum(dy):
     return out
 
 
-def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None):
+def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None, clip=None):
+    """`clip` as in adamw."""
+    if clip is not None:
+        _clip_operands(p, g, m, p_bf16, clip)
+        call("srt_sgd_momentum_clipped", _p(p), _p(g), _p(m), _p(p_bf16), p.numel(), lr, mu, wd, int(first_step), _p(clip), _stream())
+        return
     call("srt_sgd_momentum", _p(p), _p(g), _p(m), _p(p_bf16), p.numel(), lr, mu, wd, int(first_step), _stream())
 
 
-def adamw(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16=None):
+def adamw(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16=None, clip=None):
+    """`clip`: what grad_norm returned; the gradients are multiplied by its coefficient on the way in."""
+    if clip is not None:
+        _clip_operands(p, g, m, v, p_bf16, clip)
+        call("srt_adamw_clipped", _p(p), _p(g), _p(m), _p(v), _p(p_bf16), p.numel(), lr, b1, b2, eps, wd, step, _p(clip), _stream())
+        return
     call("srt_adamw", _p(p), _p(g), _p(m), _p(v), _p(p_bf16), p.numel(), lr, b1, b2, eps, wd, step, _stream())
+
+
+def _clip_operands(p, *rest):
+    *state, p_bf16, clip = rest
+    dev = _device("clipped step", p)
+    _check("clipped step", None, torch.float32, dev, p=p)
+    for t in state:
+        _check("clipped step", p.shape, torch.float32, dev, state=t)
+    _check("clipped step", p.shape, torch.bfloat16, dev, p_bf16=p_bf16)
+    _check("clipped step", (2,), torch.float32, dev, clip=clip)
+
+
+def _grad_list(name, grads, max_norm):
+    grads = list(grads)
+    if not max_norm > 0:
+        raise ValueError(f"{name}: max_norm ({max_norm}) must be positive")
+    dev = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    dtype = grads[0].dtype if grads else torch.float32
+    for g in grads:
+        _check(name, None, dtype, dev, gradient=g)
+    n = len(grads)
+    nbytes = _lib.lib().srt_grad_norm_scratch_bytes(n)
+    # the results first, the partial sums behind them
+    work = torch.empty(256 + nbytes, dtype=torch.uint8, device=dev)
+    clip = work[:8].view(torch.float32)
+    call("srt_" + name, SRT_F32 if dtype == torch.float32 else _dt(grads[0]), n, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
+         (C.c_int64 * n)(*[g.numel() for g in grads]), max_norm, clip.data_ptr(), work.data_ptr() + 256, nbytes, _stream())
+    return clip
+
+
+def grad_norm(grads, max_norm):
+    """Norm of all gradients together (a list of tensors of one type) and the coefficient that brings it down to `max_norm`,
+    min(1, max_norm / (norm + 1e-6)): a device tensor of these two, for the `clip` argument of the optimizer steps."""
+    return _grad_list("grad_norm", grads, max_norm)
+
+
+def clip_grad_norm(grads, max_norm):
+    """grad_norm that also multiplies the gradients by the coefficient, in place (torch.nn.utils.clip_grad_norm_)."""
+    return _grad_list("clip_grad_norm", grads, max_norm)
+
+
+def _rows(what, x, gamma, residual):
+    dev = _device(what, x)
+    if x.dim() < 1 or x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what}: rows of float32 or bfloat16 are wanted, not {x.dtype}")
+    _check(what, None, None, dev, x=x)
+    _check(what, x.shape, x.dtype, dev, residual=residual)
+    _check(what, x.shape[-1:], torch.float32, dev, gamma=gamma)
+    return dev, x.shape[-1], x.numel() // max(x.shape[-1], 1)
+
+
+def rmsnorm(x, gamma, eps=1e-6, residual=None):
+    """h = x + residual, y = gamma * h / rms(h) over the last axis: returns (y, h, rstd). Without a residual h is x itself."""
+    dev, Cc, rows = _rows("rmsnorm", x, gamma, residual)
+    y = torch.empty_like(x)
+    h = torch.empty_like(x) if residual is not None else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    call("srt_rmsnorm_fwd", _dt(x), _p(x), _p(residual), _p(gamma), _p(h), _p(y), _p(rstd), rows, Cc, eps, _stream())
+    return y, x if h is None else h, rstd
+
+
+def rmsnorm_e4m3(x, gamma, eps=1e-6, residual=None):
+    """rmsnorm whose output leaves in 8 bits, q * scale of its row: returns (q, scale, h, rstd)."""
+    dev, Cc, rows = _rows("rmsnorm_e4m3", x, gamma, residual)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    h = torch.empty_like(x) if residual is not None else None
+    rstd, scale = (torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) for _ in range(2))
+    call("srt_rmsnorm_fwd_e4m3", _dt(x), _p(x), _p(residual), _p(gamma), _p(h), _p(q), _p(scale), _p(rstd), rows, Cc, eps, _stream())
+    return q, scale, x if h is None else h, rstd
+
+
+def quantize_rows_e4m3(x):
+    """Rows (of weights, say) in 8 bits: (q, scale) with x close to q * scale."""
+    dev, Cc, rows = _rows("quantize_rows_e4m3", x, None, None)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    call("srt_quantize_rows_e4m3", _dt(x), _p(x), _p(q), _p(scale), rows, Cc, _stream())
+    return q, scale
+
+
+def rmsnorm_backward(dy, h, gamma, rstd, dh=None):
+    """Gradient of rmsnorm at the h and rstd that it returned: (dx, dgamma). dx is the gradient of x and of the residual; `dh`
+    is what reaches h from elsewhere (the residual path) and is added to it."""
+    dev, Cc, rows = _rows("rmsnorm_backward", h, gamma, dh)
+    _check("rmsnorm_backward", h.shape, h.dtype, dev, dy=dy)
+    _check("rmsnorm_backward", h.shape[:-1], torch.float32, dev, rstd=rstd)
+    dx = torch.empty_like(h)
+    dgamma = torch.empty(Cc, dtype=torch.float32, device=dev)
+    nbytes = _lib.lib().srt_rmsnorm_bwd_scratch_bytes(Cc)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    call("srt_rmsnorm_bwd", _dt(h), _p(dy), _p(h), _p(gamma), _p(rstd), _p(dh), _p(dx), _p(dgamma), rows, Cc, _p(scratch), nbytes, _stream())
+    return dx, dgamma
+
+
+def _ffn(what, x, w_gate_up, w_down, dtype):
+    dev = _device(what, x)
+    _check(what, None, dtype, dev, x=x, w_gate_up=w_gate_up)
+    _check(what, None, torch.bfloat16, dev, w_down=w_down)
+    if x.dim() != 2 or w_gate_up.dim() != 2 or w_down.dim() != 2 or w_gate_up.shape[0] != 2 * w_down.shape[1]:
+        raise ValueError(f"{what}: x [tokens, width], w_gate_up [2 hidden, width] and w_down [width, hidden] are wanted, not "
+                         f"{tuple(x.shape)}, {tuple(w_gate_up.shape)} and {tuple(w_down.shape)}")
+    (tokens, width), hidden = x.shape, w_down.shape[1]
+    if w_gate_up.shape[1] != width or w_down.shape[0] != width:
+        raise ValueError(f"{what}: x has {width} columns, w_gate_up {w_gate_up.shape[1]} and w_down {w_down.shape[0]} rows")
+    return dev, _lib.GatedFfnDesc(tokens, width, hidden)
+
+
+def gated_ffn(x, w_gate_up, w_down, residual=None):
+    """residual + (silu(x Wg^T) * (x Wu^T)) Wd^T with w_gate_up = Wg over Wu; bf16."""
+    dev, d = _ffn("gated_ffn", x, w_gate_up, w_down, torch.bfloat16)
+    _check("gated_ffn", x.shape, torch.bfloat16, dev, residual=residual)
+    act = torch.empty((d.tokens, d.hidden), dtype=torch.bfloat16, device=dev)
+    y = torch.empty_like(x)
+    call("srt_gated_ffn_fwd", C.byref(d), _p(x), _p(w_gate_up), _p(w_down), _p(residual), _p(act), _p(y), _stream())
+    return y
+
+
+def gated_ffn_e4m3(x, x_scale, w_gate_up, w_scale, w_down, residual=None):
+    """gated_ffn on 8-bit rows: x * x_scale of its row (rmsnorm_e4m3) and w_gate_up * w_scale of its row (quantize_rows_e4m3)."""
+    dev, d = _ffn("gated_ffn_e4m3", x, w_gate_up, w_down, torch.float8_e4m3fn)
+    _check("gated_ffn_e4m3", (d.tokens,), torch.float32, dev, x_scale=x_scale)
+    _check("gated_ffn_e4m3", (2 * d.hidden,), torch.float32, dev, w_scale=w_scale)
+    _check("gated_ffn_e4m3", x.shape, torch.bfloat16, dev, residual=residual)
+    act = torch.empty((d.tokens, d.hidden), dtype=torch.bfloat16, device=dev)
+    y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+    call("srt_gated_ffn_fwd_e4m3", C.byref(d), _p(x), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(w_down), _p(residual), _p(act), _p(y),
+         _stream())
+    return y
+
+
+def gated_ffn_backward(dy, x, w_gate_up, w_down, grad_dtype=torch.bfloat16):
+    """Gradients of gated_ffn at x, which is all that forward has to keep: (dx, dw_gate_up, dw_down), the weights' in
+    `grad_dtype` (bfloat16, or float32 for an optimizer that accumulates there). The residual's gradient is dy itself."""
+    dev, d = _ffn("gated_ffn_backward", x, w_gate_up, w_down, torch.bfloat16)
+    _check("gated_ffn_backward", x.shape, torch.bfloat16, dev, dy=dy)
+    if grad_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"gated_ffn_backward: gradients in bfloat16 or float32, not {grad_dtype}")
+    g = SRT_F32 if grad_dtype == torch.float32 else SRT_BF16
+    dx, dw_gate_up, dw_down = torch.empty_like(x), torch.empty_like(w_gate_up, dtype=grad_dtype), torch.empty_like(w_down, dtype=grad_dtype)
+    nbytes = _lib.lib().srt_gated_ffn_bwd_scratch_bytes(C.byref(d), g)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    call("srt_gated_ffn_bwd", C.byref(d), _p(dy), _p(x), _p(w_gate_up), _p(w_down), g, _p(dx), _p(dw_gate_up), _p(dw_down), _p(scratch),
+         nbytes, _stream())
+    return dx, dw_gate_up, dw_down
 
 
 def grad_accumulate(acc, g):
