@@ -526,16 +526,17 @@ int srt_rmsnorm_bwd(int dtype, const void* dy, const void* h, const float* gamma
 
 /* Gated feed-forward block: act = silu(x Wg^T) * (x Wu^T), y = residual + act Wd^T, for x [tokens][width],
  * w_gate_up = Wg over Wu [2 hidden][width], w_down = Wd [width][hidden], all bf16, fp32 accumulation; width and hidden are
- * multiples of 8, operands 16-byte aligned, matrices below 2^31 elements. residual may be null. act [tokens][hidden] (bf16) is
- * written on the way; the gate and up projections never reach memory. Backward forms them again from x: dx, dw_gate_up and
- * dw_down (each may be null; the weights' gradients are of type grad_dtype and overwritten) with
- * srt_gated_ffn_bwd_scratch_bytes of scratch, 256-byte aligned or better. The e4m3 form takes x and w_gate_up in 8 bits with
+ * multiples of 8, operands and scratch 16-byte aligned, matrices below 2^31 elements. residual may be null. The gate and up
+ * projections never reach memory. Backward forms them again from x: dx, dw_gate_up and dw_down (each may be null; the weights'
+ * gradients are of type grad_dtype and overwritten). scratch: what the _scratch_bytes calls say. The e4m3 form takes x and w_gate_up in 8 bits with
  * one fp32 scale a row (srt_rmsnorm_fwd_e4m3, srt_quantize_rows_e4m3); width is then a multiple of 16. */
 typedef struct srt_gated_ffn_desc { int tokens, width, hidden; } srt_gated_ffn_desc;
+size_t srt_gated_ffn_fwd_scratch_bytes(const srt_gated_ffn_desc* d);
 int srt_gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const void* w_gate_up, const void* w_down, const void* residual,
-                      void* act, void* y, void* stream);
+                      void* y, void* scratch, size_t scratch_bytes, void* stream);
 int srt_gated_ffn_fwd_e4m3(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gate_up,
-                           const float* w_scale, const void* w_down, const void* residual, void* act, void* y, void* stream);
+                           const float* w_scale, const void* w_down, const void* residual, void* y, void* scratch, size_t scratch_bytes,
+                           void* stream);
 size_t srt_gated_ffn_bwd_scratch_bytes(const srt_gated_ffn_desc* d, int grad_dtype);
 int srt_gated_ffn_bwd(const srt_gated_ffn_desc* d, const void* dy, const void* x, const void* w_gate_up, const void* w_down,
                       int grad_dtype, void* dx, void* dw_gate_up, void* dw_down, void* scratch, size_t scratch_bytes, void* stream);

@@ -91,8 +91,9 @@ _SIGNATURES = {
     "srt_quantize_rows_e4m3": (None, [_i, _vp, _vp, _vp, _i64, _i, _vp]),
     "srt_rmsnorm_bwd_scratch_bytes": (_sz, [_i]),
     "srt_rmsnorm_bwd": (None, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp, _sz, _vp]),
-    "srt_gated_ffn_fwd": (None, [_PF, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "srt_gated_ffn_fwd_e4m3": (None, [_PF, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "srt_gated_ffn_fwd_scratch_bytes": (_sz, [_PF]),
+    "srt_gated_ffn_fwd": (None, [_PF, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "srt_gated_ffn_fwd_e4m3": (None, [_PF, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "srt_gated_ffn_bwd_scratch_bytes": (_sz, [_PF, _i]),
     "srt_gated_ffn_bwd": (None, [_PF, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "srt_grad_accumulate": (None, [_vp, _vp, _i64, _vp]),

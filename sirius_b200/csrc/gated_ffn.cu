@@ -15,9 +15,10 @@
 // leaves is act and, in backward, dgate and dup, which the plain products of the block read.
 // No sum is shared between CTAs and none depends on the order in which tiles finish: a call repeats bit for bit.
 #include <cuda.h>
+#include <cuda_fp8.h>
 
+#include "balanced_gemm.cuh"
 #include "common.cuh"
-#include "conv_geom.cuh"
 #include "gated_ffn.cuh"
 #include "ops.cuh"
 #include "ptx.cuh"
@@ -25,8 +26,7 @@
 namespace srt {
 
 int* tc_status_device_ptr();  // igemm_tcgen05.cu
-// igemm_tcgen05.cu: tensor map of a row-major matrix of 1- or 2-byte elements, boxes of 128 bytes x box_rows, 128-byte swizzle
-int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_rows);
+int tmap_rows(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_cols, uint32_t box_rows);
 
 namespace {
 
@@ -359,6 +359,10 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
   }
 }
 
+int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_rows) {
+  return tmap_rows(tm, base, rows, cols, pitch, elem_bytes, 128u / (uint32_t)elem_bytes, box_rows);
+}
+
 constexpr size_t ffn_tail_bytes() { return (2 * F_MAX_STAGES + 4) * 8 + 16; }
 
 // How a call is cut. Clocks a k-block and SM are those of the operand stream out of L2 (about 50 bytes a clock and SM), which
@@ -462,9 +466,159 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   return plan.pair ? launch_ffn<true, false, false>(p, tm, st) : launch_ffn<false, false, false>(p, tm, st);
 }
 
-size_t up256(size_t v) { return (v + 255) / 256 * 256; }
-srt_conv_desc linear(int rows, int in, int out) { return {rows, 1, 1, in, out, 1, 1, 1, 0, 1, 1}; }
+// ---- a few tokens ---------------------------------------------------------------------------------------
+// Up to four tokens: the weights are read once and everything else is small, so the products are dot products of weight rows
+// on the CUDA cores, without the set-up of tensor memory and tensor maps. A warp has one hidden channel (its gate and its up
+// row), or a quarter of one output row; all its loads are in flight together. fp32 sums in a fixed order.
+constexpr int TOK_MAX = 4;
+constexpr int TOK_THREADS = 128;
 
+__device__ __forceinline__ float warp_add(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// 16 bytes of e4m3 as fp32.
+__device__ __forceinline__ void unpack_e4m3(const uint4& v, float (&f)[16]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> (16 * h)), __NV_E4M3);
+      const float2 t = __half22float2(__half2(r));
+      f[i * 4 + h * 2] = t.x;
+      f[i * 4 + h * 2 + 1] = t.y;
+    }
+}
+template <bool E4M3>
+__device__ __forceinline__ void unpack_any(const uint4& v, float (&f)[E4M3 ? 16 : 8]) {
+  if constexpr (E4M3) {
+    unpack_e4m3(v, f);
+  } else {
+    Vec16<bf16> a;
+    a.raw = v;
+    a.unpack(f);
+  }
+}
+
+template <int TT, bool E4M3>
+__global__ void __launch_bounds__(TOK_THREADS)
+token_gate_kernel(const uint4* __restrict__ x, const uint4* __restrict__ w, const float* __restrict__ x_scale,
+                  const float* __restrict__ w_scale, bf16* __restrict__ act, int vecs, int F) {
+  constexpr int V = E4M3 ? 16 : 8, U = 4;
+  pdl_enter();
+  const int lane = threadIdx.x & 31, f = (int)blockIdx.x * (TOK_THREADS / 32) + (threadIdx.x >> 5);
+  if (f >= F) return;
+  const uint4 *wg = w + (size_t)f * vecs, *wu = w + (size_t)(F + f) * vecs;
+  float g[TT], u[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) g[t] = u[t] = 0.f;
+  for (int v0 = lane; v0 < vecs; v0 += 32 * U) {
+    uint4 a[U], b[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const bool in = v0 + 32 * i < vecs;
+      a[i] = in ? __ldcs(wg + v0 + 32 * i) : make_uint4(0, 0, 0, 0);
+      b[i] = in ? __ldcs(wu + v0 + 32 * i) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (v0 + 32 * i >= vecs) break;
+      float fa[V], fb[V];
+      unpack_any<E4M3>(a[i], fa);
+      unpack_any<E4M3>(b[i], fb);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        float fx[V];
+        unpack_any<E4M3>(x[(size_t)t * vecs + v0 + 32 * i], fx);
+#pragma unroll
+        for (int e = 0; e < V; ++e) { g[t] = fmaf(fa[e], fx[e], g[t]); u[t] = fmaf(fb[e], fx[e], u[t]); }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    g[t] = warp_add(g[t]);
+    u[t] = warp_add(u[t]);
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      if (E4M3) {
+        g[t] *= x_scale[t] * w_scale[f];
+        u[t] *= x_scale[t] * w_scale[F + f];
+      }
+      act[(size_t)t * F + f] = __float2bfloat16_rn(g[t] * sigmoid_f(g[t]) * u[t]);
+    }
+  }
+}
+
+// One output row of Wd a block, a quarter of it a warp.
+template <int TT>
+__global__ void __launch_bounds__(TOK_THREADS)
+token_down_kernel(const uint4* __restrict__ act, const uint4* __restrict__ w, const bf16* __restrict__ residual, bf16* __restrict__ y,
+                  int vecs, int C) {
+  constexpr int U = 4, WARPS = TOK_THREADS / 32;
+  __shared__ float sh[WARPS][TT];
+  pdl_enter();
+  const int c = blockIdx.x;
+  const uint4* wr = w + (size_t)c * vecs;
+  float s[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) s[t] = 0.f;
+  for (int v0 = threadIdx.x; v0 < vecs; v0 += TOK_THREADS * U) {
+    uint4 a[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) a[i] = v0 + TOK_THREADS * i < vecs ? __ldcs(wr + v0 + TOK_THREADS * i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (v0 + TOK_THREADS * i >= vecs) break;
+      float fa[8];
+      unpack_any<false>(a[i], fa);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        float fx[8];
+        unpack_any<false>(act[(size_t)t * vecs + v0 + TOK_THREADS * i], fx);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[t] = fmaf(fa[e], fx[e], s[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    s[t] = warp_add(s[t]);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5][t] = s[t];
+  }
+  __syncthreads();
+  if (threadIdx.x < TT) {
+    const int t = threadIdx.x;
+    float r = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) r += sh[k][t];
+    if (residual) r += __bfloat162float(residual[(size_t)t * C + c]);
+    y[(size_t)t * C + c] = __float2bfloat16_rn(r);
+  }
+}
+
+template <int TT>
+int token_ffn(const srt_gated_ffn_desc& d, const void* x, const float* x_scale, const void* w_gu, const float* w_scale, const void* w_down,
+              const void* residual, void* act, void* y, cudaStream_t st) {
+  const dim3 grid(ceil_div(d.hidden, TOK_THREADS / 32));
+  if (x_scale)
+    SRT_CHECK_CUDA(launch_pdl(token_gate_kernel<TT, true>, grid, dim3(TOK_THREADS), 0, st, (const uint4*)x, (const uint4*)w_gu, x_scale, w_scale,
+                              (bf16*)act, d.width / 16, d.hidden));
+  else
+    SRT_CHECK_CUDA(launch_pdl(token_gate_kernel<TT, false>, grid, dim3(TOK_THREADS), 0, st, (const uint4*)x, (const uint4*)w_gu, x_scale, w_scale,
+                              (bf16*)act, d.width / 8, d.hidden));
+  SRT_LAUNCH_CHECK();
+  SRT_CHECK_CUDA(launch_pdl(token_down_kernel<TT>, dim3(d.width), dim3(TOK_THREADS), 0, st, (const uint4*)act, (const uint4*)w_down,
+                            (const bf16*)residual, (bf16*)y, d.hidden / 8, d.width));
+  SRT_LAUNCH_CHECK();
+  return SRT_OK;
+}
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 int check_ffn(const srt_gated_ffn_desc* d, int width_unit) {
   SRT_REQUIRE(d, "gated_ffn: null descriptor");
   SRT_REQUIRE(d->tokens >= 0 && d->width > 0 && d->hidden > 0, "gated_ffn: sizes %d, %d, %d out of range", d->tokens, d->width, d->hidden);
@@ -481,37 +635,45 @@ int ffn_aligned(std::initializer_list<const void*> ps) {
   return SRT_OK;
 }
 
-// y = residual + act Wd^T
-int down_product(const srt_gated_ffn_desc& d, const void* act, const void* w_down, const void* residual, void* y, cudaStream_t st) {
-  return conv_fprop_infer(linear(d.tokens, d.hidden, d.width), SRT_BF16, SRT_IMPL_AUTO, act, w_down, y, {nullptr, nullptr, residual, ACT_NONE}, st);
-}
+// The plain products around the gated one.
+GemmProblem down_problem(const srt_gated_ffn_desc& d) { return {d.tokens, d.width, d.hidden, false, false, SRT_BF16}; }        // y
+GemmProblem dx_problem(const srt_gated_ffn_desc& d) { return {d.tokens, d.width, 2 * d.hidden, false, true, SRT_BF16}; }
+GemmProblem dw_problem(const srt_gated_ffn_desc& d, int type) { return {2 * d.hidden, d.width, d.tokens, true, true, type}; }  // dWg over dWu
+GemmProblem dd_problem(const srt_gated_ffn_desc& d, int type) { return {d.width, d.hidden, d.tokens, true, true, type}; }      // dWd
+size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
 }  // namespace
 
+size_t gated_ffn_fwd_scratch_bytes(const srt_gated_ffn_desc& d) {
+  return up256((size_t)d.tokens * d.hidden * 2) + balanced_gemm_scratch_bytes(down_problem(d));
+}
+
 int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gu, const float* w_scale,
-                  const void* w_down, const void* residual, void* act, void* y, bool e4m3, cudaStream_t st) {
+                  const void* w_down, const void* residual, void* y, void* scratch, size_t scratch_bytes, bool e4m3, cudaStream_t st) {
   int rc = check_ffn(d, e4m3 ? 16 : 8);
   if (rc || d->tokens == 0) return rc;
-  SRT_REQUIRE(x && w_gu && w_down && act && y && (!e4m3 || (x_scale && w_scale)), "gated_ffn_fwd: null operand");
-  if ((rc = FFN_ALIGNED(x, w_gu, w_down, residual, act, y))) return rc;
+  SRT_REQUIRE(x && w_gu && w_down && y && (!e4m3 || (x_scale && w_scale)), "gated_ffn_fwd: null operand");
+  const size_t act_bytes = up256((size_t)d->tokens * d->hidden * 2);
+  SRT_REQUIRE(scratch && scratch_bytes >= act_bytes, "gated_ffn_fwd: scratch too small (%zu < %zu)", scratch_bytes, act_bytes);
+  if ((rc = FFN_ALIGNED(x, w_gu, w_down, residual, y, scratch))) return rc;
+  void* act = scratch;
+  switch (d->tokens) {
+    case 1: return token_ffn<1>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
+    case 2: return token_ffn<2>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
+    case 3: return token_ffn<3>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
+    case TOK_MAX: return token_ffn<TOK_MAX>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
+  }
   if ((rc = gated_products(*d, x, x_scale, w_gu, w_scale, nullptr, nullptr, act, nullptr, st))) return rc;
-  return down_product(*d, act, w_down, residual, y, st);
+  return balanced_gemm(down_problem(*d), act, w_down, residual, y, (char*)scratch + act_bytes, scratch_bytes - act_bytes, st);
 }
 
 GatedFfnScratch gated_ffn_scratch(const srt_gated_ffn_desc& d, int grad_dtype) {
   GatedFfnScratch s;
-  const size_t TF = (size_t)d.tokens * d.hidden, CF = (size_t)d.width * d.hidden;
+  const size_t TF = (size_t)d.tokens * d.hidden;
   s.dgu = up256(TF * 2);
-  s.grad = s.dgu + up256(TF * 4);
-  s.wgrad = s.grad + (grad_dtype == SRT_BF16 ? up256(CF * 8) : 0);  // the larger of the two gradients before it is rounded
-  size_t w = 0;
-  if (d.tokens > 0) {
-    const size_t a = conv_wgrad_scratch_bytes(linear(d.tokens, d.width, 2 * d.hidden), SRT_BF16, SRT_IMPL_AUTO);
-    const size_t b = conv_wgrad_scratch_bytes(linear(d.tokens, d.hidden, d.width), SRT_BF16, SRT_IMPL_AUTO);
-    w = a > b ? a : b;
-  }
-  s.wgrad_bytes = w;
-  s.total = s.wgrad + up256(w);
+  s.slots = s.dgu + up256(TF * 4);
+  s.total = s.slots + larger(balanced_gemm_scratch_bytes(dx_problem(d)),
+                             larger(balanced_gemm_scratch_bytes(dw_problem(d, grad_dtype)), balanced_gemm_scratch_bytes(dd_problem(d, grad_dtype))));
   return s;
 }
 
@@ -520,28 +682,23 @@ int gated_ffn_bwd(const srt_gated_ffn_desc* d, const void* dy, const void* x, co
   int rc = check_ffn(d, 8);
   if (rc) return rc;
   SRT_REQUIRE(grad_dtype == SRT_F32 || grad_dtype == SRT_BF16, "gated_ffn_bwd: gradient type %d is neither SRT_F32 nor SRT_BF16", grad_dtype);
-  const int T = d->tokens, C = d->width, F = d->hidden;
-  const size_t CF = (size_t)C * F, gsz = grad_dtype == SRT_F32 ? 4 : 2;
-  if (T == 0) {
+  const size_t CF = (size_t)d->width * d->hidden, gsz = grad_dtype == SRT_F32 ? 4 : 2;
+  if (d->tokens == 0) {
     if (dw_gu) SRT_CHECK_CUDA(cudaMemsetAsync(dw_gu, 0, 2 * CF * gsz, st));
     if (dw_down) SRT_CHECK_CUDA(cudaMemsetAsync(dw_down, 0, CF * gsz, st));
     return SRT_OK;
   }
   SRT_REQUIRE(dy && x && w_gu && w_down, "gated_ffn_bwd: null operand");
   const GatedFfnScratch s = gated_ffn_scratch(*d, grad_dtype);
-  SRT_REQUIRE(scratch && scratch_bytes >= s.total, "gated_ffn_bwd: scratch too small (%zu < %zu)", scratch_bytes, s.total);
+  SRT_REQUIRE(scratch && scratch_bytes >= s.slots, "gated_ffn_bwd: scratch too small (%zu < %zu)", scratch_bytes, s.total);
   if ((rc = FFN_ALIGNED(dy, x, w_gu, w_down, dx, dw_gu, dw_down, scratch))) return rc;
   char* base = (char*)scratch;
-  void *act = base, *dgu = base + s.dgu, *wscratch = base + s.wgrad;
+  void *act = base, *dgu = base + s.dgu, *slots = base + s.slots;
+  const size_t room = scratch_bytes - s.slots;
   if ((rc = gated_products(*d, x, nullptr, w_gu, nullptr, dy, w_down, act, dgu, st))) return rc;
-  if (dx && (rc = conv_dgrad_direct(linear(T, C, 2 * F), SRT_BF16, SRT_IMPL_AUTO, dgu, w_gu, dx, nullptr, st))) return rc;
-  auto weights = [&](const srt_conv_desc& c, const void* g, const void* in, void* out, size_t n) -> int {
-    float* f = grad_dtype == SRT_F32 ? (float*)out : (float*)(base + s.grad);
-    int r = conv_wgrad(c, SRT_BF16, SRT_IMPL_AUTO, g, in, f, wscratch, s.wgrad_bytes, st);
-    return r || grad_dtype == SRT_F32 ? r : cast_f32_to_bf16(f, out, (int64_t)n, st);
-  };
-  if (dw_gu && (rc = weights(linear(T, C, 2 * F), dgu, x, dw_gu, 2 * CF))) return rc;
-  if (dw_down && (rc = weights(linear(T, F, C), dy, act, dw_down, CF))) return rc;
+  if (dx && (rc = balanced_gemm(dx_problem(*d), dgu, w_gu, nullptr, dx, slots, room, st))) return rc;
+  if (dw_gu && (rc = balanced_gemm(dw_problem(*d, grad_dtype), dgu, x, nullptr, dw_gu, slots, room, st))) return rc;
+  if (dw_down && (rc = balanced_gemm(dd_problem(*d, grad_dtype), dy, act, nullptr, dw_down, slots, room, st))) return rc;
   return SRT_OK;
 }
 
@@ -551,14 +708,17 @@ using namespace srt;
 
 extern "C" {
 
+size_t srt_gated_ffn_fwd_scratch_bytes(const srt_gated_ffn_desc* d) { return check_ffn(d, 8) ? 0 : gated_ffn_fwd_scratch_bytes(*d); }
+
 int srt_gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const void* w_gate_up, const void* w_down, const void* residual,
-                      void* act, void* y, void* stream) {
-  return gated_ffn_fwd(d, x, nullptr, w_gate_up, nullptr, w_down, residual, act, y, false, (cudaStream_t)stream);
+                      void* y, void* scratch, size_t scratch_bytes, void* stream) {
+  return gated_ffn_fwd(d, x, nullptr, w_gate_up, nullptr, w_down, residual, y, scratch, scratch_bytes, false, (cudaStream_t)stream);
 }
 
 int srt_gated_ffn_fwd_e4m3(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gate_up,
-                           const float* w_scale, const void* w_down, const void* residual, void* act, void* y, void* stream) {
-  return gated_ffn_fwd(d, x, x_scale, w_gate_up, w_scale, w_down, residual, act, y, true, (cudaStream_t)stream);
+                           const float* w_scale, const void* w_down, const void* residual, void* y, void* scratch, size_t scratch_bytes,
+                           void* stream) {
+  return gated_ffn_fwd(d, x, x_scale, w_gate_up, w_scale, w_down, residual, y, scratch, scratch_bytes, true, (cudaStream_t)stream);
 }
 
 size_t srt_gated_ffn_bwd_scratch_bytes(const srt_gated_ffn_desc* d, int grad_dtype) {

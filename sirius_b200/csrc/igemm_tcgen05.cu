@@ -1744,8 +1744,9 @@ int tmap_batched_bf16(CUtensorMap* tm, const void* base, uint64_t kdim, uint64_t
   return make_tmap_4d(tm, base, kdim, rows, z1, z2, ld, s1, s2, box_rows);
 }
 
-// Row-major matrix of 1- or 2-byte elements, rows `pitch` elements apart, boxes of 128 bytes x box_rows, 128B swizzle.
-int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_rows) {
+// Row-major matrix of 1-byte, bf16 or fp32 elements, rows `pitch` elements apart. Boxes of 64 or 128 bytes x box_rows, swizzled
+// over that width.
+int tmap_rows(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_cols, uint32_t box_rows) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
@@ -1754,10 +1755,13 @@ int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t co
   SRT_REQUIRE(((uintptr_t)base & 15) == 0 && pitch * elem_bytes % 16 == 0, "TMA operand must be 16-byte aligned with a 16-byte multiple row pitch");
   cuuint64_t dims[2] = {cols, rows};
   cuuint64_t strides[1] = {pitch * elem_bytes};
-  cuuint32_t box[2] = {128u / (uint32_t)elem_bytes, box_rows};
+  cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(tm, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
-                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+  const CUtensorMapDataType type = elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  CUresult r = fn(tm, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_cols * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);

@@ -375,9 +375,10 @@ def gated_ffn(x, w_gate_up, w_down, residual=None):
     """residual + (silu(x Wg^T) * (x Wu^T)) Wd^T with w_gate_up = Wg over Wu; bf16."""
     dev, d = _ffn("gated_ffn", x, w_gate_up, w_down, torch.bfloat16)
     _check("gated_ffn", x.shape, torch.bfloat16, dev, residual=residual)
-    act = torch.empty((d.tokens, d.hidden), dtype=torch.bfloat16, device=dev)
+    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(C.byref(d))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     y = torch.empty_like(x)
-    call("srt_gated_ffn_fwd", C.byref(d), _p(x), _p(w_gate_up), _p(w_down), _p(residual), _p(act), _p(y), _stream())
+    call("srt_gated_ffn_fwd", C.byref(d), _p(x), _p(w_gate_up), _p(w_down), _p(residual), _p(y), _p(scratch), nbytes, _stream())
     return y
 
 
@@ -387,10 +388,11 @@ def gated_ffn_e4m3(x, x_scale, w_gate_up, w_scale, w_down, residual=None):
     _check("gated_ffn_e4m3", (d.tokens,), torch.float32, dev, x_scale=x_scale)
     _check("gated_ffn_e4m3", (2 * d.hidden,), torch.float32, dev, w_scale=w_scale)
     _check("gated_ffn_e4m3", x.shape, torch.bfloat16, dev, residual=residual)
-    act = torch.empty((d.tokens, d.hidden), dtype=torch.bfloat16, device=dev)
+    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(C.byref(d))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
-    call("srt_gated_ffn_fwd_e4m3", C.byref(d), _p(x), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(w_down), _p(residual), _p(act), _p(y),
-         _stream())
+    call("srt_gated_ffn_fwd_e4m3", C.byref(d), _p(x), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(w_down), _p(residual), _p(y), _p(scratch),
+         nbytes, _stream())
     return y
 
 

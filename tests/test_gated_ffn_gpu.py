@@ -17,7 +17,7 @@ S = 2.0 ** -18      # sigmoid in fp32
 
 # tokens, width, hidden: one token; tiles not filled and filled to the last row; widths below and beyond a k-block; hidden
 # channels below a tile, odd multiples of eight, several tiles; pairs of CTAs from about a thousand tokens on
-SIZES = [(1, 896, 4864), (1, 8, 8), (2, 64, 24), (7, 72, 40), (8, 128, 136), (24, 1040, 2008), (127, 64, 64), (128, 96, 512), (129, 136, 1032),
+SIZES = [(1, 896, 4864), (1, 8, 8), (2, 64, 24), (3, 1544, 1032), (4, 40, 4104), (5, 72, 264), (7, 72, 40), (8, 128, 136), (24, 1040, 2008), (127, 64, 64), (128, 96, 512), (129, 136, 1032),
          (255, 200, 72), (333, 896, 1064), (1000, 264, 1096), (1024, 896, 2432), (2049, 136, 4872), (4100, 64, 1160)]
 
 
@@ -114,7 +114,7 @@ def test_backward_against_differences():
         assert (got[k].double() * d).sum().sub(slope).abs() <= bound
 
 
-@pytest.mark.parametrize("t,c,f", [(1, 4096, 1016), (1, 16, 8), (9, 144, 40), (24, 1040, 2008), (130, 272, 520), (333, 896, 1064), (2049, 144, 4872)])
+@pytest.mark.parametrize("t,c,f", [(1, 4096, 1016), (1, 16, 8), (2, 1040, 520), (3, 32, 72), (4, 528, 1000), (5, 528, 1000), (9, 144, 40), (24, 1040, 2008), (130, 272, 520), (333, 896, 1064), (2049, 144, 4872)])
 def test_e4m3(t, c, f):
     s = make(t, c, f)
     xq, xs = ops.quantize_rows_e4m3(s["x"])
@@ -158,18 +158,21 @@ def test_no_tokens():
 
 @pytest.mark.parametrize("t,c,f", [(9, 72, 40), (700, 136, 1032), (1100, 264, 2056)])
 def test_rows_beyond_the_outputs_stay(t, c, f):
-    """act, y and the gradients as slices of larger buffers: the rows behind them are left as they were."""
+    """y and the gradients as slices of larger buffers: the rows behind them are left as they were."""
     s = make(t, c, f)
     d = _lib.GatedFfnDesc(t, c, f)
     st = torch.cuda.current_stream().cuda_stream
-    act, y = torch.full((t + 3, f), 7.0, device="cuda", dtype=BF), torch.full((t + 3, c), 7.0, device="cuda", dtype=BF)
-    _lib.call("srt_gated_ffn_fwd", C.byref(d), s["x"].data_ptr(), s["wgu"].data_ptr(), s["wd"].data_ptr(), None, act.data_ptr(), y.data_ptr(), st)
+    y = torch.full((t + 3, c), 7.0, device="cuda", dtype=BF)
+    n = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(C.byref(d))
+    scratch = torch.full((n + 512,), 77, dtype=torch.uint8, device="cuda")
+    _lib.call("srt_gated_ffn_fwd", C.byref(d), s["x"].data_ptr(), s["wgu"].data_ptr(), s["wd"].data_ptr(), None, y.data_ptr(), scratch.data_ptr(), n, st)
+    assert (scratch[n:] == 77).all()
     dx, dw, dd = (torch.full((n + 3, w), 7.0, device="cuda", dtype=BF) for n, w in ((t, c), (2 * f, c), (c, f)))
     n = _lib.lib().srt_gated_ffn_bwd_scratch_bytes(C.byref(d), _lib.SRT_BF16)
     scratch = torch.full((n + 512,), 77, dtype=torch.uint8, device="cuda")
     _lib.call("srt_gated_ffn_bwd", C.byref(d), s["dy"].data_ptr(), s["x"].data_ptr(), s["wgu"].data_ptr(), s["wd"].data_ptr(), _lib.SRT_BF16, dx.data_ptr(),
               dw.data_ptr(), dd.data_ptr(), scratch.data_ptr(), n, st)
-    for whole, rows, want in ((act, t, None), (y, t, ops.gated_ffn(s["x"], s["wgu"], s["wd"])), (dx, t, None), (dw, 2 * f, None), (dd, c, None)):
+    for whole, rows, want in ((y, t, ops.gated_ffn(s["x"], s["wgu"], s["wd"])), (dx, t, None), (dw, 2 * f, None), (dd, c, None)):
         assert (whole[rows:] == 7.0).all() and not (whole[:rows] == 7.0).all()
         if want is not None:
             assert torch.equal(whole[:rows], want)
