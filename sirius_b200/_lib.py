@@ -82,8 +82,8 @@ _SIGNATURES = {
     "srt_sgd_momentum": (None, [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _i, _vp]),
     "srt_adamw": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _i, _vp]),
     "srt_grad_norm_scratch_bytes": (_sz, [_i]),
-    "srt_grad_norm": (None, [_i, _i, C.POINTER(_vp), C.POINTER(_i64), _f, _vp, _vp, _sz, _vp]),
-    "srt_clip_grad_norm": (None, [_i, _i, C.POINTER(_vp), C.POINTER(_i64), _f, _vp, _vp, _sz, _vp]),
+    "srt_grad_norm": (None, [_i, _i, _vp, _vp, _f, _vp, _vp, _sz, _vp]),
+    "srt_clip_grad_norm": (None, [_i, _i, _vp, _vp, _f, _vp, _vp, _sz, _vp]),
     "srt_adamw_clipped": (None, [_vp, _vp, _vp, _vp, _vp, _i64, _d, _d, _d, _d, _d, _i, _vp, _vp]),
     "srt_sgd_momentum_clipped": (None, [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _i, _vp, _vp]),
     "srt_rmsnorm_fwd": (None, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _f, _vp]),

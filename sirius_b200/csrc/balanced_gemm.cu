@@ -6,7 +6,7 @@
 // slots of every such tile in the order of the reduction. So 152 tiles on 74 pairs take 2.05 rounds and not three, a few rows
 // against a long reduction occupy the device, no CTA waits for another, and the sums have a fixed order.
 //
-// Warps as in the gated kernels: 0 TMA, 1 MMA, 2-9 two epilogue groups that take the 32-column slabs of a tile in turn. The
+// Warps as in the gated kernels: 0 TMA, 1 MMA, 2-17 four epilogue groups that take the 32-column slabs of a tile in turn. The
 // accumulator is double-buffered in tensor memory, so the epilogue of a tile runs beside the products of the next.
 #include <cuda.h>
 
@@ -24,10 +24,11 @@ using namespace ptx;
 using bf16 = __nv_bfloat16;
 
 constexpr int BM = 128;
-constexpr int G_THREADS = 320;
+constexpr int EPI_GROUPS = 4;                     // of four warps
+constexpr int G_THREADS = 64 + 128 * EPI_GROUPS;
 constexpr int G_MAX_STAGES = 8;
 constexpr int A_BYTES = BM * 128;
-constexpr int SLAB_BYTES = BM * 128;  // 128 rows x 32 fp32 (or 32 bf16)
+constexpr int SLAB_BYTES = BM * 64;  // 128 rows x 32 bf16 or 16 fp32, 64-byte swizzle
 enum { W_GEMM_LOAD = 0x41, W_GEMM_FULL = 0x42, W_GEMM_ACC = 0x43, W_GEMM_EPI = 0x44, W_GEMM_DRAIN = 0x45 };
 
 struct GemmParams {
@@ -39,6 +40,7 @@ struct GemmParams {
   int stages, stage_bytes;
   uint32_t load_bytes;         // of one CTA a k-block
   int f32_out;
+  int b_early;                 // B may be read before the launch in front of this one has ended
   const bf16* addend;
   void* D;
   const float* slots;          // [2 sharers][rows of a unit][n]
@@ -75,9 +77,9 @@ __device__ __forceinline__ bool walk_next(const GemmParams& p, int unit, Walk& w
   w.at = stop;
   return true;
 }
-__device__ __forceinline__ void tile_at(const GemmParams& p, int t, int& m, int& n) {
+__host__ __device__ inline void tile_at(const GemmParams& p, int t, int& m, int& n) {
   const int b = t / (p.band * p.m_units), first = b * p.band;
-  const int size = min(p.band, p.n_tiles - first), r = t - first * p.m_units;
+  const int size = p.n_tiles - first < p.band ? p.n_tiles - first : p.band, r = t - first * p.m_units;
   m = r / size;
   n = first + r - m * size;
 }
@@ -91,7 +93,7 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int NS = p.stages;
   uint8_t* sOut = base + NS * p.stage_bytes;
-  uint64_t* bars = (uint64_t*)(sOut + 2 * SLAB_BYTES);
+  uint64_t* bars = (uint64_t*)(sOut + EPI_GROUPS * SLAB_BYTES);
   const uint32_t full = smem_u32(bars), empty = full + 8 * G_MAX_STAGES, acc_full = empty + 8 * G_MAX_STAGES, acc_empty = acc_full + 16;
   uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * G_MAX_STAGES + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -102,7 +104,7 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + 8 * b, 1); mbar_init(acc_empty + 8 * b, 8 * NCTA); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + 8 * b, 1); mbar_init(acc_empty + 8 * b, 4 * EPI_GROUPS * NCTA); }
     mbar_fence_init();
   }
   if (warp == 0 && lane == 0) { tma_prefetch_desc(&ta); tma_prefetch_desc(&tb); tma_prefetch_desc(&td); }
@@ -115,42 +117,86 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
   if (PAIR) cluster_sync_all();  // the peer's barriers and tensor memory exist before anything refers to them
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_ptr;
-  pdl_enter();
+  // The B tiles of the first stages of a producer that may fetch them ahead of the launch in front: they travel while that one
+  // drains.
+  const bool ahead = p.b_early && warp == 0;
+  if (!ahead) pdl_enter();
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0, s = 0;
-      uint32_t ph = 1;
+      // One thread feeds the ring, and a k-block takes it a few hundred clocks: what does not change from one to the next
+      // stays out of the loops.
+      const uint32_t bytes = p.load_bytes * NCTA, full_to = PAIR ? map_to_cta(full, 0u) : full;  // the leader's barriers
+      const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
+      int it = 0, early = 0;
+      uint32_t at = 0, bar = 0, ph = 1;  // offsets of the current stage and of its barriers
       bool ok = true;
+      auto step = [&]() {
+        at += p.stage_bytes;
+        bar += 8;
+        if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
+      };
+      auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
+        if (PAIR) tma_load_2d_pair(dst, tm, full_to + bar, x, y);
+        else tma_load_2d(dst, tm, full_to + bar, x, y);
+      };
+      auto load_a = [&](int m0, int k0) {
+        const uint32_t a = s0 + at;
+        if (A_MN) {
+          load(a, &ta, m0, k0);
+          load(a + 8192u, &ta, m0 + 64, k0);
+        } else {
+          load(a, &ta, k0, m0);
+        }
+      };
+      auto load_b = [&](int n0, int k0) {
+        const uint32_t b = s0 + at + A_BYTES;
+        if (B_MN) {
+          load(b, &tb, n0, k0);
+          if (n_cta > 64) load(b + 8192u, &tb, n0 + 64, k0);
+          if (!PAIR && n_cta > 128) {
+            load(b + 16384u, &tb, n0 + 128, k0);
+            if (n_cta > 192) load(b + 24576u, &tb, n0 + 192, k0);
+          }
+        } else {
+          load(b, &tb, k0, n0);
+        }
+      };
+      if (ahead) {
+        Walk w = walk_begin(p, unit);
+        Piece o;
+        while (early < NS && walk_next(p, unit, w, o)) {
+          int m, n;
+          tile_at(p, o.tile, m, n);
+          for (int kb = o.k0; kb < o.k1 && early < NS; ++kb, ++early) {
+            if (rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
+            load_b(n * p.n + (int)rank * n_cta, kb * 64);
+            step();
+          }
+        }
+        pdl_enter();
+        at = bar = 0;
+        ph = 1;
+      }
       Walk w = walk_begin(p, unit);
       Piece o;
       while (ok && walk_next(p, unit, w, o)) {
         int m, n;
         tile_at(p, o.tile, m, n);
         const int m0 = (m * NCTA + (int)rank) * BM, n0 = n * p.n + (int)rank * n_cta;
-        for (int kb = o.k0; kb < o.k1; ++kb) {
-          ok = mbar_wait(empty + 8 * s, ph, p.status, W_GEMM_LOAD);
+        int k0 = o.k0 * 64;
+        const int k1 = o.k1 * 64;
+        for (; it < early && k0 < k1; k0 += 64, ++it) {
+          load_a(m0, k0);
+          step();
+        }
+        for (; k0 < k1; k0 += 64, ++it) {
+          ok = mbar_wait(empty + bar, ph, p.status, W_GEMM_LOAD);
           if (!ok) break;
-          if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, p.load_bytes * NCTA);
-          const uint32_t bar = PAIR ? map_to_cta(full + 8 * s, 0u) : full + 8 * s;
-          const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + A_BYTES;
-          auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
-            if (PAIR) tma_load_2d_pair(dst, tm, bar, x, y);
-            else tma_load_2d(dst, tm, bar, x, y);
-          };
-          if (A_MN) {
-            load(a, &ta, m0, kb * 64);
-            load(a + 8192u, &ta, m0 + 64, kb * 64);
-          } else {
-            load(a, &ta, kb * 64, m0);
-          }
-          if (B_MN) {
-            for (int c = 0; c < n_cta; c += 64) load(b + (uint32_t)c * 128u, &tb, n0 + c, kb * 64);
-          } else {
-            load(b, &tb, kb * 64, n0);
-          }
-          ++it;
-          if (++s == NS) { s = 0; ph ^= 1u; }
+          if (rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
+          load_a(m0, k0);
+          load_b(n0, k0);
+          step();
         }
       }
       // a wait that gave up: the copies in flight land before the CTA's memory is given back
@@ -160,11 +206,14 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = make_idesc_bf16(BM * NCTA, p.n, A_MN, B_MN);
-      int s = 0, i = 0;
-      uint32_t ph = 0;
+      constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;  // 16 elements along the reduction
+      const uint64_t desc_a = make_smem_desc_sw128(s0, A_MN ? 8192 : 0, 1024), desc_b = make_smem_desc_sw128(s0 + A_BYTES, B_MN ? 8192 : 0, 1024);
+      const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
+      int i = 0;
+      uint32_t at = 0, bar = 0, ph = 0;
       bool ok = true;
-      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-        ok = ok && (PAIR ? mbar_wait_cluster(bar, parity, p.status, code) : mbar_wait(bar, parity, p.status, code));
+      auto wait = [&](uint32_t b, uint32_t parity, int code) {
+        ok = ok && (PAIR ? mbar_wait_cluster(b, parity, p.status, code) : mbar_wait(b, parity, p.status, code));
         if (ok) tc_fence_after_sync();
         return ok;
       };
@@ -173,20 +222,21 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
       for (; ok && walk_next(p, unit, w, o); ++i) {
         const uint32_t b2 = (uint32_t)i & 1u, acc = tmem + b2 * (uint32_t)(p.cols / 2);
         if (!wait(acc_empty + 8 * b2, ((uint32_t)(i >> 1) & 1u) ^ 1u, W_GEMM_ACC)) break;
+        uint32_t add = 0;
         for (int kb = o.k0; kb < o.k1; ++kb) {
-          if (!wait(full + 8 * s, ph, W_GEMM_FULL)) break;
-          const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + A_BYTES;
+          if (!wait(full + bar, ph, W_GEMM_FULL)) break;
+          const uint64_t ad = desc_at(desc_a, at), bd = desc_at(desc_b, at);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = A_MN ? make_smem_desc_sw128(a + k * 2048, 8192, 1024) : make_smem_desc_sw128(a + k * 32, 0, 1024);
-            const uint64_t bd = B_MN ? make_smem_desc_sw128(b + k * 2048, 8192, 1024) : make_smem_desc_sw128(b + k * 32, 0, 1024);
-            const uint32_t add = (kb != o.k0 || k != 0) ? 1u : 0u;
-            if (PAIR) umma_bf16_pair(acc, ad, bd, idesc, add);
-            else umma_bf16(acc, ad, bd, idesc, add);
+            if (PAIR) umma_bf16_pair(acc, desc_at(ad, k * a_step), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+            else umma_bf16(acc, desc_at(ad, k * a_step), desc_at(bd, k * b_step), idesc, k ? 1u : add);
           }
-          if (PAIR) umma_commit_pair(empty + 8 * s, (uint16_t)3);
-          else umma_commit(empty + 8 * s);
-          if (++s == NS) { s = 0; ph ^= 1u; }
+          add = 1;
+          if (PAIR) umma_commit_pair(empty + bar, (uint16_t)3);
+          else umma_commit(empty + bar);
+          at += p.stage_bytes;
+          bar += 8;
+          if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
         }
         if (!ok) break;
         if (PAIR) umma_commit_pair(acc_full + 8 * b2, (uint16_t)3);
@@ -220,7 +270,7 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
       fetch(grp * 32);
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * b2, (uint32_t)(i >> 1) & 1u, p.status, W_GEMM_EPI));
       tc_fence_after_sync();
-      for (int c = grp * 32; c < p.n; c += 64) {
+      for (int c = grp * 32; c < p.n; c += 32 * EPI_GROUPS) {
         if (m0 >= p.M || n0 + c >= p.N) break;  // the same for the whole group; nothing of the slab exists
         uint32_t f[32];
         tmem_ld_32x32b_x32(acc + (uint32_t)c, f);
@@ -233,31 +283,32 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[v * 8 + e] = __float_as_uint(__uint_as_float(f[v * 8 + e]) + a[e]);
           }
-          fetch(c + 64);
+          fetch(c + 32 * EPI_GROUPS);
         }
-        if (issuer) bulk_wait_group_read<0>();  // the store before has read the slab
-        named_bar_sync(1 + grp, 128);
-        if (wide) {
+        // 64 bytes of every row at a time: all 32 columns in bf16, 16 of them in fp32
 #pragma unroll
-          for (int v = 0; v < 8; ++v)
-            st_shared_v4(slab + (uint32_t)row * 128u + (uint32_t)((v ^ (row & 7)) << 4), f[v * 4], f[v * 4 + 1], f[v * 4 + 2], f[v * 4 + 3]);
-        } else {
-          uint32_t h[16];
+        for (int h = 0; h < 2; ++h) {
+          if (!wide) {
+            if (h == 1) break;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(f[2 * e]), __uint_as_float(f[2 * e + 1]));
-            h[e] = *reinterpret_cast<uint32_t*>(&v);
+            for (int e = 0; e < 16; ++e) {
+              __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(f[2 * e]), __uint_as_float(f[2 * e + 1]));
+              f[e] = *reinterpret_cast<uint32_t*>(&v);
+            }
           }
+          if (issuer) bulk_wait_group_read<0>();  // the store before has read the slab
+          named_bar_sync(1 + grp, 128);
 #pragma unroll
-          for (int v = 0; v < 4; ++v)  // 64-byte rows, 64-byte swizzle
-            st_shared_v4(slab + (uint32_t)row * 64u + (uint32_t)((v ^ ((row >> 1) & 3)) << 4), h[v * 4], h[v * 4 + 1], h[v * 4 + 2], h[v * 4 + 3]);
-        }
-        fence_proxy_async_smem();
-        named_bar_sync(1 + grp, 128);
-        if (issuer) {
-          if (whole) tma_store_2d(&td, slab, n0 + c, m0);
-          else tma_store_2d(&tslot, slab, c, (o.slot * NCTA + (int)rank) * BM);
-          bulk_commit_group();
+          for (int v = 0; v < 4; ++v)
+            st_shared_v4(slab + (uint32_t)row * 64u + (uint32_t)((v ^ ((row >> 1) & 3)) << 4), f[h * 16 + v * 4], f[h * 16 + v * 4 + 1],
+                         f[h * 16 + v * 4 + 2], f[h * 16 + v * 4 + 3]);
+          fence_proxy_async_smem();
+          named_bar_sync(1 + grp, 128);
+          if (issuer) {
+            if (whole) tma_store_2d(&td, slab, n0 + c + h * 16, m0);
+            else tma_store_2d(&tslot, slab, c + h * 16, (o.slot * NCTA + (int)rank) * BM);
+            bulk_commit_group();
+          }
         }
       }
       tc_fence_before_sync();
@@ -281,53 +332,48 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
   }
 }
 
-// The tiles whose reduction was shared: block (u, y) looks at the border between the shares of units u and u + 1; the first
-// border inside a tile stands for the tile. Sixteen rows a block.
-constexpr int JOIN_ROWS = 16, JOIN_THREADS = 256;
+// The tiles whose reduction was shared, found by the host: the slots of units u0 ... u1 in the order of the reduction, plus the
+// addend. Block (tile, part of its rows), eight columns a thread; a few tiles with many slots, whose loads a sum waits for in
+// turn, take fewer rows a block.
+// (Blocks that found their tile themselves, by divisions of 64-bit numbers: 10 to 16 us for 54 tiles.)
+constexpr int JOIN_THREADS = 256, JOIN_MAX = 160;
+struct JoinList {
+  struct { int m, n, u0, u1; } t[JOIN_MAX];
+};
 __global__ void __launch_bounds__(JOIN_THREADS)
-balanced_gemm_join_kernel(const GemmParams p, int unit_rows) {
+balanced_gemm_join_kernel(const GemmParams p, const __grid_constant__ JoinList list, int unit_rows, int block_rows) {
   pdl_enter();
-  const long long work = (long long)p.rest * p.k_blocks;
-  const int u = (int)blockIdx.x + 1;
-  const long long border = share_begin(work, u, p.sharers);
-  const int t = (int)(border / p.k_blocks);
-  const long long first = (long long)t * p.k_blocks;
-  if (border == first || border >= work || share_begin(work, u - 1, p.sharers) > first) return;
-  const int u0 = u - 1, u1 = (int)(((first + p.k_blocks) * p.sharers - 1) / work);  // units with a part of the tile
-  int m, n;
-  tile_at(p, p.rounds * p.units + t, m, n);
+  const int u0 = list.t[blockIdx.x].u0, u1 = list.t[blockIdx.x].u1;
+  const int row0 = list.t[blockIdx.x].m * unit_rows, col0 = list.t[blockIdx.x].n * p.n;
   const int per_row = p.n / 8;
-  for (int i = threadIdx.x; i < JOIN_ROWS * per_row; i += JOIN_THREADS) {
-    const int r = (int)blockIdx.y * JOIN_ROWS + i / per_row, c = (i % per_row) * 8;
-    const int row = m * unit_rows + r, col = n * p.n + c;
-    if (row >= p.M || col >= p.N) continue;  // N is a multiple of eight
-    float s[8];
-    const float* f = p.slots + ((size_t)(2 * u0 + 1) * unit_rows + r) * p.n + c;
-    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(f);
-    *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(f + 4);
+  const size_t step = (size_t)2 * unit_rows * p.n;
+  for (int i = threadIdx.x; i < block_rows * per_row; i += JOIN_THREADS) {
+    const int r = (int)blockIdx.y * block_rows + i / per_row, c = (i % per_row) * 8;
+    if (row0 + r >= p.M || col0 + c >= p.N) continue;  // N is a multiple of eight
+    const size_t at = (size_t)(row0 + r) * p.N + col0 + c;
+    Vec16<bf16> add;
+    add.raw = make_uint4(0, 0, 0, 0);
+    if (p.addend) add.load(p.addend + at);
+    const float* f = p.slots + (size_t)u0 * step + (size_t)r * p.n + c;
+    float4 s0 = *reinterpret_cast<const float4*>(f + step / 2), s1 = *reinterpret_cast<const float4*>(f + step / 2 + 4);
+    f += step;
 #pragma unroll 4
-    for (int k = u0 + 1; k <= u1; ++k) {
-      const float* g = p.slots + ((size_t)(2 * k) * unit_rows + r) * p.n + c;
-      const float4 a = *reinterpret_cast<const float4*>(g), b = *reinterpret_cast<const float4*>(g + 4);
-      s[0] += a.x; s[1] += a.y; s[2] += a.z; s[3] += a.w;
-      s[4] += b.x; s[5] += b.y; s[6] += b.z; s[7] += b.w;
+    for (int k = u0 + 1; k <= u1; ++k, f += step) {
+      const float4 a = *reinterpret_cast<const float4*>(f), b = *reinterpret_cast<const float4*>(f + 4);
+      s0.x += a.x; s0.y += a.y; s0.z += a.z; s0.w += a.w;
+      s1.x += b.x; s1.y += b.y; s1.z += b.z; s1.w += b.w;
     }
-    const size_t at = (size_t)row * p.N + col;
-    if (p.addend) {
-      Vec16<bf16> v;
-      float a[8];
-      v.load(p.addend + at);
-      v.unpack(a);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += a[e];
-    }
+    float e[8];
+    add.unpack(e);
+    e[0] += s0.x; e[1] += s0.y; e[2] += s0.z; e[3] += s0.w;
+    e[4] += s1.x; e[5] += s1.y; e[6] += s1.z; e[7] += s1.w;
     if (p.f32_out) {
-      *reinterpret_cast<float4*>((float*)p.D + at) = *reinterpret_cast<float4*>(s);
-      *reinterpret_cast<float4*>((float*)p.D + at + 4) = *reinterpret_cast<float4*>(s + 4);
+      float* d = (float*)p.D + at;
+      *reinterpret_cast<float4*>(d) = make_float4(e[0], e[1], e[2], e[3]);
+      *reinterpret_cast<float4*>(d + 4) = make_float4(e[4], e[5], e[6], e[7]);
     } else {
-      Vec16<bf16> v;
-      v.pack(s);
-      v.store((bf16*)p.D + at);
+      add.pack(e);
+      add.store((bf16*)p.D + at);
     }
   }
 }
@@ -343,7 +389,7 @@ size_t plan_bytes(const GemmPlan& g) { return g.rest ? (size_t)2 * g.sharers * (
 // Plans that need more than `room` bytes of slots are left out; one without any is always there.
 GemmPlan plan_gemm(const GemmProblem& q, size_t room) {
   constexpr int LEAST = 4;  // k-blocks of a share: less is not worth a slot
-  const int sms = sm_count(), kb = ceil_div(q.K, 64);
+  const int sms = sm_count() < JOIN_MAX ? sm_count() : JOIN_MAX, kb = ceil_div(q.K, 64);
   const int a_rows = !q.a_mn && q.M < BM ? (q.M + 7) / 8 * 8 : BM;
   GemmPlan best = {};
   double best_cost = 1e30;
@@ -381,12 +427,34 @@ GemmPlan plan_gemm(const GemmProblem& q, size_t room) {
   return best;
 }
 
+// The tiles with more than one part, each with the units that have one: a border between two shares inside a tile makes it
+// such a tile, and the first border inside stands for it.
+int join_list(const GemmParams& p, JoinList& list) {
+  const long long work = (long long)p.rest * p.k_blocks;
+  int count = 0, last = -1;
+  for (int u = 1; u < p.sharers; ++u) {
+    const long long border = share_begin(work, u, p.sharers);
+    const int t = (int)(border / p.k_blocks);
+    if (border == (long long)t * p.k_blocks) continue;
+    if (t == last) {
+      list.t[count - 1].u1 = u;
+      continue;
+    }
+    last = t;
+    int m, n;
+    tile_at(p, p.rounds * p.units + t, m, n);
+    list.t[count++] = {m, n, u - 1, u};
+  }
+  return count;
+}
+
 template <bool PAIR, bool A_MN, bool B_MN>
 int launch_gemm(GemmParams& p, const GemmPlan& g, const CUtensorMap (&tm)[4], cudaStream_t st) {
-  constexpr size_t fixed = 1024 + 2 * SLAB_BYTES + (2 * G_MAX_STAGES + 4) * 8 + 16;
+  constexpr size_t fixed = 1024 + EPI_GROUPS * SLAB_BYTES + (2 * G_MAX_STAGES + 4) * 8 + 16;
   p.stages = (int)((232448 - fixed) / p.stage_bytes);
   if (p.stages > G_MAX_STAGES) p.stages = G_MAX_STAGES;
-  SRT_CHECK_CUDA(cudaFuncSetAttribute(balanced_gemm_kernel<PAIR, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+  static SmemOptIn opt_in;
+  SRT_CHECK_CUDA(opt_in.set(balanced_gemm_kernel<PAIR, A_MN, B_MN>, 232448));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(g.units * (PAIR ? 2 : 1)));
   cfg.blockDim = dim3(G_THREADS);
@@ -407,8 +475,13 @@ int launch_gemm(GemmParams& p, const GemmPlan& g, const CUtensorMap (&tm)[4], cu
   SRT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, balanced_gemm_kernel<PAIR, A_MN, B_MN>, p, tm[0], tm[1], tm[2], tm[3]));
   SRT_LAUNCH_CHECK();
   if (g.rest == 0) return SRT_OK;
+  JoinList list;
+  const int tiles = join_list(p, list);
+  if (tiles == 0) return SRT_OK;  // every share ended with a tile
   const int rows = PAIR ? 2 * BM : BM, live = p.M < rows ? p.M : rows;
-  SRT_CHECK_CUDA(launch_pdl(balanced_gemm_join_kernel, dim3(g.sharers - 1, ceil_div(live, JOIN_ROWS)), dim3(JOIN_THREADS), 0, st, p, rows));
+  int block_rows = 32;
+  while (block_rows > 2 && tiles * ceil_div(live, block_rows) < 2 * sm_count()) block_rows /= 2;
+  SRT_CHECK_CUDA(launch_pdl(balanced_gemm_join_kernel, dim3(tiles, ceil_div(live, block_rows)), dim3(JOIN_THREADS), 0, st, p, list, rows, block_rows));
   SRT_LAUNCH_CHECK();
   return SRT_OK;
 }
@@ -418,7 +491,7 @@ int launch_gemm(GemmParams& p, const GemmPlan& g, const CUtensorMap (&tm)[4], cu
 size_t balanced_gemm_scratch_bytes(const GemmProblem& q) { return q.M > 0 && q.N > 0 && q.K > 0 ? plan_bytes(plan_gemm(q, SIZE_MAX)) : 0; }
 
 int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void* addend, void* D, void* scratch, size_t scratch_bytes,
-                  cudaStream_t st) {
+                  bool b_early, cudaStream_t st) {
   SRT_REQUIRE(q.M > 0 && q.N > 0 && q.K > 0 && (q.b_mn || !q.a_mn), "balanced_gemm: empty problem or an operand order that has no kernel");
   const GemmPlan g = plan_gemm(q, scratch && ((uintptr_t)scratch & 15) == 0 ? scratch_bytes : 0);
   GemmParams p = {};
@@ -442,6 +515,7 @@ int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void
   p.load_bytes = (uint32_t)(q.a_mn ? A_BYTES : a_rows * 128) + (uint32_t)b_bytes;
   p.stage_bytes = A_BYTES + (b_bytes + 1023) / 1024 * 1024;
   p.f32_out = q.out_dtype == SRT_F32;
+  p.b_early = b_early;
   p.addend = (const bf16*)addend;
   p.D = D;
   p.slots = (const float*)scratch;
@@ -451,10 +525,10 @@ int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void
   int rc;
   if ((rc = q.a_mn ? tmap_rows(&tm[0], A, q.K, q.M, q.M, 2, 64, 64) : tmap_rows(&tm[0], A, q.M, q.K, q.K, 2, 64, a_rows)) ||
       (rc = q.b_mn ? tmap_rows(&tm[1], B, q.K, q.N, q.N, 2, 64, 64) : tmap_rows(&tm[1], B, q.N, q.K, q.K, 2, 64, nc)) ||
-      (rc = tmap_rows(&tm[2], D, q.M, q.N, q.N, p.f32_out ? 4 : 2, 32, BM)))
+      (rc = tmap_rows(&tm[2], D, q.M, q.N, q.N, p.f32_out ? 4 : 2, p.f32_out ? 16 : 32, BM)))
     return rc;
   tm[3] = tm[2];
-  if (g.rest && (rc = tmap_rows(&tm[3], scratch, (uint64_t)2 * g.sharers * (g.pair ? 2 * BM : BM), g.n, g.n, 4, 32, BM))) return rc;
+  if (g.rest && (rc = tmap_rows(&tm[3], scratch, (uint64_t)2 * g.sharers * (g.pair ? 2 * BM : BM), g.n, g.n, 4, 16, BM))) return rc;
   if (q.a_mn) return g.pair ? launch_gemm<true, true, true>(p, g, tm, st) : launch_gemm<false, true, true>(p, g, tm, st);
   if (q.b_mn) return g.pair ? launch_gemm<true, false, true>(p, g, tm, st) : launch_gemm<false, false, true>(p, g, tm, st);
   return g.pair ? launch_gemm<true, false, false>(p, g, tm, st) : launch_gemm<false, false, false>(p, g, tm, st);

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <atomic>
 #include <string>
 
 #include "../../include/sirius_b200.h"
@@ -155,6 +156,25 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
                               Args&&... args) {
   return launch_pdl_if((pdl_classes() & PDL_MISC) != 0, kernel, grid, block, smem, st, static_cast<Args&&>(args)...);
 }
+// The dynamic shared memory a kernel may be launched with, asked for once a device; one object per kernel.
+class SmemOptIn {
+ public:
+  template <typename K>
+  cudaError_t set(K kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done_.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done_.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
+
 // Kernels that hold most of an SM's shared memory (the tensor-core GEMMs) should not sit resident waiting
 // for their predecessor while another stream could use that SM; the step executor turns early launch
 // of those off while it overlaps streams.

@@ -34,10 +34,11 @@ using namespace ptx;
 using bf16 = __nv_bfloat16;
 
 constexpr int FM = 128;                  // rows of a CTA's tile (tensor-memory lanes)
-constexpr int F_THREADS = 320;           // warp 0 TMA, warp 1 MMA, warps 2-9 two epilogue groups
+constexpr int epi_groups(bool pair) { return pair ? 4 : 2; }                  // of four warps, behind the TMA and the MMA warp
+constexpr int ffn_threads(bool pair) { return 64 + 128 * epi_groups(pair); }
 constexpr int F_MAX_STAGES = 8;
 constexpr int F_A_BYTES = FM * 128;      // one 128-byte swizzle row of the reduction a tile row
-constexpr int F_SLAB_BYTES = FM * 128;   // 128 x 64 bf16 on the way out
+constexpr int F_SLAB_BYTES = FM * 64;    // 128 x 32 bf16 on the way out, 64-byte swizzle
 enum { W_FFN_LOAD = 0x31, W_FFN_FULL = 0x32, W_FFN_ACC = 0x33, W_FFN_EPI = 0x34, W_FFN_DRAIN = 0x35 };
 
 struct FfnParams {
@@ -73,7 +74,7 @@ __device__ __forceinline__ void tile_of(const FfnParams& p, int t, int& m, int& 
 // Tensor memory, in quarters of `cols`: forward two accumulators of two quarters; backward da of even tiles | gate and up |
 // da of odd tiles, so that the da product of the next tile runs beside the epilogue of the current one.
 template <bool PAIR, bool BWD, bool E4M3>
-__global__ void __launch_bounds__(F_THREADS, PAIR ? 1 : 2)
+__global__ void __launch_bounds__(ffn_threads(PAIR), PAIR ? 1 : 2)
 gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
                  const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap twd,
                  const __grid_constant__ CUtensorMap tact, const __grid_constant__ CUtensorMap tgate,
@@ -83,8 +84,8 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int NS = p.stages;
-  uint8_t* sOut = base + NS * p.stage_bytes;  // two slabs, pairs only
-  uint64_t* bars = (uint64_t*)(sOut + (PAIR ? 2 * F_SLAB_BYTES : 0));
+  uint8_t* sOut = base + NS * p.stage_bytes;  // a slab per epilogue group, pairs only
+  uint64_t* bars = (uint64_t*)(sOut + (PAIR ? epi_groups(true) * F_SLAB_BYTES : 0));
   const uint32_t full = smem_u32(bars), empty = full + 8 * F_MAX_STAGES, acc_full = empty + 8 * F_MAX_STAGES, acc_empty = acc_full + 16;
   uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * F_MAX_STAGES + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -96,7 +97,7 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + 8 * b, 1); mbar_init(acc_empty + 8 * b, 8 * NCTA); }
+    for (int b = 0; b < 2; ++b) { mbar_init(acc_full + 8 * b, 1); mbar_init(acc_empty + 8 * b, 4 * epi_groups(PAIR) * NCTA); }
     mbar_fence_init();
   }
   if (warp == 0 && lane == 0) {
@@ -117,52 +118,49 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0, s = 0;
-      uint32_t ph = 1;
+      // One thread feeds the ring, and a k-block takes it a few hundred clocks: what does not change from one to the next
+      // stays out of the loops.
+      const uint32_t full_to = PAIR ? map_to_cta(full, 0u) : full;  // the leader's barriers
+      const uint32_t wrap = (uint32_t)NS * p.stage_bytes, gu_bytes = p.gu_bytes * NCTA, da_bytes = p.da_bytes * NCTA;
+      int it = 0;
+      uint32_t at = 0, bar = 0, ph = 1;  // offsets of the current stage and of its barriers
       bool ok = true;
-      // one k-block: `a` and the B rows of this phase into stage s
-      auto next = [&](uint32_t bytes) -> uint32_t {
-        ok = ok && mbar_wait(empty + 8 * s, ph, p.status, W_FFN_LOAD);
-        if (!ok) return 0u;
-        if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, bytes * NCTA);
-        return PAIR ? map_to_cta(full + 8 * s, 0u) : full + 8 * s;
+      auto take = [&](uint32_t bytes) {
+        ok = mbar_wait(empty + bar, ph, p.status, W_FFN_LOAD);
+        if (ok && rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
+        return ok;
       };
-      auto advance = [&]() {
+      auto load = [&](uint32_t offset, const CUtensorMap* tm, int x, int y) {
+        if (PAIR) tma_load_2d_pair(s0 + at + offset, tm, full_to + bar, x, y);
+        else tma_load_2d(s0 + at + offset, tm, full_to + bar, x, y);
+      };
+      auto step = [&]() {
         ++it;
-        if (++s == NS) { s = 0; ph ^= 1u; }
+        at += p.stage_bytes;
+        bar += 8;
+        if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
       };
       for (int t = unit; t < total && ok; t += nunits) {
         int m, n;
         tile_of(p, t, m, n);
         const int m0 = (m * NCTA + (int)rank) * FM, n0 = n * g;
         if (BWD) {
+          const int f0 = n0 + (PAIR ? (int)rank * 64 : 0);
           for (int kb = 0; kb < nkb; ++kb) {
-            const uint32_t bar = next(p.da_bytes);
-            if (!ok) break;
-            const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + F_A_BYTES;
-            if (PAIR) {
-              tma_load_2d_pair(a, &tdy, bar, kb * 64, m0);
-              tma_load_2d_pair(b, &twd, bar, n0 + (int)rank * 64, kb * 64);
-            } else {
-              tma_load_2d(a, &tdy, bar, kb * 64, m0);
-              for (int c = 0; c < g; c += 64) tma_load_2d(b + c * 128, &twd, bar, n0 + c, kb * 64);
-            }
-            advance();
+            if (!take(da_bytes)) break;
+            load(0, &tdy, kb * 64, m0);
+            load(F_A_BYTES, &twd, f0, kb * 64);
+            if (!PAIR && g > 64) load(F_A_BYTES + 8192, &twd, f0 + 64, kb * 64);
+            step();
           }
         }
+        const int w0 = n0 + (PAIR ? (int)rank * p.F : 0);
         for (int kb = 0; kb < nkb && ok; ++kb) {
-          const uint32_t bar = next(p.gu_bytes);
-          if (!ok) break;
-          const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + F_A_BYTES;
-          if (PAIR) {
-            tma_load_2d_pair(a, &tx, bar, kb * BKE, m0);
-            tma_load_2d_pair(b, &tw, bar, kb * BKE, (int)rank * p.F + n0);
-          } else {
-            tma_load_2d(a, &tx, bar, kb * BKE, m0);
-            tma_load_2d(b, &tw, bar, kb * BKE, n0);
-            tma_load_2d(b + g * 128, &tw, bar, kb * BKE, p.F + n0);
-          }
-          advance();
+          if (!take(gu_bytes)) break;
+          load(0, &tx, kb * BKE, m0);
+          load(F_A_BYTES, &tw, kb * BKE, w0);
+          if (!PAIR) load(F_A_BYTES + (uint32_t)g * 128u, &tw, kb * BKE, p.F + n0);
+          step();
         }
       }
       // a wait that gave up: the copies in flight land before the CTA's memory is given back
@@ -173,35 +171,39 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
     if (lane == 0 && rank == 0) {
       const uint32_t i_gu = E4M3 ? make_idesc_e4m3(FM * NCTA, PAIR ? 256 : 2 * g) : make_idesc_bf16(FM * NCTA, PAIR ? 256 : 2 * g, 0, 0);
       const uint32_t i_da = make_idesc_bf16(FM * NCTA, g, 0, 1);
-      int s = 0, i = 0;
-      uint32_t ph = 0;
+      const uint64_t desc_a = make_smem_desc_sw128(s0, 0, 1024), desc_b = make_smem_desc_sw128(s0 + F_A_BYTES, 0, 1024);
+      const uint64_t desc_mn = make_smem_desc_sw128(s0 + F_A_BYTES, 8192, 1024);
+      const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
+      int i = 0;
+      uint32_t at = 0, bar = 0, ph = 0;
       bool ok = true;
-      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-        ok = ok && (PAIR ? mbar_wait_cluster(bar, parity, p.status, code) : mbar_wait(bar, parity, p.status, code));
+      auto wait = [&](uint32_t b, uint32_t parity, int code) {
+        ok = ok && (PAIR ? mbar_wait_cluster(b, parity, p.status, code) : mbar_wait(b, parity, p.status, code));
         if (ok) tc_fence_after_sync();
         return ok;
       };
-      // b_mn: the B rows of this phase lie along the reduction (MN-major)
-      auto product = [&](uint32_t acc, uint32_t idesc, bool b_mn) {
+      // b_step: 16 elements along the reduction (32 in 8 bits), in a B tile that is stored along it or across it
+      auto product = [&](uint32_t acc, uint32_t idesc, uint64_t db, uint32_t b_step) {
+        uint32_t add = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!wait(full + 8 * s, ph, W_FFN_FULL)) return;
-          const uint32_t a = s0 + (uint32_t)s * p.stage_bytes, b = a + F_A_BYTES;
+          if (!wait(full + bar, ph, W_FFN_FULL)) return;
+          const uint64_t ad = desc_at(desc_a, at), bd = desc_at(db, at);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = make_smem_desc_sw128(a + k * 32, 0, 1024);
-            const uint64_t bd = b_mn ? make_smem_desc_sw128(b + k * 2048, 8192, 1024) : make_smem_desc_sw128(b + k * 32, 0, 1024);
-            const uint32_t add = (kb | k) != 0 ? 1u : 0u;
             if (E4M3) {
-              if (PAIR) umma_e4m3_pair(acc, ad, bd, idesc, add);
-              else umma_e4m3(acc, ad, bd, idesc, add);
+              if (PAIR) umma_e4m3_pair(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+              else umma_e4m3(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
             } else {
-              if (PAIR) umma_bf16_pair(acc, ad, bd, idesc, add);
-              else umma_bf16(acc, ad, bd, idesc, add);
+              if (PAIR) umma_bf16_pair(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+              else umma_bf16(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
             }
           }
-          if (PAIR) umma_commit_pair(empty + 8 * s, (uint16_t)3);
-          else umma_commit(empty + 8 * s);
-          if (++s == NS) { s = 0; ph ^= 1u; }
+          add = 1;
+          if (PAIR) umma_commit_pair(empty + bar, (uint16_t)3);
+          else umma_commit(empty + bar);
+          at += p.stage_bytes;
+          bar += 8;
+          if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
         }
       };
       for (int t = unit; t < total && ok; t += nunits, ++i) {
@@ -209,12 +211,12 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
         // tile i - 2 has been read (parity starts so that the first two waits pass)
         if (!wait(acc_empty + 8 * b, ((uint32_t)(i >> 1) & 1u) ^ 1u, W_FFN_ACC)) break;
         if (BWD) {
-          product(tmem + (b ? 3u * quarter : 0u), i_da, true);
+          product(tmem + (b ? 3u * quarter : 0u), i_da, desc_mn, 2048u);
           // gate and up have one accumulator: tile i - 1 has been read
           if (i > 0 && !wait(acc_empty + 8 * (b ^ 1u), (uint32_t)((i - 1) >> 1) & 1u, W_FFN_ACC)) break;
-          product(tmem + quarter, i_gu, false);
+          product(tmem + quarter, i_gu, desc_b, 32u);
         } else {
-          product(tmem + b * 2u * quarter, i_gu, false);
+          product(tmem + b * 2u * quarter, i_gu, desc_b, 32u);
         }
         if (!ok) break;
         if (PAIR) umma_commit_pair(acc_full + 8 * b, (uint16_t)3);
@@ -247,20 +249,20 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
         }
       };
       if constexpr (PAIR) {
-        const int c0 = grp * 64;
+        const int c0 = grp * 32;
         const bool live = m0 < p.T && n0 + c0 < p.F;  // the same for the whole group
-        uint32_t w[BWD ? 3 : 1][32];
+        uint32_t w[BWD ? 3 : 1][16];
         if (live) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint32_t gv[32], uv[32], dv[BWD ? 32 : 1];
-            tmem_ld_32x32b_x32(t_gu + (uint32_t)(c0 + h * 32), gv);
-            tmem_ld_32x32b_x32(t_gu + 128u + (uint32_t)(c0 + h * 32), uv);
-            if constexpr (BWD) tmem_ld_32x32b_x32(t_da + (uint32_t)(c0 + h * 32), dv);
+            uint32_t gv[16], uv[16], dv[BWD ? 16 : 1];
+            tmem_ld_32x32b_x16(t_gu + (uint32_t)(c0 + h * 16), gv);
+            tmem_ld_32x32b_x16(t_gu + 128u + (uint32_t)(c0 + h * 16), uv);
+            if constexpr (BWD) tmem_ld_32x32b_x16(t_da + (uint32_t)(c0 + h * 16), dv);
             tmem_ld_wait();
-            const int col = n0 + c0 + h * 32;
+            const int col = n0 + c0 + h * 16;
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
+            for (int c = 0; c < 16; c += 2) {
               float a[2], dg[2], du[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
@@ -278,24 +280,24 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
                   du[e] = da * silu;
                 }
               }
-              w[0][h * 16 + c / 2] = pack_bf16(a[0], a[1]);
+              w[0][h * 8 + c / 2] = pack_bf16(a[0], a[1]);
               if constexpr (BWD) {
-                w[1][h * 16 + c / 2] = pack_bf16(dg[0], dg[1]);
-                w[2][h * 16 + c / 2] = pack_bf16(du[0], du[1]);
+                w[1][h * 8 + c / 2] = pack_bf16(dg[0], dg[1]);
+                w[2][h * 8 + c / 2] = pack_bf16(du[0], du[1]);
               }
             }
           }
         }
         done();
         if (live) {
-          const uint32_t slab = smem_u32(sOut) + (uint32_t)grp * F_SLAB_BYTES, mine = slab + (uint32_t)row * 128u;
+          const uint32_t slab = smem_u32(sOut) + (uint32_t)grp * F_SLAB_BYTES, mine = slab + (uint32_t)row * 64u;
 #pragma unroll
           for (int o = 0; o < (BWD ? 3 : 1); ++o) {
             if (issuer) bulk_wait_group_read<0>();  // the store before has read the slab
             named_bar_sync(1 + grp, 128);
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              st_shared_v4(mine + (uint32_t)((c ^ (row & 7)) << 4), w[o][c * 4], w[o][c * 4 + 1], w[o][c * 4 + 2], w[o][c * 4 + 3]);
+            for (int c = 0; c < 4; ++c)
+              st_shared_v4(mine + (uint32_t)((c ^ ((row >> 1) & 3)) << 4), w[o][c * 4], w[o][c * 4 + 1], w[o][c * 4 + 2], w[o][c * 4 + 3]);
             fence_proxy_async_smem();
             named_bar_sync(1 + grp, 128);
             if (issuer) {
@@ -393,16 +395,17 @@ FfnPlan plan_ffn(int T, int F, bool bwd) {
 template <bool PAIR, bool BWD, bool E4M3>
 int launch_ffn(FfnParams& p, const CUtensorMap (&tm)[7], cudaStream_t st) {
   const size_t budget = PAIR || p.cols > 256 ? 232448 : 113 * 1024;  // two single CTAs share an SM where tensor memory allows
-  const size_t fixed = 1024 + (PAIR ? 2 * F_SLAB_BYTES : 0) + ffn_tail_bytes();
+  const size_t fixed = 1024 + (PAIR ? epi_groups(true) * F_SLAB_BYTES : 0) + ffn_tail_bytes();
   p.stages = (int)((budget - fixed) / p.stage_bytes);
   if (p.stages > F_MAX_STAGES) p.stages = F_MAX_STAGES;
   const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
-  SRT_CHECK_CUDA(cudaFuncSetAttribute(gated_ffn_kernel<PAIR, BWD, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+  static SmemOptIn opt_in;
+  SRT_CHECK_CUDA(opt_in.set(gated_ffn_kernel<PAIR, BWD, E4M3>, 232448));
   const int room = PAIR ? sm_count() / 2 : sm_count() * (p.cols > 256 ? 1 : 2);
   const long long total = (long long)p.m_units * p.n_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((total < room ? total : room) * (PAIR ? 2 : 1)));
-  cfg.blockDim = dim3(F_THREADS);
+  cfg.blockDim = dim3(ffn_threads(PAIR));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -456,10 +459,10 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   if ((rc = tmap_rows_128b(&tm[0], x, T, C, C, esz, a_rows)) || (rc = tmap_rows_128b(&tm[1], w_gu, 2ull * F, C, C, esz, b_rows))) return rc;
   for (int i = 2; i < 7; ++i) tm[i] = tm[0];
   if (bwd && ((rc = tmap_rows_128b(&tm[2], dy, T, C, C, 2, a_rows)) || (rc = tmap_rows_128b(&tm[3], w_down, C, F, F, 2, 64)))) return rc;
-  if (plan.pair && (rc = tmap_rows_128b(&tm[4], act, T, F, F, 2, FM))) return rc;
+  if (plan.pair && (rc = tmap_rows(&tm[4], act, T, F, F, 2, 32, FM))) return rc;
   // the two halves of dgu have maps of their own: a store that reaches beyond `hidden` is clipped in either
-  if (plan.pair && bwd && ((rc = tmap_rows_128b(&tm[5], dgu, T, F, 2ull * F, 2, FM)) ||
-                           (rc = tmap_rows_128b(&tm[6], (bf16*)dgu + F, T, F, 2ull * F, 2, FM))))
+  if (plan.pair && bwd && ((rc = tmap_rows(&tm[5], dgu, T, F, 2ull * F, 2, 32, FM)) ||
+                           (rc = tmap_rows(&tm[6], (bf16*)dgu + F, T, F, 2ull * F, 2, 32, FM))))
     return rc;
   if (bwd) return plan.pair ? launch_ffn<true, true, false>(p, tm, st) : launch_ffn<false, true, false>(p, tm, st);
   if (e4m3) return plan.pair ? launch_ffn<true, false, true>(p, tm, st) : launch_ffn<false, false, true>(p, tm, st);
@@ -554,23 +557,27 @@ token_gate_kernel(const uint4* __restrict__ x, const uint4* __restrict__ w, cons
   }
 }
 
-// One output row of Wd a block, a quarter of it a warp.
+// One output row of Wd a block, a quarter of it a warp. The first loads of the row leave before the launch in front, the
+// gate's, has ended: it does not write weights, and it has waited for whatever did. (They bypass L1.)
 template <int TT>
 __global__ void __launch_bounds__(TOK_THREADS)
-token_down_kernel(const uint4* __restrict__ act, const uint4* __restrict__ w, const bf16* __restrict__ residual, bf16* __restrict__ y,
-                  int vecs, int C) {
+token_down_kernel(const uint4* act, const uint4* __restrict__ w, const bf16* __restrict__ residual, bf16* __restrict__ y, int vecs, int C) {
   constexpr int U = 4, WARPS = TOK_THREADS / 32;
   __shared__ float sh[WARPS][TT];
-  pdl_enter();
   const int c = blockIdx.x;
   const uint4* wr = w + (size_t)c * vecs;
+  uint4 a[U];
+  auto fetch = [&](int v0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) a[i] = v0 + TOK_THREADS * i < vecs ? __ldcg(wr + v0 + TOK_THREADS * i) : make_uint4(0, 0, 0, 0);
+  };
+  fetch(threadIdx.x);
+  pdl_enter();
   float s[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) s[t] = 0.f;
   for (int v0 = threadIdx.x; v0 < vecs; v0 += TOK_THREADS * U) {
-    uint4 a[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) a[i] = v0 + TOK_THREADS * i < vecs ? __ldcs(wr + v0 + TOK_THREADS * i) : make_uint4(0, 0, 0, 0);
+    if (v0 != (int)threadIdx.x) fetch(v0);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       if (v0 + TOK_THREADS * i >= vecs) break;
@@ -664,7 +671,7 @@ int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_sca
     case TOK_MAX: return token_ffn<TOK_MAX>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
   }
   if ((rc = gated_products(*d, x, x_scale, w_gu, w_scale, nullptr, nullptr, act, nullptr, st))) return rc;
-  return balanced_gemm(down_problem(*d), act, w_down, residual, y, (char*)scratch + act_bytes, scratch_bytes - act_bytes, st);
+  return balanced_gemm(down_problem(*d), act, w_down, residual, y, (char*)scratch + act_bytes, scratch_bytes - act_bytes, true, st);
 }
 
 GatedFfnScratch gated_ffn_scratch(const srt_gated_ffn_desc& d, int grad_dtype) {
@@ -696,9 +703,10 @@ int gated_ffn_bwd(const srt_gated_ffn_desc* d, const void* dy, const void* x, co
   void *act = base, *dgu = base + s.dgu, *slots = base + s.slots;
   const size_t room = scratch_bytes - s.slots;
   if ((rc = gated_products(*d, x, nullptr, w_gu, nullptr, dy, w_down, act, dgu, st))) return rc;
-  if (dx && (rc = balanced_gemm(dx_problem(*d), dgu, w_gu, nullptr, dx, slots, room, st))) return rc;
-  if (dw_gu && (rc = balanced_gemm(dw_problem(*d, grad_dtype), dgu, x, nullptr, dw_gu, slots, room, st))) return rc;
-  if (dw_down && (rc = balanced_gemm(dd_problem(*d, grad_dtype), dy, act, nullptr, dw_down, slots, room, st))) return rc;
+  if (dx && (rc = balanced_gemm(dx_problem(*d), dgu, w_gu, nullptr, dx, slots, room, true, st))) return rc;
+  if (dw_gu && (rc = balanced_gemm(dw_problem(*d, grad_dtype), dgu, x, nullptr, dw_gu, slots, room, true, st))) return rc;
+  // act comes from the gated kernel, which is directly in front where nothing else was asked for
+  if (dw_down && (rc = balanced_gemm(dd_problem(*d, grad_dtype), dy, act, nullptr, dw_down, slots, room, dx || dw_gu, st))) return rc;
   return SRT_OK;
 }
 

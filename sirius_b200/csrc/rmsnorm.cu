@@ -7,10 +7,10 @@
 // bf16 or fp32 rows, fp32 parameters and statistics. y comes from the fp32 sum, not from the rounded h that is stored: one
 // rounding on the way to y instead of two.
 //
-// All of it is bound by memory: a row is read once, sits in the registers of one to sixteen warps (at most four 16-byte
-// vectors a lane) until its statistics are known, and is written once. Blocks walk over rows, so gamma is loaded once a block
-// and, in backward, dgamma adds up in registers over the rows of a warp; blocks leave one partial row each, which a second
-// launch adds in a fixed order. No atomics: a call repeats bit for bit.
+// All of it is bound by memory: a row is read once, sits in the registers of one to sixteen warps (16 elements a lane, 32 in
+// the longest rows) until its statistics are known, and is written once; the next row's loads are in flight meanwhile.
+// Blocks walk over rows, so gamma is loaded once a block and, in backward, dgamma adds up in registers over the rows of a
+// warp; blocks leave one partial row each, which a second launch adds in a fixed order. No atomics: a call repeats bit for bit.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -20,7 +20,7 @@ namespace srt {
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int RN_MAX_BLOCKS = 592;   // partial rows of dgamma
+constexpr int RN_MAX_BLOCKS = 160;   // partial rows of dgamma: one block an SM
 constexpr int RN_MAX_ROW_BYTES = 32768;
 constexpr float E4M3_MAX = 448.f;
 
@@ -39,15 +39,15 @@ __device__ __forceinline__ float warp_all(float v) {
   }
   return v;
 }
-// Over the W warps of a row group; `red` has a slot per warp of the block, and `turn` alternates its halves so that one
-// barrier a reduction is enough.
+// Over the W warps of a row group, which meet on a barrier of their own; `red` has a slot per warp of the block, and `turn`
+// alternates its halves so that one barrier a reduction is enough.
 template <bool MAX>
 __device__ __forceinline__ float group_all(float v, int W, float (*red)[32], int& turn) {
   v = warp_all<MAX>(v);
   if (W == 1) return v;
   const int warp = threadIdx.x >> 5, first = warp & ~(W - 1);
   if ((threadIdx.x & 31) == 0) red[turn][warp] = v;
-  __syncthreads();
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + first / W), "r"(W * 32) : "memory");
   v = red[turn][first];
   for (int w = 1; w < W; ++w) v = MAX ? max_nan(v, red[turn][first + w]) : v + red[turn][first + w];
   turn ^= 1;
@@ -69,14 +69,16 @@ struct RowShape {
 
 // NORM false: y = x, only quantised. OUT8: q and scale instead of y.
 template <typename T, int NV, bool NORM, bool OUT8>
-__global__ void __launch_bounds__(512)
-rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float* __restrict__ gamma, T* h_out, T* __restrict__ y, uint8_t* __restrict__ q, float* __restrict__ scale,
-                   float* __restrict__ rstd, float eps) {
+__global__ void __maxnreg__((NV * Vec16<T>::N > 16) ? 128 : 80)
+rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float* __restrict__ gamma, T* h_out, T* __restrict__ y,
+                   uint8_t* __restrict__ q, float* __restrict__ scale, float* __restrict__ rstd, float eps) {
   constexpr int V = Vec16<T>::N;
+  constexpr bool AHEAD = NV <= 2;  // the next row's vectors beside the current one's
   __shared__ float red[2][32];
   pdl_enter();
   const int W = s.W, groups = (int)(blockDim.x >> 5) / W, grp = (int)(threadIdx.x >> 5) / W;
   const int lane = (int)threadIdx.x - grp * W * 32, nv = s.C / V;
+  const int64_t step = (int64_t)gridDim.x * groups;
   int turn = 0;
   float gm[NORM ? NV : 1][V];
   if constexpr (NORM) {
@@ -87,22 +89,24 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
       for (int e = 0; e < V; ++e) gm[i][e] = v < nv ? gamma[v * V + e] : 0.f;
     }
   }
-  // every group of a block makes the same number of turns: the barriers inside are the block's
-  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < s.rows; r0 += (int64_t)gridDim.x * groups) {
-    const int64_t row = r0 + grp;
-    const bool live = row < s.rows;
-    const int64_t at = row * s.C;
-    Vec16<T> xv[NV], rv[NV];
+  Vec16<T> xv[NV], rv[NV];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = lane + i * W * 32;
       clear(xv[i]);
       clear(rv[i]);
-      if (live && v < nv) {
-        xv[i].load(x + at + v * V);
-        if (residual) rv[i].load(residual + at + v * V);
+      if (row < s.rows && v < nv) {
+        xv[i].load(x + row * s.C + v * V);
+        if (residual) rv[i].load(residual + row * s.C + v * V);
       }
     }
+  };
+  int64_t row = (int64_t)blockIdx.x * groups + grp;
+  if (AHEAD) fetch(row);
+  for (; row < s.rows; row += step) {
+    const int64_t at = row * s.C;
+    if (!AHEAD) fetch(row);
     float f[NV][V], sq = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -115,8 +119,13 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) sq = fmaf(f[i][e], f[i][e], sq);
-      const int v = lane + i * W * 32;
-      if (h_out && live && v < nv) {
+    }
+    if (AHEAD) fetch(row + step);
+    if (h_out) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = lane + i * W * 32;
+        if (v >= nv) continue;
         Vec16<T> o;
         o.pack(f[i]);
         o.store(h_out + at + v * V);
@@ -124,7 +133,7 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
     }
     if constexpr (NORM) {
       const float rs = rsqrtf(group_all<false>(sq, W, red, turn) / (float)s.C + eps);
-      if (rstd && live && lane == 0) rstd[row] = rs;
+      if (rstd && lane == 0) rstd[row] = rs;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -137,15 +146,15 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
 #pragma unroll
         for (int e = 0; e < V; ++e) mx = max_nan(mx, fabsf(f[i][e]));
       mx = group_all<true>(mx, W, red, turn);
-      const float sc = max_nan(mx / E4M3_MAX, 1.17549435e-38f);
-      if (live && lane == 0) scale[row] = sc;
+      const float sc = max_nan(mx / E4M3_MAX, 1.17549435e-38f), inv = 1.f / sc;
+      if (lane == 0) scale[row] = sc;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = lane + i * W * 32;
-        if (!live || v >= nv) continue;
+        if (v >= nv) continue;
         uint32_t w[V / 4];
 #pragma unroll
-        for (int e = 0; e < V; e += 4) w[e / 4] = four_e4m3(f[i][e] / sc, f[i][e + 1] / sc, f[i][e + 2] / sc, f[i][e + 3] / sc);
+        for (int e = 0; e < V; e += 4) w[e / 4] = four_e4m3(f[i][e] * inv, f[i][e + 1] * inv, f[i][e + 2] * inv, f[i][e + 3] * inv);
         if constexpr (V == 8) *reinterpret_cast<uint2*>(q + at + v * V) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(q + at + v * V) = w[0];
       }
@@ -153,7 +162,7 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = lane + i * W * 32;
-        if (!live || v >= nv) continue;
+        if (v >= nv) continue;
         Vec16<T> o;
         o.pack(f[i]);
         o.store(y + at + v * V);
@@ -163,15 +172,17 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
 }
 
 template <typename T, int NV>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, 1)
 rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const float* __restrict__ gamma,
                    const float* __restrict__ rstd, const T* dh, T* dx, float* __restrict__ partial) {
   constexpr int V = Vec16<T>::N;
-  extern __shared__ float cols[];  // [C], several row groups a block
+  constexpr bool AHEAD = NV <= 2;
+  extern __shared__ float cols[];  // [row groups of the block][C]
   __shared__ float red[2][32];
   pdl_enter();
   const int W = s.W, groups = (int)(blockDim.x >> 5) / W, grp = (int)(threadIdx.x >> 5) / W;
   const int lane = (int)threadIdx.x - grp * W * 32, nv = s.C / V;
+  const int64_t step = (int64_t)gridDim.x * groups;
   int turn = 0;
   float gm[NV][V], dg[NV][V];
 #pragma unroll
@@ -180,30 +191,38 @@ rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const
 #pragma unroll
     for (int e = 0; e < V; ++e) { gm[i][e] = v < nv ? gamma[v * V + e] : 0.f; dg[i][e] = 0.f; }
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < s.rows; r0 += (int64_t)gridDim.x * groups) {
-    const int64_t row = r0 + grp;
-    const bool live = row < s.rows;
-    const int64_t at = row * s.C;
-    Vec16<T> gv[NV], hv[NV], av[NV];
+  Vec16<T> gv[NV], hv[NV], av[NV];
+  float rs_next = 0.f;
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = lane + i * W * 32;
       clear(gv[i]);
       clear(hv[i]);
       clear(av[i]);
-      if (live && v < nv) {
-        gv[i].load(dy + at + v * V);
-        hv[i].load(h + at + v * V);
-        if (dh) av[i].load(dh + at + v * V);
+      if (row < s.rows && v < nv) {
+        gv[i].load(dy + row * s.C + v * V);
+        hv[i].load(h + row * s.C + v * V);
+        if (dh) av[i].load(dh + row * s.C + v * V);
       }
     }
-    const float rs = live ? rstd[row] : 0.f;
+    rs_next = row < s.rows ? rstd[row] : 0.f;
+  };
+  int64_t row = (int64_t)blockIdx.x * groups + grp;
+  if (AHEAD) fetch(row);
+  for (; row < s.rows; row += step) {
+    if (!AHEAD) fetch(row);
+    const float rs = rs_next;
+    Vec16<T> g0[NV], h0[NV], a0[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) { g0[i] = gv[i]; h0[i] = hv[i]; a0[i] = av[i]; }
+    if (AHEAD) fetch(row + step);
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float g[V], f[V];
-      gv[i].unpack(g);
-      hv[i].unpack(f);
+      g0[i].unpack(g);
+      h0[i].unpack(f);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float p = g[e] * (f[e] * rs);
@@ -215,77 +234,79 @@ rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = lane + i * W * 32;
-      if (!live || v >= nv) continue;
+      if (v >= nv) continue;
       float g[V], f[V], a[V];
-      gv[i].unpack(g);
-      hv[i].unpack(f);
-      av[i].unpack(a);
+      g0[i].unpack(g);
+      h0[i].unpack(f);
+      a0[i].unpack(a);
 #pragma unroll
       for (int e = 0; e < V; ++e) a[e] += rs * (g[e] * gm[i][e] - f[e] * rs * dot);
       Vec16<T> o;
       o.pack(a);
-      o.store(dx + at + v * V);
+      o.store(dx + row * s.C + v * V);
     }
   }
-  // the groups of the block one after the other, in order
-  float* out = partial + (size_t)blockIdx.x * s.C;
-  for (int k = 0; k < groups; ++k) {
-    if (grp == k) {
+  // the groups of the block in order
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = lane + i * W * 32;
-        if (v >= nv) continue;
+  for (int i = 0; i < NV; ++i) {
+    const int v = lane + i * W * 32;
+    if (v >= nv) continue;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float t = k ? cols[v * V + e] + dg[i][e] : dg[i][e];
-          if (k == groups - 1) out[v * V + e] = t;
-          else cols[v * V + e] = t;
-        }
-      }
-    }
-    if (k < groups - 1) __syncthreads();
+    for (int e = 0; e < V; e += 4)
+      *reinterpret_cast<float4*>(cols + (size_t)grp * s.C + v * V + e) = make_float4(dg[i][e], dg[i][e + 1], dg[i][e + 2], dg[i][e + 3]);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < s.C; c += blockDim.x) {
+    float t = cols[c];
+    for (int k = 1; k < groups; ++k) t += cols[(size_t)k * s.C + c];
+    partial[(size_t)blockIdx.x * s.C + c] = t;
   }
 }
-// dgamma[c] = sum of the blocks' partial rows: 32 columns x 8 lanes a block, lane l adds rows l, l + 8, ... and the lanes
+// dgamma[c] = sum of the blocks' partial rows: 32 columns x 32 lanes a block, lane l adds rows l, l + 32, ... and the lanes
 // are added in order.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 rmsnorm_dgamma_kernel(const float* __restrict__ partial, int blocks, int C, float* __restrict__ dgamma) {
-  __shared__ float sh[8][33];
+  __shared__ float sh[32][33];
   pdl_enter();
   const int cl = threadIdx.x & 31, l = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   float t = 0.f;
   if (c < C) {
 #pragma unroll 8
-    for (int b = l; b < blocks; b += 8) t += partial[(size_t)b * C + c];
+    for (int b = l; b < blocks; b += 32) t += partial[(size_t)b * C + c];
   }
   sh[l][cl] = t;
   __syncthreads();
   if (l == 0 && c < C) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += sh[k][cl];
+    for (int k = 1; k < 32; ++k) t += sh[k][cl];
     dgamma[c] = t;
   }
 }
 
-// Warps a row: as few as hold it in four vectors a lane, and more where the rows are too few to occupy the device.
+// Warps a row: as few as hold it in 16 elements a lane, and more where the rows are too few to occupy the device; only bf16
+// rows beyond 8192 have more elements a lane. Three blocks of eight warps an SM in forward (80 registers a thread), one of
+// sixteen in backward.
+// 8192 rows of 896 in bf16, inputs out of memory: forward 13.7 us with one warp and four vectors a lane, without the next
+// row in flight; backward 28.6 us.
 struct RowLaunch {
   RowShape s;
   int nv, threads;
   unsigned blocks;
 };
-RowLaunch row_launch(int64_t rows, int C, int vec, int max_blocks) {
+RowLaunch row_launch(int64_t rows, int C, int vec, int warps, int per_sm) {
   RowLaunch l;
   int W = 1;
-  while (ceil_div(C, W * 32 * vec) > 4) W *= 2;
+  while (W < 16 && C > W * 32 * 16) W *= 2;
   const int sms = sm_count();
   while (W < 16 && rows * W < 8ll * sms && ceil_div(C, W * 32 * vec) > 1) W *= 2;
   l.s = {rows, C, W};
   l.nv = ceil_div(C, W * 32 * vec);
-  const int warps = W > 4 ? W : 4;
+  if (warps < W) warps = W;
+  while (warps > W && rows * W < (int64_t)warps * sms) warps /= 2;  // one row a block before a second one
   l.threads = warps * 32;
-  const int64_t want = (rows + warps / W - 1) / (warps / W), room = (int64_t)sms * (16 / warps > 1 ? 16 / warps : 1);
+  const int64_t want = (rows + warps / W - 1) / (warps / W);
+  const int64_t room = (int64_t)(warps > 8 ? 1 : per_sm) * sms;
   l.blocks = (unsigned)(want < room ? want : room);
-  if ((int)l.blocks > max_blocks) l.blocks = max_blocks;
   return l;
 }
 
@@ -304,7 +325,7 @@ int check_ptrs(const char* what, std::initializer_list<const void*> ps) {
 template <typename T, bool NORM, bool OUT8>
 int fwd_launch(int64_t rows, int C, const void* x, const void* residual, const float* gamma, void* h, void* y, void* q, float* scale,
                float* rstd, float eps, cudaStream_t st) {
-  const RowLaunch l = row_launch(rows, C, Vec16<T>::N, 1 << 30);
+  const RowLaunch l = row_launch(rows, C, Vec16<T>::N, 8, 3);
   auto go = [&](auto kernel) -> int {
     SRT_CHECK_CUDA(launch_pdl(kernel, dim3(l.blocks), dim3(l.threads), 0, st, l.s, (const T*)x, (const T*)residual, gamma, (T*)h, (T*)y,
                               (uint8_t*)q, scale, rstd, eps));
@@ -321,13 +342,15 @@ int fwd_launch(int64_t rows, int C, const void* x, const void* residual, const f
 template <typename T>
 int bwd_launch(int64_t rows, int C, const void* dy, const void* h, const float* gamma, const float* rstd, const void* dh, void* dx,
                float* dgamma, float* partial, cudaStream_t st) {
-  const RowLaunch l = row_launch(rows, C, Vec16<T>::N, RN_MAX_BLOCKS);
-  const size_t smem = l.threads / 32 > l.s.W ? (size_t)C * sizeof(float) : 0;  // W <= 2: at most 2048 columns
+  const RowLaunch l = row_launch(rows, C, Vec16<T>::N, 16, 1);
+  SRT_REQUIRE(l.blocks <= RN_MAX_BLOCKS, "rmsnorm_bwd: %u partial rows", l.blocks);
+  const size_t smem = (size_t)(l.threads / 32 / l.s.W) * C * sizeof(float);
   auto go = [&](auto kernel) -> int {
+    if (smem > 48 * 1024) SRT_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
     SRT_CHECK_CUDA(launch_pdl(kernel, dim3(l.blocks), dim3(l.threads), smem, st, l.s, (const T*)dy, (const T*)h, gamma, rstd, (const T*)dh,
                               (T*)dx, partial));
     SRT_LAUNCH_CHECK();
-    SRT_CHECK_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3(ceil_div(C, 32)), dim3(256), 0, st, (const float*)partial, (int)l.blocks, C, dgamma));
+    SRT_CHECK_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3(ceil_div(C, 32)), dim3(1024), 0, st, (const float*)partial, (int)l.blocks, C, dgamma));
     SRT_LAUNCH_CHECK();
     return SRT_OK;
   };

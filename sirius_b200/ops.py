@@ -3,6 +3,7 @@ buffers) and calls one entry point on the current stream. Layouts are NHWC / KRS
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import torch
 
@@ -25,30 +26,34 @@ def _p(t):
     return t.data_ptr()
 
 
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream   # the handle without the Stream object around it, which takes 3 us to make
+
+
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_current_device())
 
 
-def _check(what, shape, dtype, device, **tensors):
-    """Each of `tensors` is a contiguous CUDA tensor on the current device (whose stream the call goes to), beside `device`,
-    of this shape and type. None passes; a shape or type of None is not looked at."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be a contiguous CUDA tensor")
-        if t.device != device or t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{what}: {name} is on {t.device}; operands are on the current device, cuda:{torch.cuda.current_device()}")
-        if dtype is not None and t.dtype != dtype:
-            raise TypeError(f"{what}: {name} is {t.dtype}, not {dtype}")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+def _wrong(what, name, t, shape, dtype, dev):
+    """The error that _check's operand deserves."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous CUDA tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}; operands are on the current device, cuda:{dev}")
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} is {t.dtype}, not {dtype}")
+    raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
 
 
-def _device(what, t):
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{what}: tensors are wanted")
-    return t.device
+def _check(what, name, t, shape, dtype, dev):
+    """Address of a contiguous CUDA tensor of this shape and type on the current device `dev` (whose stream the call goes to).
+    None gives None; a shape or type of None is not looked at."""
+    if t is None:
+        return None
+    if (not isinstance(t, torch.Tensor) or t.get_device() != dev or not t.is_contiguous() or (dtype is not None and t.dtype is not dtype)
+            or (shape is not None and t.shape != shape)):
+        _wrong(what, name, t, shape, dtype, dev)
+    return t.data_ptr()
 
 
 def _ep(bias, addend, addend_bits=None):
@@ -251,8 +256,8 @@ def colsum(dy):
 def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None, clip=None):
     """`clip` as in adamw."""
     if clip is not None:
-        _clip_operands(p, g, m, p_bf16, clip)
-        call("srt_sgd_momentum_clipped", _p(p), _p(g), _p(m), _p(p_bf16), p.numel(), lr, mu, wd, int(first_step), _p(clip), _stream())
+        pp, gp, mp, _, bp, cp, st = _clip_operands("sgd_momentum", p, g, m, None, p_bf16, clip)
+        call("srt_sgd_momentum_clipped", pp, gp, mp, bp, p.numel(), lr, mu, wd, int(first_step), cp, st)
         return
     call("srt_sgd_momentum", _p(p), _p(g), _p(m), _p(p_bf16), p.numel(), lr, mu, wd, int(first_step), _stream())
 
@@ -260,38 +265,42 @@ def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None, clip=None):
 def adamw(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16=None, clip=None):
     """`clip`: what grad_norm returned; the gradients are multiplied by its coefficient on the way in."""
     if clip is not None:
-        _clip_operands(p, g, m, v, p_bf16, clip)
-        call("srt_adamw_clipped", _p(p), _p(g), _p(m), _p(v), _p(p_bf16), p.numel(), lr, b1, b2, eps, wd, step, _p(clip), _stream())
+        pp, gp, mp, vp, bp, cp, st = _clip_operands("adamw", p, g, m, v, p_bf16, clip)
+        call("srt_adamw_clipped", pp, gp, mp, vp, bp, p.numel(), lr, b1, b2, eps, wd, step, cp, st)
         return
     call("srt_adamw", _p(p), _p(g), _p(m), _p(v), _p(p_bf16), p.numel(), lr, b1, b2, eps, wd, step, _stream())
 
 
-def _clip_operands(p, *rest):
-    *state, p_bf16, clip = rest
-    dev = _device("clipped step", p)
-    _check("clipped step", None, torch.float32, dev, p=p)
-    for t in state:
-        _check("clipped step", p.shape, torch.float32, dev, state=t)
-    _check("clipped step", p.shape, torch.bfloat16, dev, p_bf16=p_bf16)
-    _check("clipped step", (2,), torch.float32, dev, clip=clip)
+def _clip_operands(what, p, g, m, v, p_bf16, clip):
+    dev, f32 = _current_device(), torch.float32
+    pp = _check(what, "p", p, None, f32, dev)
+    shape = p.shape
+    return (pp, _check(what, "g", g, shape, f32, dev), _check(what, "m", m, shape, f32, dev), _check(what, "v", v, shape, f32, dev),
+            _check(what, "p_bf16", p_bf16, shape, torch.bfloat16, dev), _check(what, "clip", clip, (2,), f32, dev), _raw_stream(dev))
 
 
 def _grad_list(name, grads, max_norm):
-    grads = list(grads)
     if not max_norm > 0:
         raise ValueError(f"{name}: max_norm ({max_norm}) must be positive")
-    dev = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
-    dtype = grads[0].dtype if grads else torch.float32
-    for g in grads:
-        _check(name, None, dtype, dev, gradient=g)
+    dev = _current_device()
+    if not isinstance(grads, (list, tuple)):
+        grads = list(grads)
     n = len(grads)
+    dtype = grads[0].dtype if n else torch.float32
+    for g in grads:
+        if g.get_device() != dev or g.dtype is not dtype or not g.is_contiguous():
+            _wrong(name, "a gradient", g, None, dtype, dev)
+    kind = _dt(grads[0]) if n else SRT_F32
+    # addresses and counts behind one another, read by the call before it returns
+    words = array("q", [g.data_ptr() for g in grads])
+    words.extend([g.numel() for g in grads])
+    at = words.buffer_info()[0]
     nbytes = _lib.lib().srt_grad_norm_scratch_bytes(n)
     # the results first, the partial sums behind them
-    work = torch.empty(256 + nbytes, dtype=torch.uint8, device=dev)
-    clip = work[:8].view(torch.float32)
-    call("srt_" + name, SRT_F32 if dtype == torch.float32 else _dt(grads[0]), n, (C.c_void_p * n)(*[g.data_ptr() for g in grads]),
-         (C.c_int64 * n)(*[g.numel() for g in grads]), max_norm, clip.data_ptr(), work.data_ptr() + 256, nbytes, _stream())
-    return clip
+    work = torch.empty(64 + nbytes // 4, dtype=torch.float32, device="cuda")
+    base = work.data_ptr()
+    call("srt_" + name, kind, n, at, at + 8 * n, max_norm, base, base + 256, nbytes, _raw_stream(dev))
+    return work[:2]
 
 
 def grad_norm(grads, max_norm):
@@ -305,110 +314,124 @@ def clip_grad_norm(grads, max_norm):
     return _grad_list("clip_grad_norm", grads, max_norm)
 
 
-def _rows(what, x, gamma, residual):
-    dev = _device(what, x)
-    if x.dim() < 1 or x.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"{what}: rows of float32 or bfloat16 are wanted, not {x.dtype}")
-    _check(what, None, None, dev, x=x)
-    _check(what, x.shape, x.dtype, dev, residual=residual)
-    _check(what, x.shape[-1:], torch.float32, dev, gamma=gamma)
-    return dev, x.shape[-1], x.numel() // max(x.shape[-1], 1)
+def _row_type(what, x):
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError(f"{what}: rows in a CUDA tensor are wanted")
+    if x.dtype is torch.bfloat16:
+        return SRT_BF16
+    if x.dtype is torch.float32:
+        return SRT_F32
+    raise TypeError(f"{what}: rows of float32 or bfloat16 are wanted, not {x.dtype}")
 
 
 def rmsnorm(x, gamma, eps=1e-6, residual=None):
     """h = x + residual, y = gamma * h / rms(h) over the last axis: returns (y, h, rstd). Without a residual h is x itself."""
-    dev, Cc, rows = _rows("rmsnorm", x, gamma, residual)
+    kind, dev = _row_type("rmsnorm", x), _current_device()
+    shape = x.shape
+    xp = _check("rmsnorm", "x", x, None, None, dev)
+    rp = _check("rmsnorm", "residual", residual, shape, x.dtype, dev)
+    gp = _check("rmsnorm", "gamma", gamma, shape[-1:], torch.float32, dev)
     y = torch.empty_like(x)
-    h = torch.empty_like(x) if residual is not None else None
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    call("srt_rmsnorm_fwd", _dt(x), _p(x), _p(residual), _p(gamma), _p(h), _p(y), _p(rstd), rows, Cc, eps, _stream())
-    return y, x if h is None else h, rstd
+    h = x if residual is None else torch.empty_like(x)
+    rstd = gamma.new_empty(shape[:-1])
+    call("srt_rmsnorm_fwd", kind, xp, rp, gp, None if residual is None else h.data_ptr(), y.data_ptr(), rstd.data_ptr(), rstd.numel(),
+         shape[-1], eps, _raw_stream(dev))
+    return y, h, rstd
 
 
 def rmsnorm_e4m3(x, gamma, eps=1e-6, residual=None):
     """rmsnorm whose output leaves in 8 bits, q * scale of its row: returns (q, scale, h, rstd)."""
-    dev, Cc, rows = _rows("rmsnorm_e4m3", x, gamma, residual)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    h = torch.empty_like(x) if residual is not None else None
-    rstd, scale = (torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) for _ in range(2))
-    call("srt_rmsnorm_fwd_e4m3", _dt(x), _p(x), _p(residual), _p(gamma), _p(h), _p(q), _p(scale), _p(rstd), rows, Cc, eps, _stream())
-    return q, scale, x if h is None else h, rstd
+    kind, dev = _row_type("rmsnorm_e4m3", x), _current_device()
+    shape = x.shape
+    xp = _check("rmsnorm_e4m3", "x", x, None, None, dev)
+    rp = _check("rmsnorm_e4m3", "residual", residual, shape, x.dtype, dev)
+    gp = _check("rmsnorm_e4m3", "gamma", gamma, shape[-1:], torch.float32, dev)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    h = x if residual is None else torch.empty_like(x)
+    rstd, scale = gamma.new_empty(shape[:-1]), gamma.new_empty(shape[:-1])
+    call("srt_rmsnorm_fwd_e4m3", kind, xp, rp, gp, None if residual is None else h.data_ptr(), q.data_ptr(), scale.data_ptr(), rstd.data_ptr(),
+         rstd.numel(), shape[-1], eps, _raw_stream(dev))
+    return q, scale, h, rstd
 
 
 def quantize_rows_e4m3(x):
     """Rows (of weights, say) in 8 bits: (q, scale) with x close to q * scale."""
-    dev, Cc, rows = _rows("quantize_rows_e4m3", x, None, None)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    call("srt_quantize_rows_e4m3", _dt(x), _p(x), _p(q), _p(scale), rows, Cc, _stream())
+    kind, dev = _row_type("quantize_rows_e4m3", x), _current_device()
+    xp = _check("quantize_rows_e4m3", "x", x, None, None, dev)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    call("srt_quantize_rows_e4m3", kind, xp, q.data_ptr(), scale.data_ptr(), scale.numel(), x.shape[-1], _raw_stream(dev))
     return q, scale
 
 
 def rmsnorm_backward(dy, h, gamma, rstd, dh=None):
     """Gradient of rmsnorm at the h and rstd that it returned: (dx, dgamma). dx is the gradient of x and of the residual; `dh`
     is what reaches h from elsewhere (the residual path) and is added to it."""
-    dev, Cc, rows = _rows("rmsnorm_backward", h, gamma, dh)
-    _check("rmsnorm_backward", h.shape, h.dtype, dev, dy=dy)
-    _check("rmsnorm_backward", h.shape[:-1], torch.float32, dev, rstd=rstd)
-    dx = torch.empty_like(h)
-    dgamma = torch.empty(Cc, dtype=torch.float32, device=dev)
-    nbytes = _lib.lib().srt_rmsnorm_bwd_scratch_bytes(Cc)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    call("srt_rmsnorm_bwd", _dt(h), _p(dy), _p(h), _p(gamma), _p(rstd), _p(dh), _p(dx), _p(dgamma), rows, Cc, _p(scratch), nbytes, _stream())
+    what = "rmsnorm_backward"
+    kind, dev = _row_type(what, h), _current_device()
+    shape, dtype = h.shape, h.dtype
+    hp = _check(what, "h", h, None, None, dev)
+    dyp, dhp = _check(what, "dy", dy, shape, dtype, dev), _check(what, "dh", dh, shape, dtype, dev)
+    gp, rp = _check(what, "gamma", gamma, shape[-1:], torch.float32, dev), _check(what, "rstd", rstd, shape[:-1], torch.float32, dev)
+    dx, dgamma = torch.empty_like(h), torch.empty_like(gamma)
+    nbytes = _lib.lib().srt_rmsnorm_bwd_scratch_bytes(shape[-1])
+    scratch = gamma.new_empty(nbytes // 4)
+    call("srt_rmsnorm_bwd", kind, dyp, hp, gp, rp, dhp, dx.data_ptr(), dgamma.data_ptr(), rstd.numel(), shape[-1], scratch.data_ptr(), nbytes,
+         _raw_stream(dev))
     return dx, dgamma
 
 
-def _ffn(what, x, w_gate_up, w_down, dtype):
-    dev = _device(what, x)
-    _check(what, None, dtype, dev, x=x, w_gate_up=w_gate_up)
-    _check(what, None, torch.bfloat16, dev, w_down=w_down)
-    if x.dim() != 2 or w_gate_up.dim() != 2 or w_down.dim() != 2 or w_gate_up.shape[0] != 2 * w_down.shape[1]:
-        raise ValueError(f"{what}: x [tokens, width], w_gate_up [2 hidden, width] and w_down [width, hidden] are wanted, not "
-                         f"{tuple(x.shape)}, {tuple(w_gate_up.shape)} and {tuple(w_down.shape)}")
-    (tokens, width), hidden = x.shape, w_down.shape[1]
-    if w_gate_up.shape[1] != width or w_down.shape[0] != width:
-        raise ValueError(f"{what}: x has {width} columns, w_gate_up {w_gate_up.shape[1]} and w_down {w_down.shape[0]} rows")
-    return dev, _lib.GatedFfnDesc(tokens, width, hidden)
+def _ffn(what, x, w_gate_up, w_down, dtype, dev):
+    if not all(isinstance(t, torch.Tensor) and t.dim() == 2 for t in (x, w_gate_up, w_down)) or w_gate_up.shape[0] != 2 * w_down.shape[1]:
+        raise ValueError(f"{what}: x [tokens, width], w_gate_up [2 hidden, width] and w_down [width, hidden] are wanted")
+    tokens, width = x.shape
+    hidden = w_down.shape[1]
+    d = _lib.GatedFfnDesc(tokens, width, hidden)
+    return (d, _check(what, "x", x, None, dtype, dev), _check(what, "w_gate_up", w_gate_up, (2 * hidden, width), dtype, dev),
+            _check(what, "w_down", w_down, (width, hidden), torch.bfloat16, dev))
 
 
 def gated_ffn(x, w_gate_up, w_down, residual=None):
     """residual + (silu(x Wg^T) * (x Wu^T)) Wd^T with w_gate_up = Wg over Wu; bf16."""
-    dev, d = _ffn("gated_ffn", x, w_gate_up, w_down, torch.bfloat16)
-    _check("gated_ffn", x.shape, torch.bfloat16, dev, residual=residual)
-    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(C.byref(d))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    y = torch.empty_like(x)
-    call("srt_gated_ffn_fwd", C.byref(d), _p(x), _p(w_gate_up), _p(w_down), _p(residual), _p(y), _p(scratch), nbytes, _stream())
+    dev = _current_device()
+    d, xp, gp, wp = _ffn("gated_ffn", x, w_gate_up, w_down, torch.bfloat16, dev)
+    rp = _check("gated_ffn", "residual", residual, x.shape, torch.bfloat16, dev)
+    ref = C.byref(d)
+    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(ref)
+    scratch, y = x.new_empty(nbytes // 2), torch.empty_like(x)
+    call("srt_gated_ffn_fwd", ref, xp, gp, wp, rp, y.data_ptr(), scratch.data_ptr(), nbytes, _raw_stream(dev))
     return y
 
 
 def gated_ffn_e4m3(x, x_scale, w_gate_up, w_scale, w_down, residual=None):
     """gated_ffn on 8-bit rows: x * x_scale of its row (rmsnorm_e4m3) and w_gate_up * w_scale of its row (quantize_rows_e4m3)."""
-    dev, d = _ffn("gated_ffn_e4m3", x, w_gate_up, w_down, torch.float8_e4m3fn)
-    _check("gated_ffn_e4m3", (d.tokens,), torch.float32, dev, x_scale=x_scale)
-    _check("gated_ffn_e4m3", (2 * d.hidden,), torch.float32, dev, w_scale=w_scale)
-    _check("gated_ffn_e4m3", x.shape, torch.bfloat16, dev, residual=residual)
-    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(C.byref(d))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
-    call("srt_gated_ffn_fwd_e4m3", C.byref(d), _p(x), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(w_down), _p(residual), _p(y), _p(scratch),
-         nbytes, _stream())
+    what, dev = "gated_ffn_e4m3", _current_device()
+    d, xp, gp, wp = _ffn(what, x, w_gate_up, w_down, torch.float8_e4m3fn, dev)
+    xs = _check(what, "x_scale", x_scale, (d.tokens,), torch.float32, dev)
+    ws = _check(what, "w_scale", w_scale, (2 * d.hidden,), torch.float32, dev)
+    rp = _check(what, "residual", residual, x.shape, torch.bfloat16, dev)
+    ref = C.byref(d)
+    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(ref)
+    scratch, y = w_down.new_empty(nbytes // 2), w_down.new_empty(x.shape)
+    call("srt_gated_ffn_fwd_e4m3", ref, xp, xs, gp, ws, wp, rp, y.data_ptr(), scratch.data_ptr(), nbytes, _raw_stream(dev))
     return y
 
 
 def gated_ffn_backward(dy, x, w_gate_up, w_down, grad_dtype=torch.bfloat16):
     """Gradients of gated_ffn at x, which is all that forward has to keep: (dx, dw_gate_up, dw_down), the weights' in
     `grad_dtype` (bfloat16, or float32 for an optimizer that accumulates there). The residual's gradient is dy itself."""
-    dev, d = _ffn("gated_ffn_backward", x, w_gate_up, w_down, torch.bfloat16)
-    _check("gated_ffn_backward", x.shape, torch.bfloat16, dev, dy=dy)
+    what, dev = "gated_ffn_backward", _current_device()
+    d, xp, gp, wp = _ffn(what, x, w_gate_up, w_down, torch.bfloat16, dev)
+    dyp = _check(what, "dy", dy, x.shape, torch.bfloat16, dev)
     if grad_dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"gated_ffn_backward: gradients in bfloat16 or float32, not {grad_dtype}")
-    g = SRT_F32 if grad_dtype == torch.float32 else SRT_BF16
+        raise TypeError(f"{what}: gradients in bfloat16 or float32, not {grad_dtype}")
+    g = SRT_F32 if grad_dtype is torch.float32 else SRT_BF16
     dx, dw_gate_up, dw_down = torch.empty_like(x), torch.empty_like(w_gate_up, dtype=grad_dtype), torch.empty_like(w_down, dtype=grad_dtype)
-    nbytes = _lib.lib().srt_gated_ffn_bwd_scratch_bytes(C.byref(d), g)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    call("srt_gated_ffn_bwd", C.byref(d), _p(dy), _p(x), _p(w_gate_up), _p(w_down), g, _p(dx), _p(dw_gate_up), _p(dw_down), _p(scratch),
-         nbytes, _stream())
+    ref = C.byref(d)
+    nbytes = _lib.lib().srt_gated_ffn_bwd_scratch_bytes(ref, g)
+    scratch = x.new_empty(nbytes // 2)
+    call("srt_gated_ffn_bwd", ref, dyp, xp, gp, wp, g, dx.data_ptr(), dw_gate_up.data_ptr(), dw_down.data_ptr(), scratch.data_ptr(), nbytes,
+         _raw_stream(dev))
     return dx, dw_gate_up, dw_down
 
 
