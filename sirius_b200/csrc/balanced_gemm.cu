@@ -96,7 +96,7 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
   uint64_t* bars = (uint64_t*)(sOut + EPI_GROUPS * SLAB_BYTES);
   const uint32_t full = smem_u32(bars), empty = full + 8 * G_MAX_STAGES, acc_full = empty + 8 * G_MAX_STAGES, acc_empty = acc_full + 16;
   uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * G_MAX_STAGES + 4);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = (int)blockIdx.x / NCTA;
   const int n_cta = p.n / NCTA;  // columns of B that this CTA stages
@@ -116,95 +116,96 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
   __syncthreads();
   if (PAIR) cluster_sync_all();  // the peer's barriers and tensor memory exist before anything refers to them
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_ptr;
-  // The B tiles of the first stages of a producer that may fetch them ahead of the launch in front: they travel while that one
-  // drains.
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  // A producer that may fetch B ahead of the launch in front enters later: its first stages travel while that one drains.
   const bool ahead = p.b_early && warp == 0;
   if (!ahead) pdl_enter();
 
   if (warp == 0) {
-    if (lane == 0) {
-      // One thread feeds the ring, and a k-block takes it a few hundred clocks: what does not change from one to the next
-      // stays out of the loops.
-      const uint32_t bytes = p.load_bytes * NCTA, full_to = PAIR ? map_to_cta(full, 0u) : full;  // the leader's barriers
-      const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
-      int it = 0, early = 0;
-      uint32_t at = 0, bar = 0, ph = 1;  // offsets of the current stage and of its barriers
-      bool ok = true;
-      auto step = [&]() {
-        at += p.stage_bytes;
-        bar += 8;
-        if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
-      };
-      auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
-        if (PAIR) tma_load_2d_pair(dst, tm, full_to + bar, x, y);
-        else tma_load_2d(dst, tm, full_to + bar, x, y);
-      };
-      auto load_a = [&](int m0, int k0) {
-        const uint32_t a = s0 + at;
-        if (A_MN) {
-          load(a, &ta, m0, k0);
-          load(a + 8192u, &ta, m0 + 64, k0);
-        } else {
-          load(a, &ta, k0, m0);
-        }
-      };
-      auto load_b = [&](int n0, int k0) {
-        const uint32_t b = s0 + at + A_BYTES;
-        if (B_MN) {
-          load(b, &tb, n0, k0);
-          if (n_cta > 64) load(b + 8192u, &tb, n0 + 64, k0);
-          if (!PAIR && n_cta > 128) {
-            load(b + 16384u, &tb, n0 + 128, k0);
-            if (n_cta > 192) load(b + 24576u, &tb, n0 + 192, k0);
-          }
-        } else {
-          load(b, &tb, k0, n0);
-        }
-      };
-      if (ahead) {
-        Walk w = walk_begin(p, unit);
-        Piece o;
-        while (early < NS && walk_next(p, unit, w, o)) {
-          int m, n;
-          tile_at(p, o.tile, m, n);
-          for (int kb = o.k0; kb < o.k1 && early < NS; ++kb, ++early) {
-            if (rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
-            load_b(n * p.n + (int)rank * n_cta, kb * 64);
-            step();
-          }
-        }
-        pdl_enter();
-        at = bar = 0;
-        ph = 1;
+    // The warp walks together and one thread of it issues (see elect_one); what does not change from one k-block to the next
+    // stays out of the loops.
+    const uint32_t bytes = p.load_bytes * NCTA, full_to = PAIR ? map_to_cta(full, 0u) : full;  // the leader's barriers
+    const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
+    int it = 0, early = 0;
+    uint32_t at = 0, bar = 0, ph = 1;  // offsets of the current stage and of its barriers
+    bool ok = true;
+    auto step = [&]() {
+      at += p.stage_bytes;
+      bar += 8;
+      if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
+    };
+    auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
+      if (PAIR) tma_load_2d_pair(dst, tm, full_to + bar, x, y);
+      else tma_load_2d(dst, tm, full_to + bar, x, y);
+    };
+    auto load_a = [&](int m0, int k0) {
+      const uint32_t a = s0 + at;
+      if (A_MN) {
+        load(a, &ta, m0, k0);
+        load(a + 8192u, &ta, m0 + 64, k0);
+      } else {
+        load(a, &ta, k0, m0);
       }
+    };
+    auto load_b = [&](int n0, int k0) {
+      const uint32_t b = s0 + at + A_BYTES;
+      if (B_MN) {
+        load(b, &tb, n0, k0);
+        if (n_cta > 64) load(b + 8192u, &tb, n0 + 64, k0);
+        if (!PAIR && n_cta > 128) {
+          load(b + 16384u, &tb, n0 + 128, k0);
+          if (n_cta > 192) load(b + 24576u, &tb, n0 + 192, k0);
+        }
+      } else {
+        load(b, &tb, k0, n0);
+      }
+    };
+    if (ahead) {
       Walk w = walk_begin(p, unit);
       Piece o;
-      while (ok && walk_next(p, unit, w, o)) {
+      while (early < NS && walk_next(p, unit, w, o)) {
         int m, n;
         tile_at(p, o.tile, m, n);
-        const int m0 = (m * NCTA + (int)rank) * BM, n0 = n * p.n + (int)rank * n_cta;
-        int k0 = o.k0 * 64;
-        const int k1 = o.k1 * 64;
-        for (; it < early && k0 < k1; k0 += 64, ++it) {
-          load_a(m0, k0);
+        for (int kb = o.k0; kb < o.k1 && early < NS; ++kb, ++early) {
+          if (elect_one()) {
+            if (rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
+            load_b(n * p.n + (int)rank * n_cta, kb * 64);
+          }
           step();
         }
-        for (; k0 < k1; k0 += 64, ++it) {
-          ok = mbar_wait(empty + bar, ph, p.status, W_GEMM_LOAD);
-          if (!ok) break;
+      }
+      pdl_enter();
+      at = bar = 0;
+      ph = 1;
+    }
+    Walk w = walk_begin(p, unit);
+    Piece o;
+    while (ok && walk_next(p, unit, w, o)) {
+      int m, n;
+      tile_at(p, o.tile, m, n);
+      const int m0 = (m * NCTA + (int)rank) * BM, n0 = n * p.n + (int)rank * n_cta;
+      int k0 = o.k0 * 64;
+      const int k1 = o.k1 * 64;
+      for (; it < early && k0 < k1; k0 += 64, ++it) {
+        if (elect_one()) load_a(m0, k0);
+        step();
+      }
+      for (; k0 < k1; k0 += 64, ++it) {
+        ok = mbar_wait_warp<false>(empty + bar, ph, p.status, W_GEMM_LOAD);
+        if (!ok) break;
+        if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
           load_a(m0, k0);
           load_b(n0, k0);
-          step();
         }
+        step();
       }
-      // a wait that gave up: the copies in flight land before the CTA's memory is given back
-      if (!ok && rank == 0)
-        for (int k = it > NS ? it - NS : 0; k < it; ++k) mbar_wait(full + 8 * (k % NS), (uint32_t)(k / NS) & 1u, p.status, W_GEMM_DRAIN);
     }
+    // a wait that gave up: the copies in flight land before the CTA's memory is given back
+    if (!ok && rank == 0)
+      for (int k = it > NS ? it - NS : 0; k < it; ++k) mbar_wait_warp<false>(full + 8 * (k % NS), (uint32_t)(k / NS) & 1u, p.status, W_GEMM_DRAIN);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t idesc = make_idesc_bf16(BM * NCTA, p.n, A_MN, B_MN);
       constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;  // 16 elements along the reduction
       const uint64_t desc_a = make_smem_desc_sw128(s0, A_MN ? 8192 : 0, 1024), desc_b = make_smem_desc_sw128(s0 + A_BYTES, B_MN ? 8192 : 0, 1024);
@@ -212,35 +213,37 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
       int i = 0;
       uint32_t at = 0, bar = 0, ph = 0;
       bool ok = true;
-      auto wait = [&](uint32_t b, uint32_t parity, int code) {
-        ok = ok && (PAIR ? mbar_wait_cluster(b, parity, p.status, code) : mbar_wait(b, parity, p.status, code));
-        if (ok) tc_fence_after_sync();
-        return ok;
-      };
       Walk w = walk_begin(p, unit);
       Piece o;
       for (; ok && walk_next(p, unit, w, o); ++i) {
         const uint32_t b2 = (uint32_t)i & 1u, acc = tmem + b2 * (uint32_t)(p.cols / 2);
-        if (!wait(acc_empty + 8 * b2, ((uint32_t)(i >> 1) & 1u) ^ 1u, W_GEMM_ACC)) break;
+        ok = mbar_wait_warp<PAIR>(acc_empty + 8 * b2, ((uint32_t)(i >> 1) & 1u) ^ 1u, p.status, W_GEMM_ACC);
+        if (!ok) break;
         uint32_t add = 0;
         for (int kb = o.k0; kb < o.k1; ++kb) {
-          if (!wait(full + bar, ph, W_GEMM_FULL)) break;
-          const uint64_t ad = desc_at(desc_a, at), bd = desc_at(desc_b, at);
+          ok = mbar_wait_warp<PAIR>(full + bar, ph, p.status, W_GEMM_FULL);
+          if (!ok) break;
+          tc_fence_after_sync();
+          if (elect_one()) {
+            const uint64_t ad = desc_at(desc_a, at), bd = desc_at(desc_b, at);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (PAIR) umma_bf16_pair(acc, desc_at(ad, k * a_step), desc_at(bd, k * b_step), idesc, k ? 1u : add);
-            else umma_bf16(acc, desc_at(ad, k * a_step), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+            for (int k = 0; k < 4; ++k) {
+              if (PAIR) umma_bf16_pair(acc, desc_at(ad, k * a_step), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+              else umma_bf16(acc, desc_at(ad, k * a_step), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+            }
+            if (PAIR) umma_commit_pair(empty + bar, (uint16_t)3);
+            else umma_commit(empty + bar);
           }
           add = 1;
-          if (PAIR) umma_commit_pair(empty + bar, (uint16_t)3);
-          else umma_commit(empty + bar);
           at += p.stage_bytes;
           bar += 8;
           if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
         }
         if (!ok) break;
-        if (PAIR) umma_commit_pair(acc_full + 8 * b2, (uint16_t)3);
-        else umma_commit(acc_full + 8 * b2);
+        if (elect_one()) {
+          if (PAIR) umma_commit_pair(acc_full + 8 * b2, (uint16_t)3);
+          else umma_commit(acc_full + 8 * b2);
+        }
       }
     }
   } else {

@@ -88,7 +88,7 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
   uint64_t* bars = (uint64_t*)(sOut + (PAIR ? epi_groups(true) * F_SLAB_BYTES : 0));
   const uint32_t full = smem_u32(bars), empty = full + 8 * F_MAX_STAGES, acc_full = empty + 8 * F_MAX_STAGES, acc_empty = acc_full + 16;
   uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * F_MAX_STAGES + 4);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
   const int unit = (int)blockIdx.x / NCTA, nunits = (int)gridDim.x / NCTA;
   const int total = p.m_units * p.n_tiles, nkb = p.k_blocks, g = p.g;
@@ -113,62 +113,63 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
   __syncthreads();
   if (PAIR) cluster_sync_all();  // the peer's barriers and tensor memory exist before anything refers to them
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_ptr;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
   pdl_enter();
 
   if (warp == 0) {
-    if (lane == 0) {
-      // One thread feeds the ring, and a k-block takes it a few hundred clocks: what does not change from one to the next
-      // stays out of the loops.
-      const uint32_t full_to = PAIR ? map_to_cta(full, 0u) : full;  // the leader's barriers
-      const uint32_t wrap = (uint32_t)NS * p.stage_bytes, gu_bytes = p.gu_bytes * NCTA, da_bytes = p.da_bytes * NCTA;
-      int it = 0;
-      uint32_t at = 0, bar = 0, ph = 1;  // offsets of the current stage and of its barriers
-      bool ok = true;
-      auto take = [&](uint32_t bytes) {
-        ok = mbar_wait(empty + bar, ph, p.status, W_FFN_LOAD);
-        if (ok && rank == 0) mbar_arrive_expect_tx(full + bar, bytes);
-        return ok;
-      };
-      auto load = [&](uint32_t offset, const CUtensorMap* tm, int x, int y) {
-        if (PAIR) tma_load_2d_pair(s0 + at + offset, tm, full_to + bar, x, y);
-        else tma_load_2d(s0 + at + offset, tm, full_to + bar, x, y);
-      };
-      auto step = [&]() {
-        ++it;
-        at += p.stage_bytes;
-        bar += 8;
-        if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
-      };
-      for (int t = unit; t < total && ok; t += nunits) {
-        int m, n;
-        tile_of(p, t, m, n);
-        const int m0 = (m * NCTA + (int)rank) * FM, n0 = n * g;
-        if (BWD) {
-          const int f0 = n0 + (PAIR ? (int)rank * 64 : 0);
-          for (int kb = 0; kb < nkb; ++kb) {
-            if (!take(da_bytes)) break;
+    // The warp walks together and one thread of it issues (see elect_one); what does not change from one k-block to the next
+    // stays out of the loops.
+    const uint32_t full_to = PAIR ? map_to_cta(full, 0u) : full;  // the leader's barriers
+    const uint32_t wrap = (uint32_t)NS * p.stage_bytes, gu_bytes = p.gu_bytes * NCTA, da_bytes = p.da_bytes * NCTA;
+    int it = 0;
+    uint32_t at = 0, bar = 0, ph = 1;  // offsets of the current stage and of its barriers
+    bool ok = true;
+    auto load = [&](uint32_t offset, const CUtensorMap* tm, int x, int y) {
+      if (PAIR) tma_load_2d_pair(s0 + at + offset, tm, full_to + bar, x, y);
+      else tma_load_2d(s0 + at + offset, tm, full_to + bar, x, y);
+    };
+    auto step = [&]() {
+      ++it;
+      at += p.stage_bytes;
+      bar += 8;
+      if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
+    };
+    for (int t = unit; t < total && ok; t += nunits) {
+      int m, n;
+      tile_of(p, t, m, n);
+      const int m0 = (m * NCTA + (int)rank) * FM, n0 = n * g;
+      if (BWD) {
+        const int f0 = n0 + (PAIR ? (int)rank * 64 : 0);
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait_warp<false>(empty + bar, ph, p.status, W_FFN_LOAD);
+          if (!ok) break;
+          if (elect_one()) {
+            if (rank == 0) mbar_arrive_expect_tx(full + bar, da_bytes);
             load(0, &tdy, kb * 64, m0);
             load(F_A_BYTES, &twd, f0, kb * 64);
             if (!PAIR && g > 64) load(F_A_BYTES + 8192, &twd, f0 + 64, kb * 64);
-            step();
           }
-        }
-        const int w0 = n0 + (PAIR ? (int)rank * p.F : 0);
-        for (int kb = 0; kb < nkb && ok; ++kb) {
-          if (!take(gu_bytes)) break;
-          load(0, &tx, kb * BKE, m0);
-          load(F_A_BYTES, &tw, kb * BKE, w0);
-          if (!PAIR) load(F_A_BYTES + (uint32_t)g * 128u, &tw, kb * BKE, p.F + n0);
           step();
         }
       }
-      // a wait that gave up: the copies in flight land before the CTA's memory is given back
-      if (!ok && rank == 0)
-        for (int k = it > NS ? it - NS : 0; k < it; ++k) mbar_wait(full + 8 * (k % NS), (uint32_t)(k / NS) & 1u, p.status, W_FFN_DRAIN);
+      const int w0 = n0 + (PAIR ? (int)rank * p.F : 0);
+      for (int kb = 0; kb < nkb && ok; ++kb) {
+        ok = mbar_wait_warp<false>(empty + bar, ph, p.status, W_FFN_LOAD);
+        if (!ok) break;
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(full + bar, gu_bytes);
+          load(0, &tx, kb * BKE, m0);
+          load(F_A_BYTES, &tw, kb * BKE, w0);
+          if (!PAIR) load(F_A_BYTES + (uint32_t)g * 128u, &tw, kb * BKE, p.F + n0);
+        }
+        step();
+      }
     }
+    // a wait that gave up: the copies in flight land before the CTA's memory is given back
+    if (!ok && rank == 0)
+      for (int k = it > NS ? it - NS : 0; k < it; ++k) mbar_wait_warp<false>(full + 8 * (k % NS), (uint32_t)(k / NS) & 1u, p.status, W_FFN_DRAIN);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t i_gu = E4M3 ? make_idesc_e4m3(FM * NCTA, PAIR ? 256 : 2 * g) : make_idesc_bf16(FM * NCTA, PAIR ? 256 : 2 * g, 0, 0);
       const uint32_t i_da = make_idesc_bf16(FM * NCTA, g, 0, 1);
       const uint64_t desc_a = make_smem_desc_sw128(s0, 0, 1024), desc_b = make_smem_desc_sw128(s0 + F_A_BYTES, 0, 1024);
@@ -177,30 +178,29 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
       int i = 0;
       uint32_t at = 0, bar = 0, ph = 0;
       bool ok = true;
-      auto wait = [&](uint32_t b, uint32_t parity, int code) {
-        ok = ok && (PAIR ? mbar_wait_cluster(b, parity, p.status, code) : mbar_wait(b, parity, p.status, code));
-        if (ok) tc_fence_after_sync();
-        return ok;
-      };
       // b_step: 16 elements along the reduction (32 in 8 bits), in a B tile that is stored along it or across it
       auto product = [&](uint32_t acc, uint32_t idesc, uint64_t db, uint32_t b_step) {
         uint32_t add = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!wait(full + bar, ph, W_FFN_FULL)) return;
-          const uint64_t ad = desc_at(desc_a, at), bd = desc_at(db, at);
+          ok = mbar_wait_warp<PAIR>(full + bar, ph, p.status, W_FFN_FULL);
+          if (!ok) return;
+          tc_fence_after_sync();
+          if (elect_one()) {
+            const uint64_t ad = desc_at(desc_a, at), bd = desc_at(db, at);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (E4M3) {
-              if (PAIR) umma_e4m3_pair(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
-              else umma_e4m3(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
-            } else {
-              if (PAIR) umma_bf16_pair(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
-              else umma_bf16(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+            for (int k = 0; k < 4; ++k) {
+              if (E4M3) {
+                if (PAIR) umma_e4m3_pair(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+                else umma_e4m3(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+              } else {
+                if (PAIR) umma_bf16_pair(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+                else umma_bf16(acc, desc_at(ad, k * 32), desc_at(bd, k * b_step), idesc, k ? 1u : add);
+              }
             }
+            if (PAIR) umma_commit_pair(empty + bar, (uint16_t)3);
+            else umma_commit(empty + bar);
           }
           add = 1;
-          if (PAIR) umma_commit_pair(empty + bar, (uint16_t)3);
-          else umma_commit(empty + bar);
           at += p.stage_bytes;
           bar += 8;
           if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
@@ -209,18 +209,24 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
       for (int t = unit; t < total && ok; t += nunits, ++i) {
         const uint32_t b = (uint32_t)i & 1u;
         // tile i - 2 has been read (parity starts so that the first two waits pass)
-        if (!wait(acc_empty + 8 * b, ((uint32_t)(i >> 1) & 1u) ^ 1u, W_FFN_ACC)) break;
+        ok = mbar_wait_warp<PAIR>(acc_empty + 8 * b, ((uint32_t)(i >> 1) & 1u) ^ 1u, p.status, W_FFN_ACC);
+        if (!ok) break;
+        tc_fence_after_sync();
         if (BWD) {
           product(tmem + (b ? 3u * quarter : 0u), i_da, desc_mn, 2048u);
           // gate and up have one accumulator: tile i - 1 has been read
-          if (i > 0 && !wait(acc_empty + 8 * (b ^ 1u), (uint32_t)((i - 1) >> 1) & 1u, W_FFN_ACC)) break;
+          if (ok && i > 0) ok = mbar_wait_warp<PAIR>(acc_empty + 8 * (b ^ 1u), (uint32_t)((i - 1) >> 1) & 1u, p.status, W_FFN_ACC);
+          if (!ok) break;
+          tc_fence_after_sync();
           product(tmem + quarter, i_gu, desc_b, 32u);
         } else {
           product(tmem + b * 2u * quarter, i_gu, desc_b, 32u);
         }
         if (!ok) break;
-        if (PAIR) umma_commit_pair(acc_full + 8 * b, (uint16_t)3);
-        else umma_commit(acc_full + 8 * b);
+        if (elect_one()) {
+          if (PAIR) umma_commit_pair(acc_full + 8 * b, (uint16_t)3);
+          else umma_commit(acc_full + 8 * b);
+        }
       }
     }
   } else {

@@ -118,6 +118,29 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
   return true;
 }
 
+// One thread of a warp whose threads all come here, the same one every time. A warp that walks its loop together, with only the
+// copies, products and commits behind this, keeps their operands in the warp's own registers: in a loop of one thread each
+// tcgen05.mma took some 100 clocks to issue, whatever its size.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred P; elect.sync _|P, 0xffffffff; selp.u32 %0, 1, 0, P; }" : "=r"(p));
+  return p != 0;
+}
+// The bounded wait of a whole warp, with one outcome. CLUSTER as in mbar_wait_cluster.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* status, int code) {
+  auto passed = [&]() { return __all_sync(0xffffffffu, CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) != 0; };
+  if (passed()) return true;
+  const long long t0 = clock64();
+  while (!passed()) {
+    if (__any_sync(0xffffffffu, clock64() - t0 > kWaitLimitCycles)) {
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+  return true;
+}
+
 // ---- proxy fences -----------------------------------------------------------------------------
 // Makes generic-proxy shared-memory writes (st.shared, completed cp.async) visible to the async
 // proxy that tcgen05.mma and TMA use.
