@@ -26,8 +26,7 @@ using bf16 = __nv_bfloat16;
 constexpr int BM = 128;
 constexpr int EPI_GROUPS = 4;                     // of four warps
 constexpr int G_THREADS = 64 + 128 * EPI_GROUPS;
-constexpr int G_MAX_STAGES = 8;
-constexpr int A_BYTES = BM * 128;
+constexpr int G_MAX_STAGES = 16;
 constexpr int SLAB_BYTES = BM * 64;  // 128 rows x 32 bf16 or 16 fp32, 64-byte swizzle
 enum { W_GEMM_LOAD = 0x41, W_GEMM_FULL = 0x42, W_GEMM_ACC = 0x43, W_GEMM_EPI = 0x44, W_GEMM_DRAIN = 0x45 };
 
@@ -38,6 +37,8 @@ struct GemmParams {
   int rest, sharers;           // ... and the first `sharers` units share the `rest` tiles beyond those
   int cols;                    // tensor-memory columns
   int stages, stage_bytes;
+  uint32_t a_bytes;            // of a stage: with fewer than 128 rows only those; the products read on into what follows, and
+                               // the rows of the accumulator that this fills are not stored
   uint32_t load_bytes;         // of one CTA a k-block
   int f32_out;
   int b_early;                 // B may be read before the launch in front of this one has ended
@@ -148,7 +149,7 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
       }
     };
     auto load_b = [&](int n0, int k0) {
-      const uint32_t b = s0 + at + A_BYTES;
+      const uint32_t b = s0 + at + p.a_bytes;
       if (B_MN) {
         load(b, &tb, n0, k0);
         if (n_cta > 64) load(b + 8192u, &tb, n0 + 64, k0);
@@ -208,7 +209,7 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
     if (rank == 0) {
       const uint32_t idesc = make_idesc_bf16(BM * NCTA, p.n, A_MN, B_MN);
       constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;  // 16 elements along the reduction
-      const uint64_t desc_a = make_smem_desc_sw128(s0, A_MN ? 8192 : 0, 1024), desc_b = make_smem_desc_sw128(s0 + A_BYTES, B_MN ? 8192 : 0, 1024);
+      const uint64_t desc_a = make_smem_desc_sw128(s0, A_MN ? 8192 : 0, 1024), desc_b = make_smem_desc_sw128(s0 + p.a_bytes, B_MN ? 8192 : 0, 1024);
       const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
       int i = 0;
       uint32_t at = 0, bar = 0, ph = 0;
@@ -336,9 +337,9 @@ balanced_gemm_kernel(const GemmParams p, const __grid_constant__ CUtensorMap ta,
 }
 
 // The tiles whose reduction was shared, found by the host: the slots of units u0 ... u1 in the order of the reduction, plus the
-// addend. Block (tile, part of its rows), eight columns a thread; a few tiles with many slots, whose loads a sum waits for in
-// turn, take fewer rows a block.
-// (Blocks that found their tile themselves, by divisions of 64-bit numbers: 10 to 16 us for 54 tiles.)
+// addend. Block (tile, part of its rows); a thread has four columns of a row, eight slots in flight.
+// (Blocks that found their tile themselves, by divisions of 64-bit numbers: 10 to 16 us for 54 tiles. Several
+// rows a thread, one after the other: 7.6 to 12 us for 54 tiles of two slots, 7.8 us for two tiles of 32.)
 constexpr int JOIN_THREADS = 256, JOIN_MAX = 160;
 struct JoinList {
   struct { int m, n, u0, u1; } t[JOIN_MAX];
@@ -348,36 +349,32 @@ balanced_gemm_join_kernel(const GemmParams p, const __grid_constant__ JoinList l
   pdl_enter();
   const int u0 = list.t[blockIdx.x].u0, u1 = list.t[blockIdx.x].u1;
   const int row0 = list.t[blockIdx.x].m * unit_rows, col0 = list.t[blockIdx.x].n * p.n;
-  const int per_row = p.n / 8;
+  const int per_row = p.n / 4;
   const size_t step = (size_t)2 * unit_rows * p.n;
-  for (int i = threadIdx.x; i < block_rows * per_row; i += JOIN_THREADS) {
-    const int r = (int)blockIdx.y * block_rows + i / per_row, c = (i % per_row) * 8;
-    if (row0 + r >= p.M || col0 + c >= p.N) continue;  // N is a multiple of eight
-    const size_t at = (size_t)(row0 + r) * p.N + col0 + c;
-    Vec16<bf16> add;
-    add.raw = make_uint4(0, 0, 0, 0);
-    if (p.addend) add.load(p.addend + at);
-    const float* f = p.slots + (size_t)u0 * step + (size_t)r * p.n + c;
-    float4 s0 = *reinterpret_cast<const float4*>(f + step / 2), s1 = *reinterpret_cast<const float4*>(f + step / 2 + 4);
-    f += step;
-#pragma unroll 4
-    for (int k = u0 + 1; k <= u1; ++k, f += step) {
-      const float4 a = *reinterpret_cast<const float4*>(f), b = *reinterpret_cast<const float4*>(f + 4);
-      s0.x += a.x; s0.y += a.y; s0.z += a.z; s0.w += a.w;
-      s1.x += b.x; s1.y += b.y; s1.z += b.z; s1.w += b.w;
-    }
-    float e[8];
-    add.unpack(e);
-    e[0] += s0.x; e[1] += s0.y; e[2] += s0.z; e[3] += s0.w;
-    e[4] += s1.x; e[5] += s1.y; e[6] += s1.z; e[7] += s1.w;
-    if (p.f32_out) {
-      float* d = (float*)p.D + at;
-      *reinterpret_cast<float4*>(d) = make_float4(e[0], e[1], e[2], e[3]);
-      *reinterpret_cast<float4*>(d + 4) = make_float4(e[4], e[5], e[6], e[7]);
-    } else {
-      add.pack(e);
-      add.store((bf16*)p.D + at);
-    }
+  const int ri = threadIdx.x / per_row, r = (int)blockIdx.y * block_rows + ri, c = (threadIdx.x - ri * per_row) * 4;
+  if (ri >= block_rows || r >= unit_rows || row0 + r >= p.M || col0 + c >= p.N) return;  // N is a multiple of eight
+  const size_t at = (size_t)(row0 + r) * p.N + col0 + c;
+  uint2 add = make_uint2(0u, 0u);
+  if (p.addend) add = *reinterpret_cast<const uint2*>(p.addend + at);
+  const float* f = p.slots + (size_t)u0 * step + (size_t)r * p.n + c;
+  float4 s = *reinterpret_cast<const float4*>(f + step / 2);
+  f += step;
+  for (int k = u0 + 1; k <= u1; k += 8, f += 8 * step) {
+    float4 a[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = k + j <= u1 ? *reinterpret_cast<const float4*>(f + j * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { s.x += a[j].x; s.y += a[j].y; s.z += a[j].z; s.w += a[j].w; }
+  }
+  s.x += __uint_as_float(add.x << 16);
+  s.y += __uint_as_float(add.x & 0xffff0000u);
+  s.z += __uint_as_float(add.y << 16);
+  s.w += __uint_as_float(add.y & 0xffff0000u);
+  if (p.f32_out) {
+    *reinterpret_cast<float4*>((float*)p.D + at) = s;
+  } else {
+    __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
+    *reinterpret_cast<uint2*>((bf16*)p.D + at) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
   }
 }
 
@@ -482,8 +479,7 @@ int launch_gemm(GemmParams& p, const GemmPlan& g, const CUtensorMap (&tm)[4], cu
   const int tiles = join_list(p, list);
   if (tiles == 0) return SRT_OK;  // every share ended with a tile
   const int rows = PAIR ? 2 * BM : BM, live = p.M < rows ? p.M : rows;
-  int block_rows = 32;
-  while (block_rows > 2 && tiles * ceil_div(live, block_rows) < 2 * sm_count()) block_rows /= 2;
+  const int block_rows = JOIN_THREADS / (g.n / 4);  // one item a thread
   SRT_CHECK_CUDA(launch_pdl(balanced_gemm_join_kernel, dim3(tiles, ceil_div(live, block_rows)), dim3(JOIN_THREADS), 0, st, p, list, rows, block_rows));
   SRT_LAUNCH_CHECK();
   return SRT_OK;
@@ -515,8 +511,9 @@ int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void
   const int nc = g.pair ? g.n / 2 : g.n;
   const int a_rows = !q.a_mn && q.M < BM ? (q.M + 7) / 8 * 8 : BM;
   const int b_bytes = q.b_mn ? ceil_div(nc, 64) * 8192 : nc * 128;
-  p.load_bytes = (uint32_t)(q.a_mn ? A_BYTES : a_rows * 128) + (uint32_t)b_bytes;
-  p.stage_bytes = A_BYTES + (b_bytes + 1023) / 1024 * 1024;
+  p.a_bytes = (uint32_t)a_rows * 128;
+  p.load_bytes = p.a_bytes + (uint32_t)b_bytes;
+  p.stage_bytes = (int)p.load_bytes;  // multiples of 1024: eight rows of 128 bytes
   p.f32_out = q.out_dtype == SRT_F32;
   p.b_early = b_early;
   p.addend = (const bf16*)addend;
@@ -528,10 +525,10 @@ int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void
   int rc;
   if ((rc = q.a_mn ? tmap_rows(&tm[0], A, q.K, q.M, q.M, 2, 64, 64) : tmap_rows(&tm[0], A, q.M, q.K, q.K, 2, 64, a_rows)) ||
       (rc = q.b_mn ? tmap_rows(&tm[1], B, q.K, q.N, q.N, 2, 64, 64) : tmap_rows(&tm[1], B, q.N, q.K, q.K, 2, 64, nc)) ||
-      (rc = tmap_rows(&tm[2], D, q.M, q.N, q.N, p.f32_out ? 4 : 2, p.f32_out ? 16 : 32, BM)))
+      (rc = tmap_rows(&tm[2], D, q.M, q.N, q.N, p.f32_out ? 4 : 2, p.f32_out ? 16 : 32, a_rows)))
     return rc;
   tm[3] = tm[2];
-  if (g.rest && (rc = tmap_rows(&tm[3], scratch, (uint64_t)2 * g.sharers * (g.pair ? 2 * BM : BM), g.n, g.n, 4, 16, BM))) return rc;
+  if (g.rest && (rc = tmap_rows(&tm[3], scratch, (uint64_t)2 * g.sharers * (g.pair ? 2 * BM : BM), g.n, g.n, 4, 16, a_rows))) return rc;
   if (q.a_mn) return g.pair ? launch_gemm<true, true, true>(p, g, tm, st) : launch_gemm<false, true, true>(p, g, tm, st);
   if (q.b_mn) return g.pair ? launch_gemm<true, false, true>(p, g, tm, st) : launch_gemm<false, false, true>(p, g, tm, st);
   return g.pair ? launch_gemm<true, false, false>(p, g, tm, st) : launch_gemm<false, false, false>(p, g, tm, st);

@@ -36,8 +36,7 @@ using bf16 = __nv_bfloat16;
 constexpr int FM = 128;                  // rows of a CTA's tile (tensor-memory lanes)
 constexpr int epi_groups(bool pair) { return pair ? 4 : 2; }                  // of four warps, behind the TMA and the MMA warp
 constexpr int ffn_threads(bool pair) { return 64 + 128 * epi_groups(pair); }
-constexpr int F_MAX_STAGES = 8;
-constexpr int F_A_BYTES = FM * 128;      // one 128-byte swizzle row of the reduction a tile row
+constexpr int F_MAX_STAGES = 16;
 constexpr int F_SLAB_BYTES = FM * 64;    // 128 x 32 bf16 on the way out, 64-byte swizzle
 enum { W_FFN_LOAD = 0x31, W_FFN_FULL = 0x32, W_FFN_ACC = 0x33, W_FFN_EPI = 0x34, W_FFN_DRAIN = 0x35 };
 
@@ -47,6 +46,8 @@ struct FfnParams {
   int g;                       // hidden channels of a tile; a pair has 128
   int cols;                    // tensor-memory columns: a power of two, at least 4 g
   int stages, stage_bytes;
+  uint32_t a_bytes;            // of a stage: with fewer than 128 tokens only their rows; the products read on into what
+                               // follows, and the rows of the accumulators that this fills are not stored
   uint32_t gu_bytes, da_bytes; // what one CTA loads a k-block in either phase
   bf16 *act, *dgu;             // outputs without a tensor map (single CTAs)
   const float *x_scale, *w_scale;
@@ -85,7 +86,7 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int NS = p.stages;
   uint8_t* sOut = base + NS * p.stage_bytes;  // a slab per epilogue group, pairs only
-  uint64_t* bars = (uint64_t*)(sOut + (PAIR ? epi_groups(true) * F_SLAB_BYTES : 0));
+  uint64_t* bars = (uint64_t*)(sOut + (PAIR ? epi_groups(true) * F_SLAB_BYTES : FM * 128 - (int)p.a_bytes));
   const uint32_t full = smem_u32(bars), empty = full + 8 * F_MAX_STAGES, acc_full = empty + 8 * F_MAX_STAGES, acc_empty = acc_full + 16;
   uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * F_MAX_STAGES + 4);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -146,8 +147,8 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
           if (elect_one()) {
             if (rank == 0) mbar_arrive_expect_tx(full + bar, da_bytes);
             load(0, &tdy, kb * 64, m0);
-            load(F_A_BYTES, &twd, f0, kb * 64);
-            if (!PAIR && g > 64) load(F_A_BYTES + 8192, &twd, f0 + 64, kb * 64);
+            load(p.a_bytes, &twd, f0, kb * 64);
+            if (!PAIR && g > 64) load(p.a_bytes + 8192, &twd, f0 + 64, kb * 64);
           }
           step();
         }
@@ -159,8 +160,8 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(full + bar, gu_bytes);
           load(0, &tx, kb * BKE, m0);
-          load(F_A_BYTES, &tw, kb * BKE, w0);
-          if (!PAIR) load(F_A_BYTES + (uint32_t)g * 128u, &tw, kb * BKE, p.F + n0);
+          load(p.a_bytes, &tw, kb * BKE, w0);
+          if (!PAIR) load(p.a_bytes + (uint32_t)g * 128u, &tw, kb * BKE, p.F + n0);
         }
         step();
       }
@@ -172,8 +173,8 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
     if (rank == 0) {
       const uint32_t i_gu = E4M3 ? make_idesc_e4m3(FM * NCTA, PAIR ? 256 : 2 * g) : make_idesc_bf16(FM * NCTA, PAIR ? 256 : 2 * g, 0, 0);
       const uint32_t i_da = make_idesc_bf16(FM * NCTA, g, 0, 1);
-      const uint64_t desc_a = make_smem_desc_sw128(s0, 0, 1024), desc_b = make_smem_desc_sw128(s0 + F_A_BYTES, 0, 1024);
-      const uint64_t desc_mn = make_smem_desc_sw128(s0 + F_A_BYTES, 8192, 1024);
+      const uint64_t desc_a = make_smem_desc_sw128(s0, 0, 1024), desc_b = make_smem_desc_sw128(s0 + p.a_bytes, 0, 1024);
+      const uint64_t desc_mn = make_smem_desc_sw128(s0 + p.a_bytes, 8192, 1024);
       const uint32_t wrap = (uint32_t)NS * p.stage_bytes;
       int i = 0;
       uint32_t at = 0, bar = 0, ph = 0;
@@ -401,7 +402,8 @@ FfnPlan plan_ffn(int T, int F, bool bwd) {
 template <bool PAIR, bool BWD, bool E4M3>
 int launch_ffn(FfnParams& p, const CUtensorMap (&tm)[7], cudaStream_t st) {
   const size_t budget = PAIR || p.cols > 256 ? 232448 : 113 * 1024;  // two single CTAs share an SM where tensor memory allows
-  const size_t fixed = 1024 + (PAIR ? epi_groups(true) * F_SLAB_BYTES : 0) + ffn_tail_bytes();
+  // a single CTA with few tokens reads up to 16 KB beyond a stage's rows
+  const size_t fixed = 1024 + (PAIR ? epi_groups(true) * F_SLAB_BYTES : FM * 128 - (int)p.a_bytes) + ffn_tail_bytes();
   p.stages = (int)((budget - fixed) / p.stage_bytes);
   if (p.stages > F_MAX_STAGES) p.stages = F_MAX_STAGES;
   const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
@@ -453,7 +455,8 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   p.da_bytes = (uint32_t)a_rows * 128u + (uint32_t)da_blocks * 8192u;
   int b_bytes = (plan.pair ? 1 : 2) * b_rows * 128;
   if (bwd && da_blocks * 8192 > b_bytes) b_bytes = da_blocks * 8192;
-  p.stage_bytes = F_A_BYTES + b_bytes;
+  p.a_bytes = (uint32_t)a_rows * 128u;
+  p.stage_bytes = (int)p.a_bytes + b_bytes;
   p.act = (bf16*)act;
   p.dgu = (bf16*)dgu;
   p.x_scale = x_scale;
