@@ -374,28 +374,41 @@ int tmap_rows_128b(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t co
 
 constexpr size_t ffn_tail_bytes() { return (2 * F_MAX_STAGES + 4) * 8 + 16; }
 
-// How a call is cut. Clocks a k-block and SM are those of the operand stream out of L2 (about 50 bytes a clock and SM), which
-// bounds either form before the tensor cores do; the form and the tile width with the shorter longest SM win.
+// How a call is cut: the least time by the model of balanced_gemm.cu, in microseconds. A k-block of a product with n columns
+// takes 0.155 at least, 1.53 ns a column, its bytes at 115 KB out of L2 (half as much again where rows do not begin on 128
+// bytes), or at 40 KB out of memory where a single row of tiles reads the weights; an epilogue takes 0.35 and 18 ns a channel,
+// in backward 30, beside the next tile's products. Measured, pair against the best single width: 8192 tokens 94 and 110 us,
+// 600 x 2048 x 5632 25 and 21, 256 x 896 x 4864 10 and 8; backward, 8192: 168 and 238, 333: 26 and 21.
 struct FfnPlan {
   bool pair;
   int g;
 };
-FfnPlan plan_ffn(int T, int F, bool bwd) {
-  const int sms = sm_count();
+FfnPlan plan_ffn(int T, int C, int F, bool bwd, int esz) {
+  const int sms = sm_count(), kb = ceil_div(C, 128 / esz);
   const int a_rows = T < FM ? (T + 7) / 8 * 8 : FM;
+  const double odd_c = C * esz % 128 ? 1.5 : 1.0, odd_f = F % 64 ? 1.5 : 1.0;
+  auto k_block = [&](double a, double b, int n, bool once) {
+    double t = 0.155;
+    auto at_least = [&](double v) { t = v > t ? v : t; };
+    at_least(0.00153 * n);
+    at_least((a + b) / 115e3);
+    if (once) at_least(b / 40e3);
+    return t;
+  };
   FfnPlan best = {false, 16};
   double best_cost = 1e30;
-  for (int g = 16; g <= 128; g += bwd ? 16 : 8) {
-    const long long tiles = (long long)ceil_div(T, FM) * ceil_div(F, g);
-    const double bytes = 128.0 * a_rows * (bwd ? 2 : 1) + 256.0 * g + (bwd ? 8192.0 * ceil_div(g, 64) : 0.0);
-    const double cost = (double)ceil_div_ll(tiles, sms) * bytes;
-    if (cost < best_cost) { best_cost = cost; best = {false, g}; }
-  }
-  if (sms >= 2) {
-    const long long tiles = (long long)ceil_div(T, 2 * FM) * ceil_div(F, 128);
-    const double cost = (double)ceil_div_ll(tiles, sms / 2) * (32768.0 + (bwd ? 24576.0 : 0.0));
-    if (cost < best_cost) best = {true, 128};
-  }
+  auto consider = [&](bool pair, int g) {
+    const int m_units = ceil_div(T, pair ? 2 * FM : FM), nc = pair ? g : 2 * g;
+    const long long tiles = (long long)m_units * ceil_div(F, g);
+    const double a = 128.0 * a_rows * odd_c;
+    double t = kb * k_block(a, 128.0 * nc * odd_c, 2 * g, m_units == 1);
+    if (bwd) t += kb * k_block(a, 8192.0 * ceil_div(pair ? g / 2 : g, 64) * odd_f, g, m_units == 1);
+    const double epi = 0.35 + (bwd ? 0.030 : 0.018) * g;
+    const double cost = (double)ceil_div_ll(tiles, pair ? sms / 2 : sms) * (t > epi ? t : epi) + epi;
+    if (cost < best_cost) { best_cost = cost; best = {pair, g}; }
+  };
+  for (int g = 16; g <= 128; g += bwd ? 16 : 8) consider(false, g);
+  if (sms >= 2) consider(true, 128);
   return best;
 }
 
@@ -438,7 +451,7 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
                    const void* dy, const void* w_down, void* act, void* dgu, cudaStream_t st) {
   const bool bwd = dy != nullptr, e4m3 = x_scale != nullptr;
   const int T = d.tokens, C = d.width, F = d.hidden, esz = e4m3 ? 1 : 2;
-  const FfnPlan plan = plan_ffn(T, F, bwd);
+  const FfnPlan plan = plan_ffn(T, C, F, bwd, esz);
   FfnParams p = {};
   p.T = T;
   p.F = F;
