@@ -403,6 +403,12 @@ int srt_step_accumulate(srt_step* s);
 /* SGD-momentum update from the accumulated gradients (or the last micro-batch's if none were
  * accumulated), then refresh of the derived weight copies (GradAccumulator.step). */
 int srt_step_optimizer(srt_step* s);
+/* Clipping of the next optimizer step (of every executor; srt_step_*, srt_gpt2_*, srt_swin_*, srt_qwen2_*): the norm of the
+ * gradients that step would consume (accumulated ones where there are any) and the coefficient min(1, max_norm / (norm +
+ * 1e-6)), which the step multiplies them by on their way in; the gradient buffer stays as it is. Call it after the last
+ * forward_backward, accumulate and gradient exchange: a later one takes it back. _grad_norm waits for the norm and reads it. */
+int srt_step_clip_grad_norm(srt_step* s, float max_norm);
+int srt_step_grad_norm(srt_step* s, float* host_norm);
 /* Scaled loss of the last micro-batch; synchronises the stream (loss.item()). */
 int srt_step_loss(srt_step* s, float* host_loss);
 int srt_step_logits(srt_step* s, float* host, int B);
@@ -459,6 +465,8 @@ int srt_gpt2_upload_tokens(srt_gpt2* g, const int32_t* host_ids, int B);
 int srt_gpt2_forward_backward(srt_gpt2* g, int B, int global_batch);
 int srt_gpt2_forward_only(srt_gpt2* g, int B);
 int srt_gpt2_optimizer(srt_gpt2* g);
+int srt_gpt2_clip_grad_norm(srt_gpt2* g, float max_norm); /* as srt_step_clip_grad_norm */
+int srt_gpt2_grad_norm(srt_gpt2* g, float* host_norm);
 int srt_gpt2_loss(srt_gpt2* g, float* host_loss);        /* synchronises; loss of the last micro-batch */
 int srt_gpt2_logits(srt_gpt2* g, float* host, int B);    /* [B*seq][vocab], after forward_only */
 int srt_gpt2_synchronize(srt_gpt2* g);
@@ -565,6 +573,8 @@ int srt_swin_upload_batch(srt_swin* s, const float* host_images /* NCHW fp32 */,
 int srt_swin_forward_backward(srt_swin* s, int B, int global_batch);
 int srt_swin_forward_only(srt_swin* s, int B);
 int srt_swin_optimizer(srt_swin* s);
+int srt_swin_clip_grad_norm(srt_swin* s, float max_norm); /* as srt_step_clip_grad_norm */
+int srt_swin_grad_norm(srt_swin* s, float* host_norm);
 int srt_swin_loss(srt_swin* s, float* host_loss);
 int srt_swin_logits(srt_swin* s, float* host, int B);
 int srt_swin_synchronize(srt_swin* s);
@@ -601,8 +611,13 @@ int srt_qwen2_get_param(srt_qwen2* g, int idx, float* host, int which);
 int srt_qwen2_commit_params(srt_qwen2* g);
 int srt_qwen2_upload_tokens(srt_qwen2* g, const int32_t* host_ids, int B);
 int srt_qwen2_forward_backward(srt_qwen2* g, int B, int global_batch);
+/* on = 1: the MLPs keep their input only and backward forms the projections again (srt_gated_ffn_bwd); 6 bytes per token, layer
+ * and intermediate channel less memory. Lays the activations out anew; what they held is gone. Default 0. */
+int srt_qwen2_recompute_mlp(srt_qwen2* g, int on);
 int srt_qwen2_forward_only(srt_qwen2* g, int B);
 int srt_qwen2_optimizer(srt_qwen2* g);
+int srt_qwen2_clip_grad_norm(srt_qwen2* g, float max_norm); /* as srt_step_clip_grad_norm */
+int srt_qwen2_grad_norm(srt_qwen2* g, float* host_norm);
 int srt_qwen2_loss(srt_qwen2* g, float* host_loss);
 int srt_qwen2_logits(srt_qwen2* g, float* host, int B);
 int srt_qwen2_synchronize(srt_qwen2* g);

@@ -21,6 +21,7 @@
 #include <atomic>
 #include "common.cuh"
 #include "grad_buckets.cuh"
+#include "grad_clip.cuh"
 #include "ops.cuh"
 #include "partition_follow.cuh"
 
@@ -89,6 +90,7 @@ struct Gpt2 {
     return SRT_OK;
   }
   GradBuckets buckets;
+  GradClip clip;  // norm of the gradients, and the coefficient of the next optimizer step
   std::atomic<int> abort_flag{0};
   static constexpr int kAhead = 4;  // layers the host may run ahead of the GPU (bounds the drain after a kill)
   cudaEvent_t ahead_ev[kAhead] = {nullptr};
@@ -574,6 +576,7 @@ int srt_gpt2_forward_backward(srt_gpt2* h, int B, int global_batch) {
   SRT_REQUIRE(g && B > 0 && B == g->cur_B && global_batch >= B, "gpt2_forward_backward: upload the tokens of this batch first");
   PartitionFollower::Scope sm_scope(g->part);
   int rc;
+  g->clip.armed = false;
   if (g->act_batch < B && (rc = g->alloc_activations(B))) return rc;  // regain after a release or a shrink
   if ((rc = g->forward(B))) return rc;
   return g->backward(B, global_batch);
@@ -594,13 +597,25 @@ int srt_gpt2_optimizer(srt_gpt2* h) {
   g->opt_steps++;
   const float* grad = g->accum_pending > 0 ? g->ACC : g->G;
   int rc = adamw(g->P, grad, g->M1, g->M2, g->Pw, (int64_t)g->n_flat, g->cfg.lr, g->cfg.beta1, g->cfg.beta2, g->cfg.eps,
-                 g->cfg.weight_decay, g->opt_steps, g->stream);
+                 g->cfg.weight_decay, g->opt_steps, g->stream, g->clip.take());
   if (rc) return rc;
   if (g->accum_pending > 0) {
     SRT_CHECK_CUDA(cudaMemsetAsync(g->ACC, 0, g->n_flat * 4, g->stream));
     g->accum_pending = 0;
   }
   return SRT_OK;
+}
+
+int srt_gpt2_clip_grad_norm(srt_gpt2* h, float max_norm) {
+  Gpt2* g = (Gpt2*)h;
+  SRT_REQUIRE(g, "gpt2_clip_grad_norm: null handle");
+  PartitionFollower::Scope sm_scope(g->part);
+  return g->clip.measure(g->accum_pending > 0 ? g->ACC : g->G, (int64_t)g->n_flat, max_norm, g->stream);
+}
+int srt_gpt2_grad_norm(srt_gpt2* h, float* host_norm) {
+  Gpt2* g = (Gpt2*)h;
+  SRT_REQUIRE(g, "gpt2_grad_norm: null handle");
+  return g->clip.read(host_norm, g->stream);
 }
 
 // Mean next-token loss of the last micro-batch over its own targets (what the reference's model returns).
@@ -651,6 +666,7 @@ int srt_gpt2_accumulate(srt_gpt2* h) {
   Gpt2* g = (Gpt2*)h;
   SRT_REQUIRE(g, "gpt2_accumulate: null handle");
   g->accum_pending++;
+  g->clip.armed = false;
   return grad_accumulate(g->ACC, g->G, (int64_t)g->n_flat, g->stream);
 }
 

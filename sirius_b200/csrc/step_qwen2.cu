@@ -20,7 +20,9 @@
 #include "../../include/sirius_pool.h"
 #include <atomic>
 #include "common.cuh"
+#include "gated_ffn.cuh"
 #include "grad_buckets.cuh"
+#include "grad_clip.cuh"
 #include "ops.cuh"
 #include "partition_follow.cuh"
 
@@ -76,6 +78,13 @@ struct Qwen2 {
     return SRT_OK;
   }
   GradBuckets buckets;
+  GradClip clip;             // norm of the gradients, and the coefficient of the next optimizer step
+  // The MLP without stored projections: forward keeps its input only and backward forms gate, up and the activation again
+  // (gated_ffn.cu). Off by default.
+  bool recompute_mlp = false;
+  void* ffn_scratch = nullptr;
+  size_t ffn_scratch_bytes = 0;
+  srt_gated_ffn_desc ffn_desc(int64_t T) const { return {(int)T, C, F}; }
   int32_t *ids = nullptr, *labels = nullptr, *order = nullptr, *seg = nullptr;
   int n_unique = 0, cur_B = 0;
   std::vector<void*> allocs;
@@ -316,17 +325,23 @@ int Qwen2::alloc_activations(int B) {
   for (Layer& y : layers) {
     if ((rc = act(&y.n1o, T * C)) || (rc = act(&y.qkv_o, T * QKV)) ||
         (rc = flash ? actf(&y.rows, attention_rows_floats(B, S, Hq)) : act(&y.Pm, BH * S * S)) ||
-        (rc = act(&y.att, T * Hq * D)) || (rc = act(&y.x2, T * C)) || (rc = act(&y.n2o, T * C)) ||
-        (rc = act(&y.gu_o, T * 2 * F)) || (rc = act(&y.act, T * F)) || (rc = act(&y.xout, T * C)))
+        (rc = act(&y.att, T * Hq * D)) || (rc = act(&y.x2, T * C)) || (rc = act(&y.n2o, T * C)) || (rc = act(&y.xout, T * C)))
       return rc;
+    if (!recompute_mlp && ((rc = act(&y.gu_o, T * 2 * F)) || (rc = act(&y.act, T * F)))) return rc;
     if ((rc = zeros(&y.z1, T)) || (rc = actf(&y.r1, T)) || (rc = zeros(&y.z2, T)) || (rc = actf(&y.r2, T))) return rc;
   }
   if ((rc = act(&nfo, T * C)) || (rc = act(&logits, T * Vpad))) return rc;
   if ((rc = zeros(&zf, T)) || (rc = actf(&rf, T)) || (rc = actf(&row_loss, T))) return rc;
   if ((rc = act(&dxa, T * C)) || (rc = act(&dxb, T * C)) || (rc = act(&dqkv, T * QKV)) || (rc = act(&t1, T * Hq * D)) ||
-      (rc = act(&dkv_h, T * Hq * D)) || (rc = act(&dgu, T * 2 * F)) || (rc = act(&dact, T * F)) ||
-      (rc = act(&datt, T * Hq * D)) || (rc = act(&dln, T * C)))
+      (rc = act(&dkv_h, T * Hq * D)) || (rc = act(&datt, T * Hq * D)) || (rc = act(&dln, T * C)))
     return rc;
+  if (recompute_mlp) {
+    const size_t fwd = gated_ffn_fwd_scratch_bytes(ffn_desc(T)), bwd = gated_ffn_scratch(ffn_desc(T), SRT_F32).total;
+    ffn_scratch_bytes = fwd > bwd ? fwd : bwd;
+    if ((rc = aalloc(&ffn_scratch, ffn_scratch_bytes))) return rc;
+  } else if ((rc = act(&dgu, T * 2 * F)) || (rc = act(&dact, T * F))) {
+    return rc;
+  }
   if (!flash && ((rc = act(&dP, BH * S * S)) || (rc = act(&Tbig, BH * S * S)) || (rc = act(&t2, T * Hq * D))))
     return rc;
   act_batch = B;
@@ -401,9 +416,16 @@ int Qwen2::forward(int B) {
     if ((rc = attention_forward(y, B, scale))) return rc;
     if ((rc = linear_fwd(y.o, y.att, y.x2, x, T))) return rc;
     if ((rc = rmsnorm_fwd(y.x2, pf(y.n2), y.n2o, y.z2, y.r2, T, C, cfg.rms_eps, stream))) return rc;
-    if ((rc = linear_fwd(y.gu, y.n2o, y.gu_o, nullptr, T))) return rc;
-    if ((rc = swiglu_fwd(y.gu_o, y.act, T, F, stream))) return rc;
-    if ((rc = linear_fwd(y.down, y.act, y.xout, y.x2, T))) return rc;
+    if (recompute_mlp) {
+      const srt_gated_ffn_desc d = ffn_desc(T);
+      if ((rc = gated_ffn_fwd(&d, y.n2o, nullptr, Pw + y.gu.w_off, nullptr, Pw + y.down.w_off, y.x2, y.xout, ffn_scratch, ffn_scratch_bytes,
+                              false, stream)))
+        return rc;
+    } else {
+      if ((rc = linear_fwd(y.gu, y.n2o, y.gu_o, nullptr, T))) return rc;
+      if ((rc = swiglu_fwd(y.gu_o, y.act, T, F, stream))) return rc;
+      if ((rc = linear_fwd(y.down, y.act, y.xout, y.x2, T))) return rc;
+    }
     x = y.xout;
   }
   if ((rc = rmsnorm_fwd(x, pf(nf), nfo, zf, rf, T, C, cfg.rms_eps, stream))) return rc;
@@ -438,9 +460,16 @@ int Qwen2::backward(int B, int global_batch) {
     const __nv_bfloat16* xin = i == 0 ? x0 : layers[i - 1].xout;
     if ((rc = checkpoint())) return rc;
     // MLP
-    if ((rc = linear_bwd(y.down, dx, y.act, dact, T))) return rc;
-    if ((rc = swiglu_bwd(dact, y.gu_o, dgu, T, F, stream))) return rc;
-    if ((rc = linear_bwd(y.gu, dgu, y.n2o, dln, T))) return rc;
+    if (recompute_mlp) {
+      const srt_gated_ffn_desc d = ffn_desc(T);
+      if ((rc = gated_ffn_bwd(&d, dx, y.n2o, Pw + y.gu.w_off, Pw + y.down.w_off, SRT_F32, dln, G + y.gu.w_off, G + y.down.w_off, ffn_scratch,
+                              ffn_scratch_bytes, stream)))
+        return rc;
+    } else {
+      if ((rc = linear_bwd(y.down, dx, y.act, dact, T))) return rc;
+      if ((rc = swiglu_bwd(dact, y.gu_o, dgu, T, F, stream))) return rc;
+      if ((rc = linear_bwd(y.gu, dgu, y.n2o, dln, T))) return rc;
+    }
     if ((rc = rmsnorm_bwd(dln, y.x2, pf(y.n2), y.z2, y.r2, dx, dx_other, gf(y.n2), T, C, scratch, scratch_bytes, stream)))
       return rc;
     // attention
@@ -559,6 +588,7 @@ int srt_qwen2_forward_backward(srt_qwen2* h, int B, int global_batch) {
   SRT_REQUIRE(g && B > 0 && B == g->cur_B && global_batch >= B, "qwen2_forward_backward: upload the tokens of this batch first");
   PartitionFollower::Scope sm_scope(g->part);
   int rc;
+  g->clip.armed = false;
   if (g->act_batch < B && (rc = g->alloc_activations(B))) return rc;  // regain after a release or a shrink
   if ((rc = g->forward(B))) return rc;
   return g->backward(B, global_batch);
@@ -579,13 +609,36 @@ int srt_qwen2_optimizer(srt_qwen2* h) {
   g->opt_steps++;
   const float* grad = g->accum_pending > 0 ? g->ACC : g->G;
   int rc = adamw(g->P, grad, g->M1, g->M2, g->Pw, (int64_t)g->n_flat, g->cfg.lr, g->cfg.beta1, g->cfg.beta2, g->cfg.eps,
-                 g->cfg.weight_decay, g->opt_steps, g->stream);
+                 g->cfg.weight_decay, g->opt_steps, g->stream, g->clip.take());
   if (rc) return rc;
   if (g->accum_pending > 0) {
     SRT_CHECK_CUDA(cudaMemsetAsync(g->ACC, 0, g->n_flat * 4, g->stream));
     g->accum_pending = 0;
   }
   return SRT_OK;
+}
+
+int srt_qwen2_clip_grad_norm(srt_qwen2* h, float max_norm) {
+  Qwen2* g = (Qwen2*)h;
+  SRT_REQUIRE(g, "qwen2_clip_grad_norm: null handle");
+  PartitionFollower::Scope sm_scope(g->part);
+  return g->clip.measure(g->accum_pending > 0 ? g->ACC : g->G, (int64_t)g->n_flat, max_norm, g->stream);
+}
+int srt_qwen2_grad_norm(srt_qwen2* h, float* host_norm) {
+  Qwen2* g = (Qwen2*)h;
+  SRT_REQUIRE(g, "qwen2_grad_norm: null handle");
+  return g->clip.read(host_norm, g->stream);
+}
+
+int srt_qwen2_recompute_mlp(srt_qwen2* h, int on) {
+  Qwen2* g = (Qwen2*)h;
+  SRT_REQUIRE(g, "qwen2_recompute_mlp: null handle");
+  if (g->recompute_mlp == (on != 0)) return SRT_OK;
+  const int B = g->act_batch;
+  int rc = g->free_activation_blocks();
+  if (rc) return rc;
+  g->recompute_mlp = on != 0;
+  return B > 0 ? g->alloc_activations(B) : (int)SRT_OK;
 }
 
 int srt_qwen2_loss(srt_qwen2* h, float* host_loss) {
@@ -648,6 +701,7 @@ int srt_qwen2_accumulate(srt_qwen2* h) {
   Qwen2* g = (Qwen2*)h;
   SRT_REQUIRE(g, "qwen2_accumulate: null handle");
   g->accum_pending++;
+  g->clip.armed = false;
   return grad_accumulate(g->ACC, g->G, (int64_t)g->n_flat, g->stream);
 }
 

@@ -17,6 +17,7 @@
 #include "../../include/sirius_pool.h"
 #include "../../include/sirius_runtime.h"
 #include "common.cuh"
+#include "grad_clip.cuh"
 #include "ops.cuh"
 
 
@@ -154,6 +155,7 @@ struct Step {
   int opt_steps = 0;
   bool eval_mode = false;  // forward with BatchNorm running statistics (the inference stand-in)
   int accum_pending = 0;
+  GradClip clip;  // norm of the gradients, and the coefficient of the next optimizer step
   size_t act_bytes = 0;
 
   // Releasable part of the step's memory: saved activations, gradient ping-pong buffers, scratch.
@@ -1175,6 +1177,7 @@ int srt_step_forward_backward(srt_step* h, int B, int global_batch) {
   SRT_REQUIRE(s && B > 0 && B <= s->cfg.max_batch && global_batch >= B, "forward_backward: bad batch sizes");
   Step::SmScope sm_scope(s);
   int rc;
+  s->clip.armed = false;
   if ((rc = s->adopt_upload())) return rc;
   if (s->act_batch < B && (rc = s->alloc_activations(B))) return rc;  // regain after a release
   rc = s->forward(B);
@@ -1218,7 +1221,21 @@ int srt_step_accumulate(srt_step* h) {
   SRT_REQUIRE(s, "accumulate: null handle");
   Step::SmScope sm_scope(s);
   s->accum_pending++;
+  s->clip.armed = false;
   return grad_accumulate(s->ACC, s->G, (int64_t)s->n_flat, s->stream);
+}
+
+int srt_step_clip_grad_norm(srt_step* h, float max_norm) {
+  Step* s = (Step*)h;
+  SRT_REQUIRE(s, "clip_grad_norm: null handle");
+  Step::SmScope sm_scope(s);
+  if (int jr = s->join_side()) return jr;
+  return s->clip.measure(s->accum_pending > 0 ? s->ACC : s->G, (int64_t)s->n_flat, max_norm, s->stream);
+}
+int srt_step_grad_norm(srt_step* h, float* host_norm) {
+  Step* s = (Step*)h;
+  SRT_REQUIRE(s, "grad_norm: null handle");
+  return s->clip.read(host_norm, s->stream);
 }
 
 int srt_step_optimizer(srt_step* h) {
@@ -1228,9 +1245,10 @@ int srt_step_optimizer(srt_step* h) {
   if (int jr = s->join_side()) return jr;  // the parameters' working copy must not change under a reader
   const float* grad = s->accum_pending > 0 ? s->ACC : s->G;
   const bool bf = s->cfg.dtype == SRT_BF16;
+  const float* coefficient = s->clip.take();
   int rc = s->timed(SRT_PROF_OPTIM, (double)s->n_flat * (bf ? 22 : 20), [&] {
     return sgd_momentum(s->P, grad, s->M, bf ? s->Pw : nullptr, (int64_t)s->n_flat, s->cfg.lr, s->cfg.momentum,
-                        s->cfg.weight_decay, s->opt_steps == 0, s->stream); });
+                        s->cfg.weight_decay, s->opt_steps == 0, s->stream, coefficient); });
   if (rc) return rc;
   if (s->accum_pending > 0) {
     SRT_CHECK_CUDA(cudaMemsetAsync(s->ACC, 0, s->n_flat * 4, s->stream));

@@ -17,6 +17,7 @@
 #include "../../include/sirius_b200.h"
 #include "common.cuh"
 #include "grad_buckets.cuh"
+#include "grad_clip.cuh"
 #include "ops.cuh"
 #include "partition_follow.cuh"
 
@@ -85,7 +86,8 @@ struct Swin {
     SRT_CHECK_CUDA(cudaStreamWaitEvent(stream, ev_join, 0));
     return SRT_OK;
   }
-  GradBuckets buckets;      // units: the blocks in forward order, each stage's patch merging counted with its last block
+  GradBuckets buckets;
+  GradClip clip;  // norm of the gradients, and the coefficient of the next optimizer step      // units: the blocks in forward order, each stage's patch merging counted with its last block
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
   std::vector<void*> allocs;
@@ -556,6 +558,7 @@ int srt_swin_forward_backward(srt_swin* h, int B, int global_batch) {
   Swin* g = (Swin*)h;
   SRT_REQUIRE(g && B > 0 && B == g->cur_B && global_batch >= B, "swin_forward_backward: upload this batch first");
   PartitionFollower::Scope sm_scope(g->part);
+  g->clip.armed = false;
   int rc = g->forward(B);
   if (rc) return rc;
   return g->backward(B, global_batch);
@@ -574,9 +577,21 @@ int srt_swin_optimizer(srt_swin* h) {
   PartitionFollower::Scope sm_scope(g->part);
   g->opt_steps++;
   int rc = adamw(g->P, g->G, g->M1, g->M2, g->Pw, (int64_t)g->n_flat, g->cfg.lr, g->cfg.beta1, g->cfg.beta2, g->cfg.eps,
-                 g->cfg.weight_decay, g->opt_steps, g->stream);
+                 g->cfg.weight_decay, g->opt_steps, g->stream, g->clip.take());
   if (rc) return rc;
   return SRT_OK;
+}
+
+int srt_swin_clip_grad_norm(srt_swin* h, float max_norm) {
+  Swin* g = (Swin*)h;
+  SRT_REQUIRE(g, "swin_clip_grad_norm: null handle");
+  PartitionFollower::Scope sm_scope(g->part);
+  return g->clip.measure(g->G, (int64_t)g->n_flat, max_norm, g->stream);
+}
+int srt_swin_grad_norm(srt_swin* h, float* host_norm) {
+  Swin* g = (Swin*)h;
+  SRT_REQUIRE(g, "swin_grad_norm: null handle");
+  return g->clip.read(host_norm, g->stream);
 }
 
 // Mean cross-entropy of the last micro-batch.

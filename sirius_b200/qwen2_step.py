@@ -34,7 +34,10 @@ register({
     "srt_qwen2_commit_params": (None, [_vp]),
     "srt_qwen2_upload_tokens": (None, [_vp, _vp, _i]),
     "srt_qwen2_forward_backward": (None, [_vp, _i, _i]),
+    "srt_qwen2_recompute_mlp": (None, [_vp, _i]),
     "srt_qwen2_forward_only": (None, [_vp, _i]),
+    "srt_qwen2_clip_grad_norm": (None, [_vp, _f]),
+    "srt_qwen2_grad_norm": (None, [_vp, C.POINTER(_f)]),
     "srt_qwen2_optimizer": (None, [_vp]),
     "srt_qwen2_loss": (None, [_vp, C.POINTER(_f)]),
     "srt_qwen2_logits": (None, [_vp, _vp, _i]),
@@ -55,13 +58,16 @@ class Qwen2Step(GradBucketsMixin):
     `transformers.Qwen2ForCausalLM.state_dict()` (`lm_head.weight` is the tied token table and is not listed)."""
 
     def __init__(self, n_layer=24, n_head=14, n_kv_head=2, hidden=896, intermediate=4864, vocab=151936, max_batch=4, seq=2048,
-                 rope_theta=1e6, rms_eps=1e-6, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, pool=None):
+                 rope_theta=1e6, rms_eps=1e-6, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, pool=None,
+                 recompute_mlp=False):
         cfg = Qwen2ConfigC(n_layer, n_head, n_kv_head, hidden, intermediate, vocab, max_batch, seq, rope_theta, rms_eps, lr,
                            betas[0], betas[1], eps, weight_decay)
         self.cfg, self.seq, self.vocab, self.max_batch = cfg, seq, vocab, max_batch
         self._h = _vp()
         self.pool = pool
         call("srt_qwen2_create_with_pool", C.byref(cfg), pool if pool else None, C.byref(self._h))
+        if recompute_mlp:
+            self.recompute_mlp()
         self.params = {}
         name, shape, ndim = C.create_string_buffer(256), (_i64 * 2)(), _i()
         for i in range(_lib.lib().srt_qwen2_num_params(self._h)):
@@ -102,11 +108,26 @@ class Qwen2Step(GradBucketsMixin):
         self._B = a.shape[0]
         call("srt_qwen2_upload_tokens", self._h, a.ctypes.data_as(_vp), self._B)
 
+    def recompute_mlp(self, on: bool = True) -> None:
+        """The MLPs keep their input only; backward forms their projections again. Saves 6 bytes per token, layer and
+        intermediate channel."""
+        call("srt_qwen2_recompute_mlp", self._h, int(on))
+
     def forward_backward(self, global_batch=None) -> None:
         call("srt_qwen2_forward_backward", self._h, self._B, global_batch or self._B)
 
     def forward_only(self) -> None:
         call("srt_qwen2_forward_only", self._h, self._B)
+
+    def clip_grad_norm(self, max_norm: float) -> None:
+        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them)."""
+        call("srt_qwen2_clip_grad_norm", self._h, max_norm)
+
+    def grad_norm(self) -> float:
+        """The norm that clip_grad_norm found; waits for it."""
+        v = C.c_float()
+        call("srt_qwen2_grad_norm", self._h, C.byref(v))
+        return v.value
 
     def optimizer_step(self) -> None:
         call("srt_qwen2_optimizer", self._h)

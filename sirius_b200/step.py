@@ -35,6 +35,8 @@ register({
     "srt_step_forward_only": (None, [_vp, _i]),
     "srt_step_forward_infer": (None, [_vp, _i]),
     "srt_step_accumulate": (None, [_vp]),
+    "srt_step_clip_grad_norm": (None, [_vp, C.c_float]),
+    "srt_step_grad_norm": (None, [_vp, C.POINTER(C.c_float)]),
     "srt_step_optimizer": (None, [_vp]),
     "srt_step_loss": (None, [_vp, C.POINTER(C.c_float)]),
     "srt_step_logits": (None, [_vp, _vp, _i]),
@@ -161,6 +163,16 @@ class ResNetStep:
 
     def accumulate(self) -> None:
         call("srt_step_accumulate", self._h)
+
+    def clip_grad_norm(self, max_norm: float) -> None:
+        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them)."""
+        call("srt_step_clip_grad_norm", self._h, max_norm)
+
+    def grad_norm(self) -> float:
+        """The norm that clip_grad_norm found; waits for it."""
+        v = C.c_float()
+        call("srt_step_grad_norm", self._h, C.byref(v))
+        return v.value
 
     def optimizer_step(self) -> None:
         call("srt_step_optimizer", self._h)

@@ -32,6 +32,8 @@ register({
     "srt_swin_upload_batch": (None, [_vp, _vp, _vp, _i]),
     "srt_swin_forward_backward": (None, [_vp, _i, _i]),
     "srt_swin_forward_only": (None, [_vp, _i]),
+    "srt_swin_clip_grad_norm": (None, [_vp, _f]),
+    "srt_swin_grad_norm": (None, [_vp, C.POINTER(_f)]),
     "srt_swin_optimizer": (None, [_vp]),
     "srt_swin_loss": (None, [_vp, C.POINTER(_f)]),
     "srt_swin_logits": (None, [_vp, _vp, _i]),
@@ -100,6 +102,16 @@ class SwinStep(GradBucketsMixin):
 
     def forward_only(self) -> None:
         call("srt_swin_forward_only", self._h, self._B)
+
+    def clip_grad_norm(self, max_norm: float) -> None:
+        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them)."""
+        call("srt_swin_clip_grad_norm", self._h, max_norm)
+
+    def grad_norm(self) -> float:
+        """The norm that clip_grad_norm found; waits for it."""
+        v = C.c_float()
+        call("srt_swin_grad_norm", self._h, C.byref(v))
+        return v.value
 
     def optimizer_step(self) -> None:
         call("srt_swin_optimizer", self._h)
