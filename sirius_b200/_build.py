@@ -15,6 +15,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "build"
 LIB = PKG / "libsirius_b200.so"
+BINDING_SRC = CSRC / "binding" / "ops_module.cpp"
+BINDING = PKG / "_ops_native.so"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 NVCC_FLAGS = [
@@ -48,6 +50,25 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
                 print(line)
 
 
+def _build_binding(force: bool) -> None:
+    """The native front ends of ops.py, against the torch of this interpreter (found, not imported)."""
+    import importlib.util
+    import sysconfig
+    torch_dir = Path(next(iter(importlib.util.find_spec("torch").submodule_search_locations)))
+    newest = max(BINDING_SRC.stat().st_mtime, *(h.stat().st_mtime for h in (PKG.parent / "include").glob("*.h")))
+    if not force and BINDING.exists() and BINDING.stat().st_mtime >= newest:
+        return
+    cuda = Path(NVCC).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}",
+           "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda / "include"), str(BINDING_SRC), "-o", str(BINDING), f"-L{torch_dir / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed on {BINDING_SRC.name}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every source for sm_100a and link the shared library. Returns its path."""
     BUILD.mkdir(exist_ok=True)
@@ -59,9 +80,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         stale = force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, newest_hdr)
         if stale:
             jobs.append((src, obj))
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
-            list(ex.map(lambda j: _compile(j[0], j[1], verbose), jobs))
+    with ThreadPoolExecutor(max_workers=max(1, min(8, len(jobs) + 1))) as ex:
+        binding = ex.submit(_build_binding, force)
+        list(ex.map(lambda j: _compile(j[0], j[1], verbose), jobs))
+        binding.result()
     if jobs or not LIB.exists():
         cmd = [NVCC, "-shared", "-o", str(LIB), *map(str, objs), "-lpthread", "-lrt", "-ldl"]
         res = subprocess.run(cmd, capture_output=True, text=True)

@@ -3,7 +3,6 @@ buffers) and calls one entry point on the current stream. Layouts are NHWC / KRS
 from __future__ import annotations
 
 import ctypes as C
-from array import array
 
 import torch
 
@@ -26,34 +25,26 @@ def _p(t):
     return t.data_ptr()
 
 
-_current_device = torch.cuda.current_device
-_raw_stream = torch._C._cuda_getCurrentRawStream   # the handle without the Stream object around it, which takes 3 us to make
-
-
 def _stream():
-    return _raw_stream(_current_device())
+    return torch.cuda.current_stream().cuda_stream
 
 
-def _wrong(what, name, t, shape, dtype, dev):
-    """The error that _check's operand deserves."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be a contiguous CUDA tensor")
-    if t.get_device() != dev:
-        raise ValueError(f"{what}: {name} is on {t.device}; operands are on the current device, cuda:{dev}")
-    if dtype is not None and t.dtype is not dtype:
-        raise TypeError(f"{what}: {name} is {t.dtype}, not {dtype}")
-    raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+_ops_native = None
 
 
-def _check(what, name, t, shape, dtype, dev):
-    """Address of a contiguous CUDA tensor of this shape and type on the current device `dev` (whose stream the call goes to).
-    None gives None; a shape or type of None is not looked at."""
-    if t is None:
-        return None
-    if (not isinstance(t, torch.Tensor) or t.get_device() != dev or not t.is_contiguous() or (dtype is not None and t.dtype is not dtype)
-            or (shape is not None and t.shape != shape)):
-        _wrong(what, name, t, shape, dtype, dev)
-    return t.data_ptr()
+def _native():
+    """The native front ends (csrc/binding/ops_module.cpp), bound to the library that _lib has loaded."""
+    global _ops_native
+    if _ops_native is None:
+        _lib.lib()
+        try:
+            from . import _ops_native as module
+        except ImportError as e:
+            raise _lib.SrtError("sirius_b200/_ops_native.so is missing or does not fit this torch: build it with "
+                                f"`python -m sirius_b200._build` ({e})") from e
+        module.bind(str(_lib.LIB_PATH), _lib.SrtError)
+        _ops_native = module
+    return _ops_native
 
 
 def _ep(bias, addend, addend_bits=None):
@@ -256,8 +247,7 @@ def colsum(dy):
 def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None, clip=None):
     """`clip` as in adamw."""
     if clip is not None:
-        pp, gp, mp, _, bp, cp, st = _clip_operands("sgd_momentum", p, g, m, None, p_bf16, clip)
-        call("srt_sgd_momentum_clipped", pp, gp, mp, bp, p.numel(), lr, mu, wd, int(first_step), cp, st)
+        (_ops_native or _native()).sgd_momentum_clipped(p, g, m, lr, mu, wd, first_step, p_bf16, clip)
         return
     call("srt_sgd_momentum", _p(p), _p(g), _p(m), _p(p_bf16), p.numel(), lr, mu, wd, int(first_step), _stream())
 
@@ -265,174 +255,67 @@ def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None, clip=None):
 def adamw(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16=None, clip=None):
     """`clip`: what grad_norm returned; the gradients are multiplied by its coefficient on the way in."""
     if clip is not None:
-        pp, gp, mp, vp, bp, cp, st = _clip_operands("adamw", p, g, m, v, p_bf16, clip)
-        call("srt_adamw_clipped", pp, gp, mp, vp, bp, p.numel(), lr, b1, b2, eps, wd, step, cp, st)
+        (_ops_native or _native()).adamw_clipped(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16, clip)
         return
     call("srt_adamw", _p(p), _p(g), _p(m), _p(v), _p(p_bf16), p.numel(), lr, b1, b2, eps, wd, step, _stream())
 
 
-def _clip_operands(what, p, g, m, v, p_bf16, clip):
-    dev, f32 = _current_device(), torch.float32
-    pp = _check(what, "p", p, None, f32, dev)
-    shape = p.shape
-    return (pp, _check(what, "g", g, shape, f32, dev), _check(what, "m", m, shape, f32, dev), _check(what, "v", v, shape, f32, dev),
-            _check(what, "p_bf16", p_bf16, shape, torch.bfloat16, dev), _check(what, "clip", clip, (2,), f32, dev), _raw_stream(dev))
-
-
-def _grad_list(name, grads, max_norm):
-    if not max_norm > 0:
-        raise ValueError(f"{name}: max_norm ({max_norm}) must be positive")
-    dev = _current_device()
-    if not isinstance(grads, (list, tuple)):
-        grads = list(grads)
-    n = len(grads)
-    dtype = grads[0].dtype if n else torch.float32
-    for g in grads:
-        if g.get_device() != dev or g.dtype is not dtype or not g.is_contiguous():
-            _wrong(name, "a gradient", g, None, dtype, dev)
-    kind = _dt(grads[0]) if n else SRT_F32
-    # addresses and counts behind one another, read by the call before it returns
-    words = array("q", [g.data_ptr() for g in grads])
-    words.extend([g.numel() for g in grads])
-    at = words.buffer_info()[0]
-    nbytes = _lib.lib().srt_grad_norm_scratch_bytes(n)
-    # the results first, the partial sums behind them
-    work = torch.empty(64 + nbytes // 4, dtype=torch.float32, device="cuda")
-    base = work.data_ptr()
-    call("srt_" + name, kind, n, at, at + 8 * n, max_norm, base, base + 256, nbytes, _raw_stream(dev))
-    return work[:2]
-
-
+# ---- operators of the decoder's feed-forward half and of its optimizer step -------------------------------------
+# Tensors are contiguous CUDA tensors on the current device, and the call goes to its current stream; anything else raises
+# ValueError or TypeError and names the operand.
 def grad_norm(grads, max_norm):
-    """Norm of all gradients together (a list of tensors of one type) and the coefficient that brings it down to `max_norm`,
-    min(1, max_norm / (norm + 1e-6)): a device tensor of these two, for the `clip` argument of the optimizer steps."""
-    return _grad_list("grad_norm", grads, max_norm)
+    """Norm of all gradients together (a list of tensors, all float32 or all bfloat16) and the coefficient that brings it down
+    to `max_norm`, min(1, max_norm / (norm + 1e-6)): a device tensor of these two, for the `clip` argument of the optimizer
+    steps."""
+    return (_ops_native or _native()).grad_norm(grads, max_norm, False)
 
 
 def clip_grad_norm(grads, max_norm):
-    """grad_norm that also multiplies the gradients by the coefficient, in place (torch.nn.utils.clip_grad_norm_)."""
-    return _grad_list("clip_grad_norm", grads, max_norm)
-
-
-def _row_type(what, x):
-    if not isinstance(x, torch.Tensor) or x.dim() < 1:
-        raise ValueError(f"{what}: rows in a CUDA tensor are wanted")
-    if x.dtype is torch.bfloat16:
-        return SRT_BF16
-    if x.dtype is torch.float32:
-        return SRT_F32
-    raise TypeError(f"{what}: rows of float32 or bfloat16 are wanted, not {x.dtype}")
+    """grad_norm that also multiplies the gradients by the coefficient, in place (torch.nn.utils.clip_grad_norm_). No two of
+    them overlap."""
+    return (_ops_native or _native()).grad_norm(grads, max_norm, True)
 
 
 def rmsnorm(x, gamma, eps=1e-6, residual=None):
-    """h = x + residual, y = gamma * h / rms(h) over the last axis: returns (y, h, rstd). Without a residual h is x itself."""
-    kind, dev = _row_type("rmsnorm", x), _current_device()
-    shape = x.shape
-    xp = _check("rmsnorm", "x", x, None, None, dev)
-    rp = _check("rmsnorm", "residual", residual, shape, x.dtype, dev)
-    gp = _check("rmsnorm", "gamma", gamma, shape[-1:], torch.float32, dev)
-    y = torch.empty_like(x)
-    h = x if residual is None else torch.empty_like(x)
-    rstd = gamma.new_empty(shape[:-1])
-    call("srt_rmsnorm_fwd", kind, xp, rp, gp, None if residual is None else h.data_ptr(), y.data_ptr(), rstd.data_ptr(), rstd.numel(),
-         shape[-1], eps, _raw_stream(dev))
-    return y, h, rstd
+    """h = x + residual, y = gamma * h / rms(h) over the last axis, x in bfloat16 or float32, gamma in float32: returns
+    (y, h, rstd). Without a residual h is x itself."""
+    return (_ops_native or _native()).rmsnorm(x, gamma, eps, residual)
 
 
 def rmsnorm_e4m3(x, gamma, eps=1e-6, residual=None):
     """rmsnorm whose output leaves in 8 bits, q * scale of its row: returns (q, scale, h, rstd)."""
-    kind, dev = _row_type("rmsnorm_e4m3", x), _current_device()
-    shape = x.shape
-    xp = _check("rmsnorm_e4m3", "x", x, None, None, dev)
-    rp = _check("rmsnorm_e4m3", "residual", residual, shape, x.dtype, dev)
-    gp = _check("rmsnorm_e4m3", "gamma", gamma, shape[-1:], torch.float32, dev)
-    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    h = x if residual is None else torch.empty_like(x)
-    rstd, scale = gamma.new_empty(shape[:-1]), gamma.new_empty(shape[:-1])
-    call("srt_rmsnorm_fwd_e4m3", kind, xp, rp, gp, None if residual is None else h.data_ptr(), q.data_ptr(), scale.data_ptr(), rstd.data_ptr(),
-         rstd.numel(), shape[-1], eps, _raw_stream(dev))
-    return q, scale, h, rstd
+    return (_ops_native or _native()).rmsnorm_e4m3(x, gamma, eps, residual)
 
 
 def quantize_rows_e4m3(x):
     """Rows (of weights, say) in 8 bits: (q, scale) with x close to q * scale."""
-    kind, dev = _row_type("quantize_rows_e4m3", x), _current_device()
-    xp = _check("quantize_rows_e4m3", "x", x, None, None, dev)
-    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    call("srt_quantize_rows_e4m3", kind, xp, q.data_ptr(), scale.data_ptr(), scale.numel(), x.shape[-1], _raw_stream(dev))
-    return q, scale
+    return (_ops_native or _native()).quantize_rows_e4m3(x)
 
 
 def rmsnorm_backward(dy, h, gamma, rstd, dh=None):
     """Gradient of rmsnorm at the h and rstd that it returned: (dx, dgamma). dx is the gradient of x and of the residual; `dh`
     is what reaches h from elsewhere (the residual path) and is added to it."""
-    what = "rmsnorm_backward"
-    kind, dev = _row_type(what, h), _current_device()
-    shape, dtype = h.shape, h.dtype
-    hp = _check(what, "h", h, None, None, dev)
-    dyp, dhp = _check(what, "dy", dy, shape, dtype, dev), _check(what, "dh", dh, shape, dtype, dev)
-    gp, rp = _check(what, "gamma", gamma, shape[-1:], torch.float32, dev), _check(what, "rstd", rstd, shape[:-1], torch.float32, dev)
-    dx, dgamma = torch.empty_like(h), torch.empty_like(gamma)
-    nbytes = _lib.lib().srt_rmsnorm_bwd_scratch_bytes(shape[-1])
-    scratch = gamma.new_empty(nbytes // 4)
-    call("srt_rmsnorm_bwd", kind, dyp, hp, gp, rp, dhp, dx.data_ptr(), dgamma.data_ptr(), rstd.numel(), shape[-1], scratch.data_ptr(), nbytes,
-         _raw_stream(dev))
-    return dx, dgamma
-
-
-def _ffn(what, x, w_gate_up, w_down, dtype, dev):
-    if not all(isinstance(t, torch.Tensor) and t.dim() == 2 for t in (x, w_gate_up, w_down)) or w_gate_up.shape[0] != 2 * w_down.shape[1]:
-        raise ValueError(f"{what}: x [tokens, width], w_gate_up [2 hidden, width] and w_down [width, hidden] are wanted")
-    tokens, width = x.shape
-    hidden = w_down.shape[1]
-    d = _lib.GatedFfnDesc(tokens, width, hidden)
-    return (d, _check(what, "x", x, None, dtype, dev), _check(what, "w_gate_up", w_gate_up, (2 * hidden, width), dtype, dev),
-            _check(what, "w_down", w_down, (width, hidden), torch.bfloat16, dev))
+    return (_ops_native or _native()).rmsnorm_backward(dy, h, gamma, rstd, dh)
 
 
 def gated_ffn(x, w_gate_up, w_down, residual=None):
-    """residual + (silu(x Wg^T) * (x Wu^T)) Wd^T with w_gate_up = Wg over Wu; bf16."""
-    dev = _current_device()
-    d, xp, gp, wp = _ffn("gated_ffn", x, w_gate_up, w_down, torch.bfloat16, dev)
-    rp = _check("gated_ffn", "residual", residual, x.shape, torch.bfloat16, dev)
-    ref = C.byref(d)
-    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(ref)
-    scratch, y = x.new_empty(nbytes // 2), torch.empty_like(x)
-    call("srt_gated_ffn_fwd", ref, xp, gp, wp, rp, y.data_ptr(), scratch.data_ptr(), nbytes, _raw_stream(dev))
-    return y
+    """residual + (silu(x Wg^T) * (x Wu^T)) Wd^T for x [tokens, width], w_gate_up = Wg over Wu [2 hidden, width] and w_down = Wd
+    [width, hidden], in bfloat16; width and hidden are multiples of 8."""
+    return (_ops_native or _native()).gated_ffn(x, w_gate_up, w_down, residual)
 
 
 def gated_ffn_e4m3(x, x_scale, w_gate_up, w_scale, w_down, residual=None):
-    """gated_ffn on 8-bit rows: x * x_scale of its row (rmsnorm_e4m3) and w_gate_up * w_scale of its row (quantize_rows_e4m3)."""
-    what, dev = "gated_ffn_e4m3", _current_device()
-    d, xp, gp, wp = _ffn(what, x, w_gate_up, w_down, torch.float8_e4m3fn, dev)
-    xs = _check(what, "x_scale", x_scale, (d.tokens,), torch.float32, dev)
-    ws = _check(what, "w_scale", w_scale, (2 * d.hidden,), torch.float32, dev)
-    rp = _check(what, "residual", residual, x.shape, torch.bfloat16, dev)
-    ref = C.byref(d)
-    nbytes = _lib.lib().srt_gated_ffn_fwd_scratch_bytes(ref)
-    scratch, y = w_down.new_empty(nbytes // 2), w_down.new_empty(x.shape)
-    call("srt_gated_ffn_fwd_e4m3", ref, xp, xs, gp, ws, wp, rp, y.data_ptr(), scratch.data_ptr(), nbytes, _raw_stream(dev))
-    return y
+    """gated_ffn on 8-bit rows: x * x_scale of its row (rmsnorm_e4m3) and w_gate_up * w_scale of its row (quantize_rows_e4m3);
+    w_down, residual and the result in bfloat16. width is a multiple of 16."""
+    return (_ops_native or _native()).gated_ffn_e4m3(x, x_scale, w_gate_up, w_scale, w_down, residual)
 
 
 def gated_ffn_backward(dy, x, w_gate_up, w_down, grad_dtype=torch.bfloat16):
     """Gradients of gated_ffn at x, which is all that forward has to keep: (dx, dw_gate_up, dw_down), the weights' in
     `grad_dtype` (bfloat16, or float32 for an optimizer that accumulates there). The residual's gradient is dy itself."""
-    what, dev = "gated_ffn_backward", _current_device()
-    d, xp, gp, wp = _ffn(what, x, w_gate_up, w_down, torch.bfloat16, dev)
-    dyp = _check(what, "dy", dy, x.shape, torch.bfloat16, dev)
     if grad_dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"{what}: gradients in bfloat16 or float32, not {grad_dtype}")
-    g = SRT_F32 if grad_dtype is torch.float32 else SRT_BF16
-    dx, dw_gate_up, dw_down = torch.empty_like(x), torch.empty_like(w_gate_up, dtype=grad_dtype), torch.empty_like(w_down, dtype=grad_dtype)
-    ref = C.byref(d)
-    nbytes = _lib.lib().srt_gated_ffn_bwd_scratch_bytes(ref, g)
-    scratch = x.new_empty(nbytes // 2)
-    call("srt_gated_ffn_bwd", ref, dyp, xp, gp, wp, g, dx.data_ptr(), dw_gate_up.data_ptr(), dw_down.data_ptr(), scratch.data_ptr(), nbytes,
-         _raw_stream(dev))
-    return dx, dw_gate_up, dw_down
+        raise TypeError(f"gated_ffn_backward: gradients in bfloat16 or float32, not {grad_dtype}")
+    return (_ops_native or _native()).gated_ffn_backward(dy, x, w_gate_up, w_down, grad_dtype is torch.float32)
 
 
 def grad_accumulate(acc, g):
