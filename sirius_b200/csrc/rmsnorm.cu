@@ -262,23 +262,26 @@ rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const
     partial[(size_t)blockIdx.x * s.C + c] = t;
   }
 }
-// dgamma[c] = sum of the blocks' partial rows: 32 columns x 32 lanes a block, lane l adds rows l, l + 32, ... and the lanes
+// dgamma[c] = sum of the blocks' partial rows: 16 columns x 16 lanes a block, lane l adds rows l, l + 16, ... and the lanes
 // are added in order.
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(256)
 rmsnorm_dgamma_kernel(const float* __restrict__ partial, int blocks, int C, float* __restrict__ dgamma) {
-  __shared__ float sh[32][33];
+  __shared__ float sh[16][17];
   pdl_enter();
-  const int cl = threadIdx.x & 31, l = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
+  const int cl = threadIdx.x & 15, l = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
   float t = 0.f;
   if (c < C) {
-#pragma unroll 8
-    for (int b = l; b < blocks; b += 32) t += partial[(size_t)b * C + c];
+    float v[RN_MAX_BLOCKS / 16];
+#pragma unroll
+    for (int k = 0; k < RN_MAX_BLOCKS / 16; ++k) v[k] = l + 16 * k < blocks ? partial[(size_t)(l + 16 * k) * C + c] : 0.f;
+#pragma unroll
+    for (int k = 0; k < RN_MAX_BLOCKS / 16; ++k) t += v[k];
   }
   sh[l][cl] = t;
   __syncthreads();
   if (l == 0 && c < C) {
 #pragma unroll
-    for (int k = 1; k < 32; ++k) t += sh[k][cl];
+    for (int k = 1; k < 16; ++k) t += sh[k][cl];
     dgamma[c] = t;
   }
 }
@@ -350,7 +353,7 @@ int bwd_launch(int64_t rows, int C, const void* dy, const void* h, const float* 
     SRT_CHECK_CUDA(launch_pdl(kernel, dim3(l.blocks), dim3(l.threads), smem, st, l.s, (const T*)dy, (const T*)h, gamma, rstd, (const T*)dh,
                               (T*)dx, partial));
     SRT_LAUNCH_CHECK();
-    SRT_CHECK_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3(ceil_div(C, 32)), dim3(1024), 0, st, (const float*)partial, (int)l.blocks, C, dgamma));
+    SRT_CHECK_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3(ceil_div(C, 16)), dim3(256), 0, st, (const float*)partial, (int)l.blocks, C, dgamma));
     SRT_LAUNCH_CHECK();
     return SRT_OK;
   };
