@@ -10,6 +10,9 @@
 // blocks take in turn. Bound by memory: one read for the norm; clipping in place reads and writes once more. The second
 // launch walks the chunks backwards, so that what the first one read last comes out of L2, and every block adds the partial
 // sums for itself instead of waiting for a launch between.
+#include <algorithm>
+#include <vector>
+
 #include "common.cuh"
 #include "grad_clip.cuh"
 
@@ -199,6 +202,28 @@ int run(int tensors, void* const* grads, const int64_t* counts, float max_norm, 
   return SRT_OK;
 }
 
+// A tensor that shares memory with another one, or -1. Lists that ascend in memory, as an executor lays its gradients out, need
+// one look; others are put in order.
+int first_overlap(int esz, int tensors, void* const* grads, const int64_t* counts) {
+  auto begin = [&](int i) { return (uintptr_t)grads[i]; };
+  auto end = [&](int i) { return (uintptr_t)grads[i] + (uintptr_t)counts[i] * esz; };
+  uintptr_t reached = 0;
+  bool ascending = true;
+  for (int i = 0; i < tensors && ascending; ++i) {
+    if (counts[i] == 0) continue;
+    ascending = begin(i) >= reached;
+    reached = end(i);
+  }
+  if (ascending) return -1;
+  std::vector<int> order;
+  for (int i = 0; i < tensors; ++i)
+    if (counts[i] > 0) order.push_back(i);
+  std::sort(order.begin(), order.end(), [&](int a, int b) { return begin(a) < begin(b); });
+  for (size_t k = 1; k < order.size(); ++k)
+    if (begin(order[k]) < end(order[k - 1])) return order[k];
+  return -1;
+}
+
 }  // namespace
 
 size_t grad_norm_scratch_bytes(int tensors) {
@@ -217,6 +242,10 @@ int grad_norm(int dtype, int tensors, void* const* grads, const int64_t* counts,
     chunks += counts[i] / GC_CHUNK + 1;
   }
   SRT_REQUIRE(chunks < (1ll << 30), "grad_norm: more than 2^45 elements");
+  if (scale) {
+    const int twice = first_overlap(dtype == SRT_F32 ? 4 : 2, tensors, grads, counts);
+    SRT_REQUIRE(twice < 0, "clip_grad_norm: tensor %d shares memory with another and would be scaled twice", twice);
+  }
   SRT_REQUIRE(scratch && ((uintptr_t)scratch & 7) == 0 && scratch_bytes >= grad_norm_scratch_bytes(tensors),
               "grad_norm: scratch missing, unaligned or too small (%zu < %zu)", scratch_bytes, grad_norm_scratch_bytes(tensors));
   if (dtype == SRT_F32)

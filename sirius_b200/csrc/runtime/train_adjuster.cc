@@ -86,13 +86,13 @@ int srt_adjuster_model_mem_param(const char* model_name, double* base_mb, double
 
 // The same line for this library's bf16 executors on a B200, measured with `python -m sirius_b200.mem_model`
 // (device memory taken by the executor at two batch sizes; resnet152 at 224x224, gpt2 at 1024 tokens, qwen = the
-// 0.5B shape at 2048 tokens). The swin_b_ddp entry adds the gradient buckets' bf16 wire buffer to swin_b. A change of what
+// 0.5B shape at 2048 tokens, qwen_recompute the same with srt_qwen2_recompute_mlp). The swin_b_ddp entry adds the gradient buckets' bf16 wire buffer to swin_b. A change of what
 // the executors keep moves these lines: tests/test_mem_model_gpu.py holds the table to the device.
 int srt_adjuster_model_mem_param_measured(const char* model_name, double* base_mb, double* slope_mb) {
   SRT_REQUIRE(model_name && base_mb && slope_mb, "model_mem_param_measured: null argument");
   static const struct { const char* name; double base, slope; } kTable[] = {
       {"resnet152", 1347, 105}, {"swin_b", 1727, 122}, {"swin_b_ddp", 1897, 122}, {"gpt2", 2759, 402},
-      {"qwen", 10581, 2549}};
+      {"qwen", 10581, 2549}, {"qwen_recompute", 10537, 1201}};
   for (const auto& e : kTable)
     if (std::string(model_name) == e.name) { *base_mb = e.base; *slope_mb = e.slope; return SRT_OK; }
   set_error("train adjuster: no measured memory line for model '%s'", model_name);

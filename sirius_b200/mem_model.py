@@ -38,7 +38,7 @@ def _fit(make, b_lo, b_hi):
             "batches": [b_lo, b_hi], "device_mb": [round(lo_dev, 1), round(hi_dev, 1)]}
 
 
-def measure(models=("resnet152", "swin_b", "gpt2", "qwen")) -> dict:
+def measure(models=("resnet152", "swin_b", "gpt2", "qwen", "qwen_recompute")) -> dict:
     import torch
     from .gpt2_step import Gpt2Step
     from .qwen2_step import Qwen2Step
@@ -51,6 +51,7 @@ def measure(models=("resnet152", "swin_b", "gpt2", "qwen")) -> dict:
         "swin_b": (lambda b: SwinStep(max_batch=b), 8, 32),
         "gpt2": (lambda b: Gpt2Step(max_batch=b, seq=1024), 2, 8),
         "qwen": (lambda b: Qwen2Step(max_batch=b, seq=2048), 1, 4),
+        "qwen_recompute": (lambda b: Qwen2Step(max_batch=b, seq=2048, recompute_mlp=True), 1, 4),
     }
     out = {}
     for m in models:

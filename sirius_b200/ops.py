@@ -271,8 +271,8 @@ def grad_norm(grads, max_norm):
 
 
 def clip_grad_norm(grads, max_norm):
-    """grad_norm that also multiplies the gradients by the coefficient, in place (torch.nn.utils.clip_grad_norm_). No two of
-    them overlap."""
+    """grad_norm that also multiplies the gradients by the coefficient, in place (torch.nn.utils.clip_grad_norm_).
+    Tensors that share memory are refused."""
     return (_ops_native or _native()).grad_norm(grads, max_norm, True)
 
 

@@ -84,6 +84,28 @@ def test_nothing_to_clip():
             assert f(grads, 1.0).tolist() == [0.0, 1.0]
 
 
+def test_tensors_that_share_memory():
+    from sirius_b200._lib import SrtError
+    flat = torch.randn(1000, device="cuda")
+    before = flat.clone()
+    for grads in ([flat[:600], flat[500:]], [flat[700:], flat[:300], flat[200:500]], [flat, flat], [flat[10:20], flat[5:11]]):
+        with pytest.raises(SrtError, match="shares memory"):
+            ops.clip_grad_norm(grads, 1e-3)
+        assert torch.equal(flat, before)
+        assert torch.isfinite(ops.grad_norm(grads, 1.0)).all()
+    for grads in ([flat[500:], flat[:500]], [flat[10:20], flat[:0], flat[:10], flat[20:]], [flat[20:], flat[10:10], flat[:20]]):
+        flat.copy_(before)
+        ops.clip_grad_norm(grads, 1e-3)
+        assert abs(float(flat.double().norm()) - 1e-3) < 1e-6
+
+
+def test_an_empty_step():
+    e = torch.empty(0, device="cuda")
+    clip = ops.grad_norm([], 1.0)
+    ops.adamw(e, e, e, e, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, clip=clip)
+    ops.sgd_momentum(e, e, e, 1e-3, 0.9, 0.0, True, clip=clip)
+
+
 @pytest.mark.parametrize("n", [1, 5, 1000, 100003, 1 << 20])
 @pytest.mark.parametrize("share", [0.25, 4.0])
 def test_adamw_takes_the_coefficient(n, share):

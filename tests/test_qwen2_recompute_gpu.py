@@ -94,3 +94,56 @@ def test_shrunk_and_regained_batches():
     assert two[0] == small[0] and all(np.array_equal(two[1][n], small[1][n]) for n in two[1])
     step.close()
     fresh.close()
+
+
+def test_memory_line_of_the_adjuster():
+    """As for the other executors: what the trainer registers as model "qwen_recompute" has a line of its own, half as steep."""
+    import ctypes as C
+    import gc
+
+    import torch
+
+    from sirius_b200 import mem_model
+    from sirius_b200._lib import call
+    gc.collect()
+    torch.cuda.empty_cache()
+    got = mem_model.measure(("qwen_recompute",))["qwen_recompute"]
+    base, slope = C.c_double(), C.c_double()
+    call("srt_adjuster_model_mem_param_measured", b"qwen_recompute", C.byref(base), C.byref(slope))
+    for batch, mb in zip(got["batches"], got["device_mb"]):
+        assert abs(base.value + slope.value * batch - mb) <= 0.1 * mb, (got, base.value, slope.value)
+    assert abs(slope.value - got["slope_mb"]) <= 0.1 * got["slope_mb"], (got, slope.value)
+
+
+@pytest.mark.parametrize("recompute", [False, True])
+def test_clipped_steps_on_a_partition_of_the_device(recompute):
+    """The step and its clipping while training has a part of the SMs: kernels are cut for that width, the work is the same."""
+    import ctypes as C
+
+    from sirius_b200._lib import call
+    full = (1 << 64) - 1
+    B, S = 2, 128
+    state = O.state_arrays(O.build_model(**TINY, seed=0))
+    ids = O.make_tokens(B, S, TINY["vocab"], 1)[0]
+
+    def run(mask):
+        step = Qwen2Step(**TINY, max_batch=B, seq=S, recompute_mlp=recompute)
+        try:
+            step.load_state_dict(state)
+            if mask is not None:
+                step.follow_sm_mask(True)
+                call("srt_set_sm_mask", (C.c_uint64 * 3)(*mask))
+            loss, grads = grads_of(step, ids)
+            step.clip_grad_norm(0.5)
+            return loss, grads, step.grad_norm(), step.current_sms()
+        finally:
+            call("srt_set_sm_mask", (C.c_uint64 * 3)(full, full, full))
+            step.close()
+    whole, part = run(None), run((full, 0, 0))
+    assert part[3] <= 64 < whole[3]
+    assert abs(part[0] - whole[0]) <= 1e-3 * abs(whole[0]) and abs(part[2] - whole[2]) <= 2e-2 * whole[2]
+    top = max(float(np.linalg.norm(g)) for g in whole[1].values())
+    for n, g in whole[1].items():
+        # sums cut elsewhere round elsewhere: the same bound as against the oracle
+        assert np.linalg.norm(part[1][n] - g) <= 5e-2 * np.linalg.norm(g) + 1e-3 * top, n
+    assert ops.tc_status() == 0
