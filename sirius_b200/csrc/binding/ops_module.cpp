@@ -2,8 +2,8 @@
 // workspaces and the C entry point in one native call. As Python over ctypes the same took 13 us for a norm and 0.4 us per
 // gradient of a list, most of what a short call costs; here 5 us and 0.02.
 //
-// Module sirius_b200._ops_native. bind(path, error) opens libsirius_b200.so (the one that ctypes has open already) and keeps
-// the exception of failing calls. Wrong operands raise ValueError or TypeError and name the operand.
+// Module sirius_b200._ops_native. bind(path, error, no_memory) opens libsirius_b200.so (the one that ctypes has open already)
+// and keeps the exceptions. Wrong operands raise ValueError or TypeError and name the operand.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -44,7 +44,7 @@ struct Library {
   ENTRY(srt_sgd_momentum_clipped);
 } lib;
 #undef ENTRY
-PyObject* call_error = nullptr;
+PyObject *call_error = nullptr, *memory_error = nullptr;
 
 // ---- errors ----------------------------------------------------------------------------------------------
 struct Raise {  // thrown with the Python error to set
@@ -67,12 +67,28 @@ PyObject* guarded(F&& f) {
   } catch (const Raise& e) {
     PyErr_SetString(e.type, e.text.c_str());
   } catch (const PySet&) {
+  } catch (const c10::OutOfMemoryError& e) {
+    PyErr_SetString(memory_error, e.what_without_backtrace());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   } catch (...) {
     PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
   }
   return nullptr;
+}
+
+// The interpreter's lock is given up around allocations and entry points: both may wait, for memory or for a full launch queue,
+// and other threads go on meanwhile.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+template <typename F>
+auto unlocked(F&& f) {
+  Unlocked u;
+  return f();
 }
 
 // ---- arguments -------------------------------------------------------------------------------------------
@@ -169,9 +185,13 @@ PyObject* rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const float eps = (float)number(a[2]);
     const void* residual = c.optional(a[3], "residual", x.scalar_type(), x.sizes());
     const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
-    Tensor y = like(x), h = residual ? like(x) : Tensor(), rstd = at::empty(lead, gamma.options());
-    check(lib.srt_rmsnorm_fwd(kind, x.data_ptr(), residual, gamma.data_ptr<float>(), residual ? h.data_ptr() : nullptr, y.data_ptr(),
-                              rstd.data_ptr<float>(), rows_of(lead), C, eps, c.stream()),
+    Tensor y, h, rstd;
+    check(unlocked([&] {
+            y = like(x), rstd = at::empty(lead, gamma.options());
+            if (residual) h = like(x);
+            return lib.srt_rmsnorm_fwd(kind, x.data_ptr(), residual, gamma.data_ptr<float>(), residual ? h.data_ptr() : nullptr, y.data_ptr(),
+                                       rstd.data_ptr<float>(), rows_of(lead), C, eps, c.stream());
+          }),
           "srt_rmsnorm_fwd");
     return tuple(wrap(y), residual ? wrap(h) : same(a[0]), wrap(rstd));
   });
@@ -187,10 +207,13 @@ PyObject* rmsnorm_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const float eps = (float)number(a[2]);
     const void* residual = c.optional(a[3], "residual", x.scalar_type(), x.sizes());
     const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
-    Tensor q = like(x, at::kFloat8_e4m3fn), h = residual ? like(x) : Tensor();
-    Tensor scale = at::empty(lead, gamma.options()), rstd = at::empty(lead, gamma.options());
-    check(lib.srt_rmsnorm_fwd_e4m3(kind, x.data_ptr(), residual, gamma.data_ptr<float>(), residual ? h.data_ptr() : nullptr, q.data_ptr(),
-                                   scale.data_ptr<float>(), rstd.data_ptr<float>(), rows_of(lead), C, eps, c.stream()),
+    Tensor q, h, scale, rstd;
+    check(unlocked([&] {
+            q = like(x, at::kFloat8_e4m3fn), scale = at::empty(lead, gamma.options()), rstd = at::empty(lead, gamma.options());
+            if (residual) h = like(x);
+            return lib.srt_rmsnorm_fwd_e4m3(kind, x.data_ptr(), residual, gamma.data_ptr<float>(), residual ? h.data_ptr() : nullptr, q.data_ptr(),
+                                            scale.data_ptr<float>(), rstd.data_ptr<float>(), rows_of(lead), C, eps, c.stream());
+          }),
           "srt_rmsnorm_fwd_e4m3");
     return tuple(wrap(q), wrap(scale), residual ? wrap(h) : same(a[0]), wrap(rstd));
   });
@@ -203,8 +226,11 @@ PyObject* quantize_rows_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& x = c.tensor(a[0], "x");
     const int kind = row_kind(c, x, "x"), C = columns(c, x, "x");
     const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
-    Tensor q = like(x, at::kFloat8_e4m3fn), scale = make(lead, at::kFloat, c.device);
-    check(lib.srt_quantize_rows_e4m3(kind, x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), rows_of(lead), C, c.stream()),
+    Tensor q, scale;
+    check(unlocked([&] {
+            q = like(x, at::kFloat8_e4m3fn), scale = make(lead, at::kFloat, c.device);
+            return lib.srt_quantize_rows_e4m3(kind, x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), rows_of(lead), C, c.stream());
+          }),
           "srt_quantize_rows_e4m3");
     return tuple(wrap(q), wrap(scale));
   });
@@ -222,9 +248,13 @@ PyObject* rmsnorm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& rstd = c.tensor(a[3], "rstd", at::kFloat, lead);
     const void* dh = c.optional(a[4], "dh", h.scalar_type(), h.sizes());
     const size_t need = lib.srt_rmsnorm_bwd_scratch_bytes(C);
-    Tensor dx = like(h), dgamma = like(gamma), scratch = bytes(need, c.device);
-    check(lib.srt_rmsnorm_bwd(kind, dy.data_ptr(), h.data_ptr(), gamma.data_ptr<float>(), rstd.data_ptr<float>(), dh, dx.data_ptr(),
-                              dgamma.data_ptr<float>(), rows_of(lead), C, scratch.data_ptr(), need, c.stream()),
+    Tensor dx, dgamma;
+    check(unlocked([&] {
+            dx = like(h), dgamma = like(gamma);
+            const Tensor scratch = bytes(need, c.device);
+            return lib.srt_rmsnorm_bwd(kind, dy.data_ptr(), h.data_ptr(), gamma.data_ptr<float>(), rstd.data_ptr<float>(), dh, dx.data_ptr(),
+                                       dgamma.data_ptr<float>(), rows_of(lead), C, scratch.data_ptr(), need, c.stream());
+          }),
           "srt_rmsnorm_bwd");
     return tuple(wrap(dx), wrap(dgamma));
   });
@@ -253,9 +283,13 @@ PyObject* gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Ffn f = ffn(c, a[0], a[1], a[2], at::kBFloat16);
     const void* residual = c.optional(a[3], "residual", at::kBFloat16, f.x.sizes());
     const size_t need = lib.srt_gated_ffn_fwd_scratch_bytes(&f.d);
-    Tensor y = like(f.x), scratch = bytes(need, c.device);
-    check(lib.srt_gated_ffn_fwd(&f.d, f.x.data_ptr(), f.w_gate_up.data_ptr(), f.w_down.data_ptr(), residual, y.data_ptr(), scratch.data_ptr(),
-                                need, c.stream()),
+    Tensor y;
+    check(unlocked([&] {
+            y = like(f.x);
+            const Tensor scratch = bytes(need, c.device);
+            return lib.srt_gated_ffn_fwd(&f.d, f.x.data_ptr(), f.w_gate_up.data_ptr(), f.w_down.data_ptr(), residual, y.data_ptr(),
+                                         scratch.data_ptr(), need, c.stream());
+          }),
           "srt_gated_ffn_fwd");
     return wrap(y);
   });
@@ -270,9 +304,13 @@ PyObject* gated_ffn_e4m3(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& w_scale = c.tensor(a[3], "w_scale", at::kFloat, {2 * (int64_t)f.d.hidden});
     const void* residual = c.optional(a[5], "residual", at::kBFloat16, f.x.sizes());
     const size_t need = lib.srt_gated_ffn_fwd_scratch_bytes(&f.d);
-    Tensor y = like(f.x, at::kBFloat16), scratch = bytes(need, c.device);
-    check(lib.srt_gated_ffn_fwd_e4m3(&f.d, f.x.data_ptr(), x_scale.data_ptr<float>(), f.w_gate_up.data_ptr(), w_scale.data_ptr<float>(),
-                                     f.w_down.data_ptr(), residual, y.data_ptr(), scratch.data_ptr(), need, c.stream()),
+    Tensor y;
+    check(unlocked([&] {
+            y = like(f.x, at::kBFloat16);
+            const Tensor scratch = bytes(need, c.device);
+            return lib.srt_gated_ffn_fwd_e4m3(&f.d, f.x.data_ptr(), x_scale.data_ptr<float>(), f.w_gate_up.data_ptr(), w_scale.data_ptr<float>(),
+                                              f.w_down.data_ptr(), residual, y.data_ptr(), scratch.data_ptr(), need, c.stream());
+          }),
           "srt_gated_ffn_fwd_e4m3");
     return wrap(y);
   });
@@ -288,9 +326,13 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int kind = wide ? SRT_F32 : SRT_BF16;
     const at::ScalarType type = wide ? at::kFloat : at::kBFloat16;
     const size_t need = lib.srt_gated_ffn_bwd_scratch_bytes(&f.d, kind);
-    Tensor dx = like(f.x), dw_gate_up = like(f.w_gate_up, type), dw_down = like(f.w_down, type), scratch = bytes(need, c.device);
-    check(lib.srt_gated_ffn_bwd(&f.d, dy.data_ptr(), f.x.data_ptr(), f.w_gate_up.data_ptr(), f.w_down.data_ptr(), kind, dx.data_ptr(),
-                                dw_gate_up.data_ptr(), dw_down.data_ptr(), scratch.data_ptr(), need, c.stream()),
+    Tensor dx, dw_gate_up, dw_down;
+    check(unlocked([&] {
+            dx = like(f.x), dw_gate_up = like(f.w_gate_up, type), dw_down = like(f.w_down, type);
+            const Tensor scratch = bytes(need, c.device);
+            return lib.srt_gated_ffn_bwd(&f.d, dy.data_ptr(), f.x.data_ptr(), f.w_gate_up.data_ptr(), f.w_down.data_ptr(), kind, dx.data_ptr(),
+                                         dw_gate_up.data_ptr(), dw_down.data_ptr(), scratch.data_ptr(), need, c.stream());
+          }),
           "srt_gated_ffn_bwd");
     return tuple(wrap(dx), wrap(dw_gate_up), wrap(dw_down));
   });
@@ -328,11 +370,14 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (c.device < 0) c.device = c10::cuda::current_device();
     const size_t need = lib.srt_grad_norm_scratch_bytes((int)tensors);
-    Tensor work = bytes(256 + need, c.device);  // the results first, the partial sums behind them
-    char* base = (char*)work.data_ptr();
+    Tensor work;  // the results first, the partial sums behind them
     const int kind = type == at::kFloat ? SRT_F32 : SRT_BF16;
-    const int status = in_place ? lib.srt_clip_grad_norm(kind, (int)tensors, ptr.data(), numel.data(), max_norm, (float*)base, base + 256, need, c.stream())
-                                : lib.srt_grad_norm(kind, (int)tensors, ptr.data(), numel.data(), max_norm, (float*)base, base + 256, need, c.stream());
+    const int status = unlocked([&] {
+      work = bytes(256 + need, c.device);
+      char* base = (char*)work.data_ptr();
+      return in_place ? lib.srt_clip_grad_norm(kind, (int)tensors, ptr.data(), numel.data(), max_norm, (float*)base, base + 256, need, c.stream())
+                      : lib.srt_grad_norm(kind, (int)tensors, ptr.data(), numel.data(), max_norm, (float*)base, base + 256, need, c.stream());
+    });
     check(status, in_place ? "srt_clip_grad_norm" : "srt_grad_norm");
     return wrap(work.slice(0, 0, 8).view(at::kFloat));
   });
@@ -357,8 +402,11 @@ PyObject* adamw_clipped(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const State s = state(c, a[0], a[1], a[2], a[3], a[10], a[11]);
     const long step = PyLong_AsLong(a[9]);
     if (step == -1 && PyErr_Occurred()) throw PySet{};
-    check(lib.srt_adamw_clipped(s.p, s.g, s.m, s.v, s.p_bf16, s.n, number(a[4]), number(a[5]), number(a[6]), number(a[7]), number(a[8]),
-                                step > INT32_MAX ? INT32_MAX : (int)step, s.clip, c.stream()),
+    const double lr = number(a[4]), b1 = number(a[5]), b2 = number(a[6]), eps = number(a[7]), wd = number(a[8]);
+    check(unlocked([&] {
+            return lib.srt_adamw_clipped(s.p, s.g, s.m, s.v, s.p_bf16, s.n, lr, b1, b2, eps, wd, step > INT32_MAX ? INT32_MAX : (int)step, s.clip,
+                                         c.stream());
+          }),
           "srt_adamw_clipped");
     Py_RETURN_NONE;
   });
@@ -369,18 +417,19 @@ PyObject* sgd_momentum_clipped(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Call c("sgd_momentum");
     count(n, 9, c.what);
     const State s = state(c, a[0], a[1], a[2], nullptr, a[7], a[8]);
-    check(lib.srt_sgd_momentum_clipped(s.p, s.g, s.m, s.p_bf16, s.n, (float)number(a[3]), (float)number(a[4]), (float)number(a[5]),
-                                       PyObject_IsTrue(a[6]) == 1, s.clip, c.stream()),
+    const float lr = (float)number(a[3]), mu = (float)number(a[4]), wd = (float)number(a[5]);
+    const int first_step = PyObject_IsTrue(a[6]) == 1;
+    check(unlocked([&] { return lib.srt_sgd_momentum_clipped(s.p, s.g, s.m, s.p_bf16, s.n, lr, mu, wd, first_step, s.clip, c.stream()); }),
           "srt_sgd_momentum_clipped");
     Py_RETURN_NONE;
   });
 }
 
-// (path of the library, exception of failing calls)
+// (path of the library, exceptions of failing calls and of device memory that ran out)
 PyObject* bind(PyObject*, PyObject* args) {
   const char* path;
-  PyObject* error;
-  if (!PyArg_ParseTuple(args, "sO", &path, &error)) return nullptr;
+  PyObject *error, *no_memory;
+  if (!PyArg_ParseTuple(args, "sOO", &path, &error, &no_memory)) return nullptr;
   void* handle = dlopen(path, RTLD_NOW | RTLD_LOCAL);
   if (!handle) return PyErr_Format(PyExc_OSError, "%s", dlerror());
   bool all = true;
@@ -406,6 +455,8 @@ PyObject* bind(PyObject*, PyObject* args) {
   FIND(srt_sgd_momentum_clipped)
 #undef FIND
   if (!all) return PyErr_Format(PyExc_OSError, "%s lacks%s", path, missing.c_str());
+  Py_INCREF(no_memory);
+  Py_XSETREF(memory_error, no_memory);
   Py_INCREF(error);
   Py_XSETREF(call_error, error);
   Py_RETURN_NONE;

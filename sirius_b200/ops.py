@@ -42,7 +42,7 @@ def _native():
         except ImportError as e:
             raise _lib.SrtError("sirius_b200/_ops_native.so is missing or does not fit this torch: build it with "
                                 f"`python -m sirius_b200._build` ({e})") from e
-        module.bind(str(_lib.LIB_PATH), _lib.SrtError)
+        module.bind(str(_lib.LIB_PATH), _lib.SrtError, torch.OutOfMemoryError)
         _ops_native = module
     return _ops_native
 

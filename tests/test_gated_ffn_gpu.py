@@ -219,3 +219,36 @@ def test_captured_and_replayed_on_two_streams():
     for o, w, s in zip(outs, want, sets):
         assert all(torch.equal(a, b) for a, b in zip(o, w))
         assert torch.equal(ops.gated_ffn(s["x"], s["wgu"], s["wd"], s["res"]), w[0])
+
+
+def test_two_threads_at_once():
+    """Two host threads, each on its own stream, take the same calls as one."""
+    import threading
+    sets = [make(5, 136, 264), make(600, 136, 1032)]
+
+    def calls(s):
+        y, h, rstd = ops.rmsnorm(s["x"], s["gamma"], 1e-6, s["res"])
+        return (y, h, rstd, ops.gated_ffn(y, s["wgu"], s["wd"], h), *ops.gated_ffn_backward(s["dy"], y, s["wgu"], s["wd"]),
+                ops.grad_norm([s["wgu"], s["wd"]], 1.0))
+    for s in sets:
+        s["gamma"] = torch.linspace(0.5, 1.5, s["x"].shape[1], device="cuda")
+    want = [calls(s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(s, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(100):
+                    got = calls(s)
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, w)):
+                wrong.append("results")
+        except Exception as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=run, args=a) for a in zip(sets, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and ops.tc_status() == 0
