@@ -385,11 +385,15 @@ int srt_adamw(float* p, const float* g, float* m, float* v, void* p_bf16, int64_
 int srt_adamw_clipped(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, double lr, double beta1, double beta2,
                       double eps, double wd, int step, const float* clip, void* stream) {
   SRT_REQUIRE(n >= 0 && (n == 0 || (p && g && m && v && clip)), "adamw_clipped: bad argument");
+  SRT_REQUIRE((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v | (uintptr_t)clip) & 3) == 0 && ((uintptr_t)p_bf16 & 1) == 0,
+              "adamw_clipped: operands must be aligned to their elements");
   return adamw_clipped(p, g, m, v, p_bf16, n, lr, beta1, beta2, eps, wd, step, clip, ST(stream));
 }
 int srt_sgd_momentum_clipped(float* p, const float* g, float* m, void* p_bf16, int64_t n, float lr, float mu, float wd, int first_step,
                              const float* clip, void* stream) {
   SRT_REQUIRE(n >= 0 && (n == 0 || (p && g && m && clip)), "sgd_momentum_clipped: bad argument");
+  SRT_REQUIRE((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)clip) & 3) == 0 && ((uintptr_t)p_bf16 & 1) == 0,
+              "sgd_momentum_clipped: operands must be aligned to their elements");
   return sgd_momentum(p, g, m, p_bf16, n, lr, mu, wd, first_step, ST(stream), clip + 1);
 }
 int srt_grad_accumulate(float* acc, float* g, int64_t n, void* stream) {

@@ -303,15 +303,13 @@ __global__ void sgd_momentum_kernel(float* __restrict__ p, const float* __restri
       reinterpret_cast<uint2*>(pb)[i] = o;
     }
   }
-  // scalar tail
-  if (blockIdx.x == 0) {
-    for (int64_t j = n4 * 4 + threadIdx.x; j < n; j += blockDim.x) {
-      const float d = fmaf(wd, p[j], __fmul_rn(g[j], k));
-      const float mj = first_step ? d : fmaf(mu, m[j], d);
-      m[j] = mj;
-      p[j] = fmaf(-lr, mj, p[j]);
-      if (pb) pb[j] = __float2bfloat16_rn(p[j]);
-    }
+  // what is left over, or everything when a buffer is not aligned for the vectors (n4 = 0)
+  for (i = n4 * 4 + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
+    const float d = fmaf(wd, p[i], __fmul_rn(g[i], k));
+    const float mi = first_step ? d : fmaf(mu, m[i], d);
+    m[i] = mi;
+    p[i] = fmaf(-lr, mi, p[i]);
+    if (pb) pb[i] = __float2bfloat16_rn(p[i]);
   }
 }
 
@@ -579,8 +577,9 @@ int colsum(int dtype, const void* dy, int64_t rows, int K, float* out, cudaStrea
 int sgd_momentum(float* p, const float* g, float* m, void* pb, int64_t n, float lr, float mu,
                  float wd, int first_step, cudaStream_t st, const float* coefficient) {
   if (n == 0) return SRT_OK;
-  const int64_t n4 = n / 4;
-  launch_pdl(sgd_momentum_kernel, dim3(stream_grid(n4 > 0 ? n4 : 1, 8)), dim3(NT), 0, st, 
+  const bool vectors = ((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m) & 15) | ((uintptr_t)pb & 7)) == 0;
+  const int64_t n4 = vectors ? n / 4 : 0;
+  launch_pdl(sgd_momentum_kernel, dim3(stream_grid(n4 > 0 ? n4 : n, 8)), dim3(NT), 0, st, 
       p, g, m, (__nv_bfloat16*)pb, n4, n, lr, mu, wd, first_step, coefficient);
   SRT_LAUNCH_CHECK();
   return SRT_OK;

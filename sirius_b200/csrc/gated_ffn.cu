@@ -685,6 +685,7 @@ int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_sca
   const size_t act_bytes = up256((size_t)d->tokens * d->hidden * 2);
   SRT_REQUIRE(scratch && scratch_bytes >= act_bytes, "gated_ffn_fwd: scratch too small (%zu < %zu)", scratch_bytes, act_bytes);
   if ((rc = FFN_ALIGNED(x, w_gu, w_down, residual, y, scratch))) return rc;
+  SRT_REQUIRE((((uintptr_t)x_scale | (uintptr_t)w_scale) & 3) == 0, "gated_ffn: scales must be aligned to 4 bytes");
   void* act = scratch;
   switch (d->tokens) {
     case 1: return token_ffn<1>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);

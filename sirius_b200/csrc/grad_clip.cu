@@ -11,6 +11,7 @@
 // launch walks the chunks backwards, so that what the first one read last comes out of L2, and every block adds the partial
 // sums for itself instead of waiting for a launch between.
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "common.cuh"
@@ -203,7 +204,7 @@ int run(int tensors, void* const* grads, const int64_t* counts, float max_norm, 
 }
 
 // A tensor that shares memory with another one, or -1. Lists that ascend in memory, as an executor lays its gradients out, need
-// one look; others are put in order.
+// one look; others are put in order. -2: no memory for that.
 int first_overlap(int esz, int tensors, void* const* grads, const int64_t* counts) {
   auto begin = [&](int i) { return (uintptr_t)grads[i]; };
   auto end = [&](int i) { return (uintptr_t)grads[i] + (uintptr_t)counts[i] * esz; };
@@ -216,6 +217,11 @@ int first_overlap(int esz, int tensors, void* const* grads, const int64_t* count
   }
   if (ascending) return -1;
   std::vector<int> order;
+  try {
+    order.reserve((size_t)tensors);
+  } catch (const std::bad_alloc&) {
+    return -2;
+  }
   for (int i = 0; i < tensors; ++i)
     if (counts[i] > 0) order.push_back(i);
   std::sort(order.begin(), order.end(), [&](int a, int b) { return begin(a) < begin(b); });
@@ -234,16 +240,21 @@ int grad_norm(int dtype, int tensors, void* const* grads, const int64_t* counts,
               size_t scratch_bytes, cudaStream_t st) {
   SRT_REQUIRE(dtype == SRT_F32 || dtype == SRT_BF16, "grad_norm: bad dtype %d", dtype);
   SRT_REQUIRE(tensors >= 0 && (tensors == 0 || (grads && counts)) && clip, "grad_norm: null argument");
+  SRT_REQUIRE(((uintptr_t)clip & 3) == 0, "grad_norm: clip is not aligned to its elements");
   SRT_REQUIRE(max_norm > 0.f, "grad_norm: max_norm (%g) must be positive", (double)max_norm);
   int64_t chunks = 0;
   for (int i = 0; i < tensors; ++i) {
     SRT_REQUIRE(counts[i] >= 0 && (counts[i] == 0 || grads[i]), "grad_norm: tensor %d has no memory or a negative count", i);
     SRT_REQUIRE(((uintptr_t)grads[i] & (dtype == SRT_F32 ? 3 : 1)) == 0, "grad_norm: tensor %d is not aligned to its elements", i);
     chunks += counts[i] / GC_CHUNK + 1;
+    SRT_REQUIRE(chunks < (1ll << 30), "grad_norm: more than 2^45 elements");
   }
-  SRT_REQUIRE(chunks < (1ll << 30), "grad_norm: more than 2^45 elements");
   if (scale) {
     const int twice = first_overlap(dtype == SRT_F32 ? 4 : 2, tensors, grads, counts);
+    if (twice == -2) {
+      set_error("clip_grad_norm: no host memory for a list of %d tensors", tensors);
+      return SRT_ERR_NOMEM;
+    }
     SRT_REQUIRE(twice < 0, "clip_grad_norm: tensor %d shares memory with another and would be scaled twice", twice);
   }
   SRT_REQUIRE(scratch && ((uintptr_t)scratch & 7) == 0 && scratch_bytes >= grad_norm_scratch_bytes(tensors),

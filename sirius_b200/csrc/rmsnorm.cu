@@ -316,12 +316,13 @@ RowLaunch row_launch(int64_t rows, int C, int vec, int warps, int per_sm) {
 int check_rows(const char* what, int dtype, int64_t rows, int C) {
   SRT_REQUIRE(dtype == SRT_F32 || dtype == SRT_BF16, "%s: bad dtype %d", what, dtype);
   SRT_REQUIRE(rows >= 0 && C > 0 && C % 8 == 0, "%s: C (%d) must be a positive multiple of 8, rows not negative", what, C);
-  SRT_REQUIRE(C * (dtype == SRT_F32 ? 4 : 2) <= RN_MAX_ROW_BYTES, "%s: rows of %d elements are longer than %d bytes", what, C, RN_MAX_ROW_BYTES);
+  SRT_REQUIRE((int64_t)C * (dtype == SRT_F32 ? 4 : 2) <= RN_MAX_ROW_BYTES, "%s: rows of %d elements are longer than %d bytes", what, C, RN_MAX_ROW_BYTES);
   SRT_REQUIRE(rows < (1ll << 31), "%s: more than 2^31 rows", what);
   return SRT_OK;
 }
-int check_ptrs(const char* what, std::initializer_list<const void*> ps) {
+int check_ptrs(const char* what, std::initializer_list<const void*> ps, std::initializer_list<const void*> floats) {
   for (const void* p : ps) SRT_REQUIRE(((uintptr_t)p & 15) == 0, "%s: operands must be 16-byte aligned", what);
+  for (const void* p : floats) SRT_REQUIRE(((uintptr_t)p & 3) == 0, "%s: parameters and statistics must be aligned to 4 bytes", what);
   return SRT_OK;
 }
 
@@ -377,7 +378,7 @@ int srt_rmsnorm_fwd(int dtype, const void* x, const void* residual, const float*
   int rc = check_rows("rmsnorm_fwd", dtype, rows, C);
   if (rc || rows == 0) return rc;
   SRT_REQUIRE(x && gamma && y, "rmsnorm_fwd: null operand");
-  if ((rc = check_ptrs("rmsnorm_fwd", {x, residual, h, y}))) return rc;
+  if ((rc = check_ptrs("rmsnorm_fwd", {x, residual, h, y}, {gamma, rstd}))) return rc;
   return dtype == SRT_F32 ? fwd_launch<float, true, false>(rows, C, x, residual, gamma, h, y, nullptr, nullptr, rstd, eps, (cudaStream_t)stream)
                           : fwd_launch<bf16, true, false>(rows, C, x, residual, gamma, h, y, nullptr, nullptr, rstd, eps, (cudaStream_t)stream);
 }
@@ -387,7 +388,7 @@ int srt_rmsnorm_fwd_e4m3(int dtype, const void* x, const void* residual, const f
   int rc = check_rows("rmsnorm_fwd_e4m3", dtype, rows, C);
   if (rc || rows == 0) return rc;
   SRT_REQUIRE(x && gamma && q && scale, "rmsnorm_fwd_e4m3: null operand");
-  if ((rc = check_ptrs("rmsnorm_fwd_e4m3", {x, residual, h, q}))) return rc;
+  if ((rc = check_ptrs("rmsnorm_fwd_e4m3", {x, residual, h, q}, {gamma, scale, rstd}))) return rc;
   return dtype == SRT_F32 ? fwd_launch<float, true, true>(rows, C, x, residual, gamma, h, nullptr, q, scale, rstd, eps, (cudaStream_t)stream)
                           : fwd_launch<bf16, true, true>(rows, C, x, residual, gamma, h, nullptr, q, scale, rstd, eps, (cudaStream_t)stream);
 }
@@ -396,7 +397,7 @@ int srt_quantize_rows_e4m3(int dtype, const void* x, void* q, float* scale, int6
   int rc = check_rows("quantize_rows_e4m3", dtype, rows, C);
   if (rc || rows == 0) return rc;
   SRT_REQUIRE(x && q && scale, "quantize_rows_e4m3: null operand");
-  if ((rc = check_ptrs("quantize_rows_e4m3", {x, q}))) return rc;
+  if ((rc = check_ptrs("quantize_rows_e4m3", {x, q}, {scale}))) return rc;
   return dtype == SRT_F32 ? fwd_launch<float, false, true>(rows, C, x, nullptr, nullptr, nullptr, nullptr, q, scale, nullptr, 0.f, (cudaStream_t)stream)
                           : fwd_launch<bf16, false, true>(rows, C, x, nullptr, nullptr, nullptr, nullptr, q, scale, nullptr, 0.f, (cudaStream_t)stream);
 }
@@ -415,7 +416,7 @@ int srt_rmsnorm_bwd(int dtype, const void* dy, const void* h, const float* gamma
   SRT_REQUIRE(dy && h && gamma && rstd && dx, "rmsnorm_bwd: null operand");
   SRT_REQUIRE(scratch && scratch_bytes >= srt_rmsnorm_bwd_scratch_bytes(C), "rmsnorm_bwd: scratch too small (%zu < %zu)", scratch_bytes,
               srt_rmsnorm_bwd_scratch_bytes(C));
-  if ((rc = check_ptrs("rmsnorm_bwd", {dy, h, dh, dx}))) return rc;
+  if ((rc = check_ptrs("rmsnorm_bwd", {dy, h, dh, dx}, {gamma, rstd, dgamma, scratch}))) return rc;
   return dtype == SRT_F32 ? bwd_launch<float>(rows, C, dy, h, gamma, rstd, dh, dx, dgamma, (float*)scratch, (cudaStream_t)stream)
                           : bwd_launch<bf16>(rows, C, dy, h, gamma, rstd, dh, dx, dgamma, (float*)scratch, (cudaStream_t)stream);
 }

@@ -174,3 +174,23 @@ def test_captured_lists_of_many_tensors():
         flat.copy_(start)
         graph.replay()
         assert torch.equal(clip, want) and torch.equal(flat, clipped)
+
+
+@pytest.mark.parametrize("n", [5, 4099, 300001])
+def test_steps_on_views_off_a_vector_boundary(n):
+    """Views that begin at any element take the same step as copies of them that begin on a boundary."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for shift in (1, 2, 3):
+        flat = [torch.randn(n + 4, device="cuda", generator=g).square() * 0.01 for _ in range(4)]
+        views, copies = [t[shift:shift + n] for t in flat], [t[shift:shift + n].clone() for t in flat]
+        outside = [t.clone() for t in flat]
+        low = [torch.empty(n + 4, device="cuda", dtype=BF)[shift:shift + n], torch.empty(n, device="cuda", dtype=BF)]
+        clip = ops.grad_norm([views[1]], 0.5)
+        for k, t in enumerate((views, copies)):
+            ops.sgd_momentum(*t[:3], 0.1, 0.9, 1e-4, False, p_bf16=low[k], clip=clip)
+        assert torch.equal(*low)
+        for k, t in enumerate((views, copies)):
+            ops.adamw(*t, 1e-3, 0.9, 0.99, 1e-8, 0.01, 3, p_bf16=low[k], clip=clip)
+        assert torch.equal(*low) and all(torch.equal(a, b) for a, b in zip(views, copies))
+        for t, o in zip(flat, outside):
+            assert torch.equal(t[:shift], o[:shift]) and torch.equal(t[shift + n:], o[shift + n:])

@@ -149,3 +149,23 @@ def test_workspaces_are_sized_on_the_host():
     d = C.byref(GatedFfnDesc(100, 64, 128))
     assert lib.srt_gated_ffn_fwd_scratch_bytes(d) >= 100 * 128 * 2
     assert lib.srt_gated_ffn_bwd_scratch_bytes(d, SRT_F32) >= 100 * 128 * 6
+
+
+@pytest.mark.parametrize("c", [1 << 28, 1 << 29, 1 << 30, (1 << 31) - 8])
+def test_rows_whose_bytes_pass_32_bits(c):
+    for dtype in (SRT_F32, SRT_BF16):
+        rc, text = status("srt_rmsnorm_fwd", dtype, P, None, P, None, P, None, 1, c, 1e-6, None)
+        assert rc == 1 and "longer" in text
+
+
+def test_pointers_between_two_elements():
+    for name, args in (("srt_rmsnorm_fwd", (SRT_F32, P, None, P + 2, None, P, None, 4, 8, 1e-6, None)),
+                       ("srt_rmsnorm_fwd_e4m3", (SRT_F32, P, None, P, None, P, P + 1, None, 4, 8, 1e-6, None)),
+                       ("srt_rmsnorm_bwd", (SRT_F32, P, P, P, P, None, P, P + 2, 4, 8, P, 1 << 40, None)),
+                       ("srt_gated_ffn_fwd_e4m3", (C.byref(GatedFfnDesc(4, 32, 16)), P, P + 2, P, P, P, None, P, P, 1 << 50, None)),
+                       ("srt_grad_norm", (SRT_F32, 0, None, None, 1.0, P + 2, P, 1 << 40, None)),
+                       ("srt_adamw_clipped", (P + 2, P, P, P, None, 4, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, P, None)),
+                       ("srt_adamw_clipped", (P, P, P, P, P + 1, 4, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1, P, None)),
+                       ("srt_sgd_momentum_clipped", (P, P, P, None, 4, 0.1, 0.9, 0.0, 1, P + 1, None))):
+        rc, text = status(name, *args)
+        assert rc == 1 and "aligned" in text, (name, rc, text)
