@@ -199,7 +199,6 @@ int srt_sgd_momentum(float* p, const float* g, float* m, void* p_bf16, int64_t n
 /* AdamW with fp32 state; step counts from 1. */
 int srt_adamw(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, float lr,
               float beta1, float beta2, float eps, float wd, int step, void* stream);
-/* acc += g ; g = 0  (GradAccumulator.accumulate). */
 /* Clipping by the norm of all gradients together (torch.nn.utils.clip_grad_norm_): clip[0] = sqrt(sum of squares, in 64 bits)
  * over `tensors` device arrays of one dtype, clip[1] = min(1, max_norm / (clip[0] + 1e-6)). srt_clip_grad_norm also multiplies
  * the arrays by clip[1] in place; the clipped optimizer steps take it from `clip` instead, which saves that pass. grads and
@@ -213,6 +212,7 @@ int srt_adamw_clipped(float* p, const float* g, float* m, float* v, void* p_bf16
                       double eps, double wd, int step, const float* clip, void* stream);
 int srt_sgd_momentum_clipped(float* p, const float* g, float* m, void* p_bf16, int64_t n, float lr, float mu, float wd, int first_step,
                              const float* clip, void* stream);
+/* acc += g ; g = 0  (GradAccumulator.accumulate). */
 int srt_grad_accumulate(float* acc, float* g, int64_t n, void* stream);
 
 /* ---- layout / dtype helpers ---------------------------------------------------------------- */
@@ -405,8 +405,8 @@ int srt_step_accumulate(srt_step* s);
 int srt_step_optimizer(srt_step* s);
 /* Clipping of the next optimizer step (of every executor; srt_step_*, srt_gpt2_*, srt_swin_*, srt_qwen2_*): the norm of the
  * gradients that step would consume (accumulated ones where there are any) and the coefficient min(1, max_norm / (norm +
- * 1e-6)), which the step multiplies them by on their way in; the gradient buffer stays as it is. Call it after the last
- * forward_backward, accumulate and gradient exchange: a later one takes it back. _grad_norm waits for the norm and reads it. */
+ * 1e-6)), which the step multiplies them by on their way in; the gradient buffer stays as it is. Call it after the
+ * gradient exchange; a later forward_backward or accumulate takes it back. _grad_norm waits for the norm and reads it. */
 int srt_step_clip_grad_norm(srt_step* s, float max_norm);
 int srt_step_grad_norm(srt_step* s, float* host_norm);
 /* Scaled loss of the last micro-batch; synchronises the stream (loss.item()). */
