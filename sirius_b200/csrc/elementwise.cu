@@ -313,12 +313,13 @@ __global__ void sgd_momentum_kernel(float* __restrict__ p, const float* __restri
   }
 }
 
-// One AdamW element (decoupled decay, bias corrections folded into step_size and bc2_sqrt).
+// One AdamW element (decoupled decay, bias corrections folded into step_size and bc2_sqrt). The fused products of the moments are
+// written out: left to the compiler, the choice of the one to fuse moves with the code around it, and their last bit with that.
 __device__ inline float adamw_element(float pi, float gi, float& m, float& v, float lr, float b1, float b2, float c1, float c2,
                                       float eps, float wd, float step_size, float bc2_sqrt) {
   pi = pi * (1.f - lr * wd);
-  m = b1 * m + c1 * gi;
-  v = b2 * v + c2 * gi * gi;
+  m = fmaf(c1, gi, b1 * m);
+  v = fmaf(c2 * gi, gi, b2 * v);
   const float denom = sqrtf(v) / bc2_sqrt + eps;
   return pi - step_size * (m / denom);
 }

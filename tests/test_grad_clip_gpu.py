@@ -194,3 +194,21 @@ def test_steps_on_views_off_a_vector_boundary(n):
         assert torch.equal(*low) and all(torch.equal(a, b) for a, b in zip(views, copies))
         for t, o in zip(flat, outside):
             assert torch.equal(t[:shift], o[:shift]) and torch.equal(t[shift + n:], o[shift + n:])
+
+
+@pytest.mark.parametrize("n", [1000, 100003])
+def test_adamw_keeps_its_roundings(n):
+    """m = fma(1 - b1, g, b1 m), v = fma((1 - b2) g, g, b2 v): with g, m and v of eight bits the sums below are exact in 64 bits,
+    so one rounding is left in each. With or without a coefficient of one, the bits are the same."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    r = lambda s: (torch.randn(n, device="cuda", generator=g) * s).to(BF).float()
+    p, gr, m, v = r(0.05), r(1e-2), r(1e-3), r(1e-2).square().to(BF).float()
+    b1, b2 = 0.875, 0.9375
+    c1, c2 = 1 - b1, 1 - b2
+    want_m = (c1 * gr.double() + (b1 * m).double()).float()
+    want_v = ((c2 * gr).double() * gr.double() + (b2 * v).double()).float()
+    a, b = ([t.clone() for t in (p, gr, m, v)] for _ in range(2))
+    ops.adamw(*a, 2.0 ** -10, b1, b2, 2.0 ** -27, 0.0, 1)
+    ops.adamw(*b, 2.0 ** -10, b1, b2, 2.0 ** -27, 0.0, 1, clip=ops.grad_norm([b[1]], 1e6))
+    assert torch.equal(a[2], want_m) and torch.equal(a[3], want_v)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
