@@ -537,7 +537,8 @@ int srt_rmsnorm_bwd(int dtype, const void* dy, const void* h, const float* gamma
  * multiples of 8, operands and scratch 16-byte aligned, matrices below 2^31 elements. residual may be null. The gate and up
  * projections never reach memory. Backward forms them again from x: dx, dw_gate_up and dw_down (each may be null; the weights'
  * gradients are of type grad_dtype and overwritten). scratch: what the _scratch_bytes calls say. Outputs and
- * scratch overlap nothing else. The e4m3 form takes x and w_gate_up in 8 bits with
+ * scratch overlap nothing else. A call repeats bit for bit; the order of its sums depends on the sizes and on the SMs at hand,
+ * so a token beside others may differ from the same token alone in the last bits. The e4m3 form takes x and w_gate_up in 8 bits with
  * one fp32 scale a row (srt_rmsnorm_fwd_e4m3, srt_quantize_rows_e4m3); width is then a multiple of 16. */
 typedef struct srt_gated_ffn_desc { int tokens, width, hidden; } srt_gated_ffn_desc;
 size_t srt_gated_ffn_fwd_scratch_bytes(const srt_gated_ffn_desc* d);

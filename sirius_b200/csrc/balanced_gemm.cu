@@ -4,11 +4,14 @@
 // all, and what is left over, fewer tiles than units, is cut along the reduction into as many equal ranges as there are units.
 // A unit that has only a part of a tile's reduction leaves fp32 sums in a slot of its own, and a second, small launch adds the
 // slots of every such tile in the order of the reduction. So 152 tiles on 74 pairs take 2.05 rounds and not three, a few rows
-// against a long reduction occupy the device, no CTA waits for another, and the sums have a fixed order.
+// against a long reduction occupy the device, no CTA waits for another, and the sums have a fixed order. With few tiles a
+// cluster shares each, and the parts meet in its shared memory instead (split_gemm_kernel).
 //
 // Warps as in the gated kernels: 0 TMA, 1 MMA, 2-17 four epilogue groups that take the 32-column slabs of a tile in turn. The
 // accumulator is double-buffered in tensor memory, so the epilogue of a tile runs beside the products of the next.
 #include <cuda.h>
+
+#include <atomic>
 
 #include "balanced_gemm.cuh"
 #include "ptx.cuh"
@@ -378,16 +381,231 @@ balanced_gemm_join_kernel(const GemmParams p, const __grid_constant__ JoinList l
   }
 }
 
+// ---- a tile a cluster -------------------------------------------------------------------------------------
+// With few tiles a cluster of c CTAs shares one: each takes a part of the reduction in 128 elements a stage (two blocks of 64),
+// leaves its fp32 sums in its own shared memory, and adds a part of the tile from all of them in the order of the reduction.
+// One launch, and no slots in memory. What a few tokens need: their products wait for memory and for launches, not for the
+// tensor cores.
+constexpr int SPLIT_MAX = 8;  // CTAs of a portable cluster
+struct SplitParams {
+  int M, N, n, c, m_units, steps;  // steps of 128 along the reduction, at least c
+  int cols;                        // tensor-memory columns
+  int stages;
+  uint32_t a_bytes, b_bytes;       // of a block; as in GemmParams, few rows are staged alone
+  int f32_out, b_early;
+  const bf16* addend;
+  void* D;
+  int* status;
+};
+template <bool B_MN>
+__global__ void __launch_bounds__(G_THREADS, 1)
+split_gemm_kernel(const SplitParams p, const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int NS = p.stages;
+  const uint32_t stage_bytes = 2u * (p.a_bytes + p.b_bytes);
+  uint64_t* bars = (uint64_t*)(base + (uint32_t)NS * stage_bytes + BM * 128 - p.a_bytes);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * G_MAX_STAGES, acc_full = empty + 8 * G_MAX_STAGES;
+  uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * G_MAX_STAGES + 1);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const uint32_t s0 = smem_u32(base), rank = cluster_ctarank();
+  const int tile = (int)blockIdx.x / p.c, m0 = tile % p.m_units * BM, n0 = tile / p.m_units * p.n;
+  const int k0 = p.steps * (int)rank / p.c, k1 = p.steps * ((int)rank + 1) / p.c;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+  }
+  if (warp == 0 && lane == 0) { tma_prefetch_desc(&ta); tma_prefetch_desc(&tb); }
+  if (warp == 1) { tmem_alloc(smem_u32(tmem_ptr), p.cols); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  const bool ahead = p.b_early && warp == 0;
+  if (!ahead) pdl_enter();
+
+  if (warp == 0) {
+    const uint32_t wrap = (uint32_t)NS * stage_bytes;
+    uint32_t at = 0, bar = 0, ph = 1;
+    auto step = [&]() {
+      at += stage_bytes;
+      bar += 8;
+      if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
+    };
+    auto load_a = [&](int k) {
+      tma_load_2d(s0 + at, &ta, full + bar, k * 128, m0);
+      tma_load_2d(s0 + at + p.a_bytes, &ta, full + bar, k * 128 + 64, m0);
+    };
+    auto load_b = [&](int k) {
+      mbar_arrive_expect_tx(full + bar, stage_bytes);
+      uint32_t b = s0 + at + 2u * p.a_bytes;
+      if (B_MN) {
+        for (int h = 0; h < 2; ++h)
+          for (int x = 0; x < p.n; x += 64, b += 8192u) tma_load_2d(b, &tb, full + bar, n0 + x, k * 128 + h * 64);
+      } else {
+        tma_load_2d(b, &tb, full + bar, k * 128, n0);
+        tma_load_2d(b + p.b_bytes, &tb, full + bar, k * 128 + 64, n0);
+      }
+    };
+    int early = k0;
+    if (ahead) {
+      for (; early < k1 && early < k0 + NS; ++early) {
+        if (elect_one()) load_b(early);
+        step();
+      }
+      pdl_enter();
+      at = bar = 0;
+      ph = 1;
+    }
+    int k = k0;
+    for (; k < early; ++k) {
+      if (elect_one()) load_a(k);
+      step();
+    }
+    bool ok = true;
+    for (; k < k1; ++k) {
+      ok = mbar_wait_warp<false>(empty + bar, ph, p.status, W_GEMM_LOAD);
+      if (!ok) break;
+      if (elect_one()) {
+        load_b(k);
+        load_a(k);
+      }
+      step();
+    }
+    // a wait that gave up: the copies in flight land before the CTA's memory is given back
+    if (!ok)
+      for (int i = k - k0 > NS ? k - k0 - NS : 0; i < k - k0; ++i) mbar_wait_warp<false>(full + 8 * (i % NS), (uint32_t)(i / NS) & 1u, p.status, W_GEMM_DRAIN);
+  } else if (warp == 1) {
+    const uint32_t idesc = make_idesc_bf16(BM, p.n, 0, B_MN);
+    constexpr uint32_t b_step = B_MN ? 2048u : 32u;
+    const uint64_t desc_a = make_smem_desc_sw128(s0, 0, 1024), desc_b = make_smem_desc_sw128(s0 + 2u * p.a_bytes, B_MN ? 8192 : 0, 1024);
+    const uint32_t wrap = (uint32_t)NS * stage_bytes;
+    uint32_t at = 0, bar = 0, ph = 0, add = 0;
+    bool ok = true;
+    for (int k = k0; k < k1; ++k) {
+      ok = mbar_wait_warp<false>(full + bar, ph, p.status, W_GEMM_FULL);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint64_t ad = desc_at(desc_a, at), bd = desc_at(desc_b, at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          umma_bf16(tmem, desc_at(ad, (j & 3) * 32 + (j >> 2) * p.a_bytes), desc_at(bd, (j & 3) * b_step + (j >> 2) * p.b_bytes), idesc, j ? 1u : add);
+        umma_commit(empty + bar);
+      }
+      add = 1;
+      at += stage_bytes;
+      bar += 8;
+      if (at == wrap) { at = 0; bar = 0; ph ^= 1u; }
+    }
+    if (ok && elect_one()) umma_commit(acc_full);
+  } else {
+    // the sums into shared memory, over the stages that the products have read; rows 16 bytes apart in their banks
+    const int grp = (warp - 2) >> 2, q = warp & 3, row = q * 32 + lane;
+    __all_sync(0xffffffffu, mbar_wait(acc_full, 0, p.status, W_GEMM_EPI));
+    tc_fence_after_sync();
+    if (q * 32 < (int)(p.a_bytes >> 7))  // rows that were staged
+      for (int c = grp * 32; c < p.n; c += 32 * EPI_GROUPS) {
+        uint32_t f[32];
+        tmem_ld_32x32b_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, f);
+        tmem_ld_wait();
+        if (row < (int)(p.a_bytes >> 7)) {
+          const uint32_t dst = s0 + (uint32_t)(row * (p.n + 4) + c) * 4u;
+#pragma unroll
+          for (int v = 0; v < 8; ++v) st_shared_v4(dst + 16u * v, f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
+        }
+      }
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  cluster_sync_all();  // every CTA's sums are there (and every warp of this CTA is)
+
+  const int per_row = p.n / 4, rows = min(BM, p.M - m0);
+  for (int i = (int)rank * G_THREADS + tid; i < rows * per_row; i += p.c * G_THREADS) {
+    const int r = i / per_row, col = (i - r * per_row) * 4;
+    if (n0 + col >= p.N) continue;  // N is a multiple of eight
+    const size_t at = (size_t)(m0 + r) * p.N + n0 + col;
+    const uint32_t src = s0 + (uint32_t)(r * (p.n + 4) + col) * 4u;
+    float4 v[SPLIT_MAX];
+#pragma unroll
+    for (int k = 0; k < SPLIT_MAX; ++k)
+      if (k < p.c) v[k] = ld_cluster_f4(map_to_cta(src, (uint32_t)k));
+    float4 t = v[0];
+#pragma unroll
+    for (int k = 1; k < SPLIT_MAX; ++k)
+      if (k < p.c) { t.x += v[k].x; t.y += v[k].y; t.z += v[k].z; t.w += v[k].w; }
+    if (p.addend) {
+      const uint2 a = *reinterpret_cast<const uint2*>(p.addend + at);
+      t.x += __uint_as_float(a.x << 16);
+      t.y += __uint_as_float(a.x & 0xffff0000u);
+      t.z += __uint_as_float(a.y << 16);
+      t.w += __uint_as_float(a.y & 0xffff0000u);
+    }
+    if (p.f32_out) {
+      *reinterpret_cast<float4*>((float*)p.D + at) = t;
+    } else {
+      __nv_bfloat162 lo = __floats2bfloat162_rn(t.x, t.y), hi = __floats2bfloat162_rn(t.z, t.w);
+      *reinterpret_cast<uint2*>((bf16*)p.D + at) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+    }
+  }
+  cluster_sync_all();  // the sums outlive their readers
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, p.cols);
+  }
+}
+
 // How a problem is cut: the cut with the least time by this model, in microseconds, of which the constants were measured (with
 // both forms, every tile width and all three operand orders, 74 pairs busy). A k-block takes 0.155 at least, 1.53 ns a column
 // of the tile for the products, and its bytes at 115 KB out of L2 (rows that do not begin on 128 bytes take half as much again),
 // or, where B is read only once, 40 KB out of memory. An epilogue takes 0.35 and 10 ns a column, in fp32 17, and runs beside the
 // next tile's products. Sharing the rest of the tiles takes a launch and the slots' way to memory and back, some 3.5 MB.
 // Against the best cut found by trying all: within 5 % for 13 of 16 problems of 8 to 8192 rows.
+//
+// A tile a cluster of c takes 3.6 to begin and end, 0.16 c and 0.195 ns an element of the tile to bring the parts together, and
+// a step of 128 along the reduction 0.28 at least, 2.8 ns a column, its bytes at 160 KB and 16.5 TB/s on all of them; where B is
+// read only once, at 65 KB and 6.3 TB/s out of memory. (On this scale the other cuts begin with 1.5.) Measured with weights out
+// of memory, sharing units and a second launch against clusters: 24 x 4096 x 11008 22.6 and 18.4 us, 5 x 896 x 4864 10.3 and 6.4,
+// 128 x 896 x 4864 11.5 and 8.0, 333 x 896 x 9728 (B across) 17.4 and 14.3, 512 x 896 x 4864 13.9 and 11.2, 600 x 2048 x 5632
+// 18.7 and 18.4, 1024 x 896 x 4864 15.0 and 15.2. Whole device only: in a partition clusters may not find their SMs.
 struct GemmPlan {
   bool pair;
   int n, m_units, n_tiles, tiles, units, rounds, rest, sharers;
+  int split;  // CTAs of a cluster that share a tile each, or 0
 };
+// Clusters of c CTAs of split_gemm_kernel that the device holds at one time, as the driver counts them (0 if it does not); asked
+// for once a device.
+template <bool B_MN>
+int clusters_that_fit(int c) {
+  static std::atomic<int> known[16][SPLIT_MAX + 1];  // one more than the count
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return 0;
+  const int k = known[dev][c].load(std::memory_order_relaxed);
+  if (k) return k - 1;
+  constexpr int smem = 232448;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)c);
+  cfg.blockDim = dim3(G_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)c;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(split_gemm_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, split_gemm_kernel<B_MN>, &cfg) != cudaSuccess || n < 0) {
+    cudaGetLastError();
+    n = 0;
+  }
+  known[dev][c].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
 size_t plan_bytes(const GemmPlan& g) { return g.rest ? (size_t)2 * g.sharers * (g.pair ? 2 * BM : BM) * g.n * sizeof(float) : 0; }
 // Plans that need more than `room` bytes of slots are left out; one without any is always there.
 GemmPlan plan_gemm(const GemmProblem& q, size_t room) {
@@ -397,6 +615,37 @@ GemmPlan plan_gemm(const GemmProblem& q, size_t room) {
   const bool a_odd = (q.a_mn ? q.M : q.K) % 64 != 0, b_odd = (q.b_mn ? q.N : q.K) % 64 != 0;
   GemmPlan best = {};
   double best_cost = 1e30;
+  for (int c = 1; c <= (q.a_mn || sm_limit() != 0 ? 0 : SPLIT_MAX); ++c) {
+    const int fit = q.b_mn ? clusters_that_fit<true>(c) : clusters_that_fit<false>(c), steps = ceil_div(ceil_div(q.K, 128), c);
+    if (steps * (c - 1) >= ceil_div(q.K, 128)) continue;  // a CTA without a step
+    for (int n = 32; n <= 256; n += 32) {
+      if (n > 32 && n - 32 >= q.N) continue;  // wider than the matrix
+      const int m_units = ceil_div(q.M, BM), n_tiles = ceil_div(q.N, n);
+      if ((long long)m_units * n_tiles > fit) continue;
+      const double all = (double)m_units * n_tiles * c;
+      const double a_bytes = 256.0 * a_rows * (a_odd ? 1.5 : 1.0);
+      const double b_bytes = 2.0 * (q.b_mn ? 8192.0 * ceil_div(n, 64) : 128.0 * n) * (b_odd ? 1.5 : 1.0);
+      double t = 0.28;
+      auto at_least = [&](double v) { t = v > t ? v : t; };
+      at_least(0.0028 * n);
+      at_least((a_bytes + b_bytes) / 160e3);
+      at_least((a_bytes + b_bytes) * all / 16.5e6);
+      if (m_units == 1) {
+        at_least(b_bytes / 65e3);
+        at_least(b_bytes * all / 6.3e6);
+      }
+      const double cost = 3.6 - 1.5 + 0.16 * c + 0.195e-3 * a_rows * n + steps * t;
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {};
+        best.n = n;
+        best.m_units = m_units;
+        best.n_tiles = n_tiles;
+        best.tiles = best.units = m_units * n_tiles;
+        best.split = c;
+      }
+    }
+  }
   for (int pair = 0; pair <= (sms >= 2 && q.M > BM ? 1 : 0); ++pair) {
     for (int n = 32; n <= 256; n += 32) {
       if (n > 32 && n - 32 >= q.N) continue;  // wider than the matrix
@@ -495,6 +744,34 @@ int launch_gemm(GemmParams& p, const GemmPlan& g, const CUtensorMap (&tm)[4], cu
   return SRT_OK;
 }
 
+template <bool B_MN>
+int launch_split(SplitParams& p, const CUtensorMap (&tm)[4], cudaStream_t st) {
+  const size_t fixed = 1024 + BM * 128 - p.a_bytes + (2 * G_MAX_STAGES + 1) * 8 + 16, stage = 2 * (size_t)(p.a_bytes + p.b_bytes);
+  p.stages = (int)((232448 - fixed) / stage);
+  if (p.stages > G_MAX_STAGES) p.stages = G_MAX_STAGES;
+  const size_t sums = (size_t)(p.a_bytes >> 7) * (p.n + 4) * 4;
+  SRT_REQUIRE(p.stages >= 2 && sums <= p.stages * stage, "balanced_gemm: a tile of %d columns does not fit a cluster", p.n);
+  static SmemOptIn opt_in;
+  SRT_CHECK_CUDA(opt_in.set(split_gemm_kernel<B_MN>, 232448));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.m_units * ceil_div(p.N, p.n) * p.c));
+  cfg.blockDim = dim3(G_THREADS);
+  cfg.dynamicSmemBytes = fixed + (size_t)p.stages * stage;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = (pdl_big_kernels() && (pdl_classes() & PDL_GEMM) != 0) ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.c;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  SRT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, split_gemm_kernel<B_MN>, p, tm[0], tm[1]));
+  SRT_LAUNCH_CHECK();
+  return SRT_OK;
+}
+
 }  // namespace
 
 size_t balanced_gemm_scratch_bytes(const GemmProblem& q) { return q.M > 0 && q.N > 0 && q.K > 0 ? plan_bytes(plan_gemm(q, SIZE_MAX)) : 0; }
@@ -538,6 +815,25 @@ int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void
       (rc = tmap_rows(&tm[2], D, q.M, q.N, q.N, p.f32_out ? 4 : 2, p.f32_out ? 16 : 32, a_rows)))
     return rc;
   tm[3] = tm[2];
+  if (g.split) {
+    SplitParams s = {};
+    s.M = q.M;
+    s.N = q.N;
+    s.n = g.n;
+    s.c = g.split;
+    s.m_units = g.m_units;
+    s.steps = ceil_div(q.K, 128);
+    s.cols = 32;
+    while (s.cols < g.n) s.cols *= 2;
+    s.a_bytes = p.a_bytes;
+    s.b_bytes = (uint32_t)b_bytes;
+    s.f32_out = p.f32_out;
+    s.b_early = b_early;
+    s.addend = p.addend;
+    s.D = D;
+    s.status = p.status;
+    return q.b_mn ? launch_split<true>(s, tm, st) : launch_split<false>(s, tm, st);
+  }
   if (g.rest && (rc = tmap_rows(&tm[3], scratch, (uint64_t)2 * g.sharers * (g.pair ? 2 * BM : BM), g.n, g.n, 4, 16, a_rows))) return rc;
   if (q.a_mn) return g.pair ? launch_gemm<true, true, true>(p, g, tm, st) : launch_gemm<false, true, true>(p, g, tm, st);
   if (q.b_mn) return g.pair ? launch_gemm<true, false, true>(p, g, tm, st) : launch_gemm<false, false, true>(p, g, tm, st);

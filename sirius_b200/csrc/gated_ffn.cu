@@ -492,10 +492,18 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
 }
 
 // ---- a few tokens ---------------------------------------------------------------------------------------
-// Up to four tokens: the weights are read once and everything else is small, so the products are dot products of weight rows
+// One to four tokens: the weights are read once and everything else is small, so the products are dot products of weight rows
 // on the CUDA cores, without the set-up of tensor memory and tensor maps. A warp has one hidden channel (its gate and its up
 // row), or a quarter of one output row; all its loads are in flight together. fp32 sums in a fixed order.
+//
+// What a token more costs here grows with the weights, and the tensor cores take it for nothing: so the more weights, the fewer
+// tokens. Measured with weights out of memory, dot products and tensor cores, us: 896 x 4864 1 token 8.7 and 11.9, 3 11.9 and
+// 11.9, 4 13.0 and 12.0; 2048 x 8192 1 token 21.6 and 25.0, 2 25.1 and 25.0, 3 28.6 and 25.0; 4096 x 11008 1 token 50.0 and
+// 47.5, in 8 bits 36.0 and 36.0; 1024 x 2816 in 8 bits 1 token 5.6 and 9.6, 4 8.3 and 9.7.
 constexpr int TOK_MAX = 4;
+bool few_tokens(const srt_gated_ffn_desc& d) {
+  return d.tokens <= TOK_MAX && (long long)d.tokens * (d.tokens > 1 ? d.tokens - 1 : 1) * d.width * d.hidden <= 36000000;
+}
 constexpr int TOK_THREADS = 128;
 
 __device__ __forceinline__ float warp_add(float v) {
@@ -687,7 +695,7 @@ int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_sca
   if ((rc = FFN_ALIGNED(x, w_gu, w_down, residual, y, scratch))) return rc;
   SRT_REQUIRE((((uintptr_t)x_scale | (uintptr_t)w_scale) & 3) == 0, "gated_ffn: scales must be aligned to 4 bytes");
   void* act = scratch;
-  switch (d->tokens) {
+  switch (few_tokens(*d) ? d->tokens : 0) {
     case 1: return token_ffn<1>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
     case 2: return token_ffn<2>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);
     case 3: return token_ffn<3>(*d, x, x_scale, w_gu, w_scale, w_down, residual, act, y, st);

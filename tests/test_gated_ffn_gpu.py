@@ -252,3 +252,35 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong and ops.tc_status() == 0
+
+
+# cuts of the plain products: a tile a cluster, of every cluster size there is; token counts at the bounds of the dot products
+FEW = [(1, 4096, 11008), (2, 2048, 8192), (2, 2048, 8200), (3, 896, 4864), (4, 896, 4864), (4, 712, 4104), (5, 896, 4864), (16, 2048, 8192),
+       (24, 4096, 11008), (33, 5120, 6920), (64, 1536, 8960), (100, 1024, 4096), (128, 896, 1288), (200, 896, 4864), (200, 1544, 8936), (512, 896, 4864),
+       (640, 1024, 1096)]
+
+
+@pytest.mark.parametrize("t,c,f", FEW)
+def test_few_tokens_against_long_reductions(t, c, f):
+    s = make(t, c, f)
+    y = ops.gated_ffn(s["x"], s["wgu"], s["wd"], residual=s["res"])
+    got = ops.gated_ffn_backward(s["dy"], s["x"], s["wgu"], s["wd"])
+    assert ops.tc_status() == 0
+    close(y, *reference(s["x"], s["wgu"], s["wd"], s["res"]), "y")
+    want, tol = reference(s["x"], s["wgu"], s["wd"], dy=s["dy"])
+    for a, b, e, what in zip(got, want, tol, ("dx", "dw_gate_up", "dw_down")):
+        close(a, b, (e + H * (b.abs() + e)) * 1.01, what)
+    assert torch.equal(y, ops.gated_ffn(s["x"], s["wgu"], s["wd"], residual=s["res"]))
+    assert torch.equal(got[0], ops.gated_ffn_backward(s["dy"], s["x"], s["wgu"], s["wd"])[0])
+
+
+@pytest.mark.parametrize("t,c,f", [(7, 136, 4104), (24, 896, 4864), (300, 264, 4104)])
+def test_bad_tokens_in_shared_tiles(t, c, f):
+    """A token that is not a number leaves the other rows of its tile alone."""
+    s = make(t, c, f)
+    want, dwant = ops.gated_ffn(s["x"], s["wgu"], s["wd"], s["res"]), ops.gated_ffn_backward(s["dy"], s["x"], s["wgu"], s["wd"])[0]
+    x = s["x"].clone()
+    x[t - 2, 5] = float("nan")
+    y, dx = ops.gated_ffn(x, s["wgu"], s["wd"], s["res"]), ops.gated_ffn_backward(s["dy"], x, s["wgu"], s["wd"])[0]
+    good = torch.arange(t, device="cuda") != t - 2
+    assert torch.equal(y[good], want[good]) and torch.equal(dx[good], dwant[good]) and y[t - 2].isnan().all()
