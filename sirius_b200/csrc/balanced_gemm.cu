@@ -606,13 +606,15 @@ int clusters_that_fit(int c) {
   known[dev][c].store(n + 1, std::memory_order_relaxed);
   return n;
 }
+int a_pitch(const GemmProblem& q) { return q.a_pitch ? q.a_pitch : q.a_mn ? q.M : q.K; }
+int b_pitch(const GemmProblem& q) { return q.b_pitch ? q.b_pitch : q.b_mn ? q.N : q.K; }
 size_t plan_bytes(const GemmPlan& g) { return g.rest ? (size_t)2 * g.sharers * (g.pair ? 2 * BM : BM) * g.n * sizeof(float) : 0; }
 // Plans that need more than `room` bytes of slots are left out; one without any is always there.
 GemmPlan plan_gemm(const GemmProblem& q, size_t room) {
   constexpr int LEAST = 4;  // k-blocks of a share: less is not worth a slot
   const int sms = sm_count() < JOIN_MAX ? sm_count() : JOIN_MAX, kb = ceil_div(q.K, 64);
   const int a_rows = !q.a_mn && q.M < BM ? (q.M + 7) / 8 * 8 : BM;
-  const bool a_odd = (q.a_mn ? q.M : q.K) % 64 != 0, b_odd = (q.b_mn ? q.N : q.K) % 64 != 0;
+  const bool a_odd = a_pitch(q) % 64 != 0, b_odd = b_pitch(q) % 64 != 0;
   GemmPlan best = {};
   double best_cost = 1e30;
   for (int c = 1; c <= (q.a_mn || sm_limit() != 0 ? 0 : SPLIT_MAX); ++c) {
@@ -778,7 +780,8 @@ size_t balanced_gemm_scratch_bytes(const GemmProblem& q) { return q.M > 0 && q.N
 
 int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void* addend, void* D, void* scratch, size_t scratch_bytes,
                   bool b_early, cudaStream_t st) {
-  SRT_REQUIRE(q.M > 0 && q.N > 0 && q.K > 0 && (q.b_mn || !q.a_mn), "balanced_gemm: empty problem or an operand order that has no kernel");
+  SRT_REQUIRE(q.M > 0 && q.N > 0 && q.K > 0 && (q.b_mn || !q.a_mn) && a_pitch(q) >= (q.a_mn ? q.M : q.K) && b_pitch(q) >= (q.b_mn ? q.N : q.K),
+              "balanced_gemm: empty problem or an operand order that has no kernel");
   const GemmPlan g = plan_gemm(q, scratch && ((uintptr_t)scratch & 15) == 0 ? scratch_bytes : 0);
   GemmParams p = {};
   p.M = q.M;
@@ -810,8 +813,8 @@ int balanced_gemm(const GemmProblem& q, const void* A, const void* B, const void
   SRT_REQUIRE(p.status != nullptr, "tcgen05 status word unavailable");
   CUtensorMap tm[4];
   int rc;
-  if ((rc = q.a_mn ? tmap_rows(&tm[0], A, q.K, q.M, q.M, 2, 64, 64) : tmap_rows(&tm[0], A, q.M, q.K, q.K, 2, 64, a_rows)) ||
-      (rc = q.b_mn ? tmap_rows(&tm[1], B, q.K, q.N, q.N, 2, 64, 64) : tmap_rows(&tm[1], B, q.N, q.K, q.K, 2, 64, nc)) ||
+  if ((rc = q.a_mn ? tmap_rows(&tm[0], A, q.K, q.M, a_pitch(q), 2, 64, 64) : tmap_rows(&tm[0], A, q.M, q.K, a_pitch(q), 2, 64, a_rows)) ||
+      (rc = q.b_mn ? tmap_rows(&tm[1], B, q.K, q.N, b_pitch(q), 2, 64, 64) : tmap_rows(&tm[1], B, q.N, q.K, b_pitch(q), 2, 64, nc)) ||
       (rc = tmap_rows(&tm[2], D, q.M, q.N, q.N, p.f32_out ? 4 : 2, p.f32_out ? 16 : 32, a_rows)))
     return rc;
   tm[3] = tm[2];

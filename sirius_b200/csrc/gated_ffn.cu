@@ -50,6 +50,7 @@ struct FfnParams {
                                // follows, and the rows of the accumulators that this fills are not stored
   uint32_t gu_bytes, da_bytes; // what one CTA loads a k-block in either phase
   bf16 *act, *dgu;             // outputs without a tensor map (single CTAs)
+  int act_pitch, dgu_pitch;    // of their rows
   const float *x_scale, *w_scale;
   int* status;
 };
@@ -342,12 +343,12 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
               }
               Vec16<bf16> o;
               o.pack(a);
-              o.store(p.act + (size_t)mrow * p.F + f);
+              o.store(p.act + (size_t)mrow * p.act_pitch + f);
               if constexpr (BWD) {
                 o.pack(dg);
-                o.store(p.dgu + (size_t)mrow * 2 * p.F + f);
+                o.store(p.dgu + (size_t)mrow * p.dgu_pitch + f);
                 o.pack(du);
-                o.store(p.dgu + (size_t)mrow * 2 * p.F + p.F + f);
+                o.store(p.dgu + (size_t)mrow * p.dgu_pitch + p.F + f);
               }
             }
           }
@@ -446,6 +447,11 @@ int launch_ffn(FfnParams& p, const CUtensorMap (&tm)[7], cudaStream_t st) {
   return SRT_OK;
 }
 
+// The rows of act and dgu begin on 128 bytes, whatever `hidden` is: TMA takes half as much time again for rows that do not
+// (1237 x 1544 x 8936, forward: 103.8 us with rows of `hidden`, 96.7 with these).
+int act_pitch(const srt_gated_ffn_desc& d) { return (d.hidden + 63) / 64 * 64; }
+int dgu_pitch(const srt_gated_ffn_desc& d) { return (2 * d.hidden + 63) / 64 * 64; }
+
 // act, and with dy also dgu = (dgate, dup), from x and the weights.
 int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_scale, const void* w_gu, const float* w_scale,
                    const void* dy, const void* w_down, void* act, void* dgu, cudaStream_t st) {
@@ -472,6 +478,8 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   p.stage_bytes = (int)p.a_bytes + b_bytes;
   p.act = (bf16*)act;
   p.dgu = (bf16*)dgu;
+  p.act_pitch = act_pitch(d);
+  p.dgu_pitch = dgu_pitch(d);
   p.x_scale = x_scale;
   p.w_scale = w_scale;
   p.status = tc_status_device_ptr();
@@ -481,10 +489,10 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   if ((rc = tmap_rows_128b(&tm[0], x, T, C, C, esz, a_rows)) || (rc = tmap_rows_128b(&tm[1], w_gu, 2ull * F, C, C, esz, b_rows))) return rc;
   for (int i = 2; i < 7; ++i) tm[i] = tm[0];
   if (bwd && ((rc = tmap_rows_128b(&tm[2], dy, T, C, C, 2, a_rows)) || (rc = tmap_rows_128b(&tm[3], w_down, C, F, F, 2, 64)))) return rc;
-  if (plan.pair && (rc = tmap_rows(&tm[4], act, T, F, F, 2, 32, FM))) return rc;
+  if (plan.pair && (rc = tmap_rows(&tm[4], act, T, F, p.act_pitch, 2, 32, FM))) return rc;
   // the two halves of dgu have maps of their own: a store that reaches beyond `hidden` is clipped in either
-  if (plan.pair && bwd && ((rc = tmap_rows(&tm[5], dgu, T, F, 2ull * F, 2, 32, FM)) ||
-                           (rc = tmap_rows(&tm[6], (bf16*)dgu + F, T, F, 2ull * F, 2, 32, FM))))
+  if (plan.pair && bwd && ((rc = tmap_rows(&tm[5], dgu, T, F, p.dgu_pitch, 2, 32, FM)) ||
+                           (rc = tmap_rows(&tm[6], (bf16*)dgu + F, T, F, p.dgu_pitch, 2, 32, FM))))
     return rc;
   if (bwd) return plan.pair ? launch_ffn<true, true, false>(p, tm, st) : launch_ffn<false, true, false>(p, tm, st);
   if (e4m3) return plan.pair ? launch_ffn<true, false, true>(p, tm, st) : launch_ffn<false, false, true>(p, tm, st);
@@ -673,16 +681,16 @@ int ffn_aligned(std::initializer_list<const void*> ps) {
 }
 
 // The plain products around the gated one.
-GemmProblem down_problem(const srt_gated_ffn_desc& d) { return {d.tokens, d.width, d.hidden, false, false, SRT_BF16}; }        // y
-GemmProblem dx_problem(const srt_gated_ffn_desc& d) { return {d.tokens, d.width, 2 * d.hidden, false, true, SRT_BF16}; }
-GemmProblem dw_problem(const srt_gated_ffn_desc& d, int type) { return {2 * d.hidden, d.width, d.tokens, true, true, type}; }  // dWg over dWu
-GemmProblem dd_problem(const srt_gated_ffn_desc& d, int type) { return {d.width, d.hidden, d.tokens, true, true, type}; }      // dWd
+GemmProblem down_problem(const srt_gated_ffn_desc& d) { return {d.tokens, d.width, d.hidden, false, false, SRT_BF16, act_pitch(d)}; }  // y
+GemmProblem dx_problem(const srt_gated_ffn_desc& d) { return {d.tokens, d.width, 2 * d.hidden, false, true, SRT_BF16, dgu_pitch(d)}; }
+GemmProblem dw_problem(const srt_gated_ffn_desc& d, int type) { return {2 * d.hidden, d.width, d.tokens, true, true, type, dgu_pitch(d)}; }  // dWg over dWu
+GemmProblem dd_problem(const srt_gated_ffn_desc& d, int type) { return {d.width, d.hidden, d.tokens, true, true, type, 0, act_pitch(d)}; }   // dWd
 size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
 }  // namespace
 
 size_t gated_ffn_fwd_scratch_bytes(const srt_gated_ffn_desc& d) {
-  return up256((size_t)d.tokens * d.hidden * 2) + balanced_gemm_scratch_bytes(down_problem(d));
+  return up256((size_t)d.tokens * act_pitch(d) * 2) + balanced_gemm_scratch_bytes(down_problem(d));
 }
 
 int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_scale, const void* w_gu, const float* w_scale,
@@ -690,7 +698,7 @@ int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_sca
   int rc = check_ffn(d, e4m3 ? 16 : 8);
   if (rc || d->tokens == 0) return rc;
   SRT_REQUIRE(x && w_gu && w_down && y && (!e4m3 || (x_scale && w_scale)), "gated_ffn_fwd: null operand");
-  const size_t act_bytes = up256((size_t)d->tokens * d->hidden * 2);
+  const size_t act_bytes = up256((size_t)d->tokens * act_pitch(*d) * 2);
   SRT_REQUIRE(scratch && scratch_bytes >= act_bytes, "gated_ffn_fwd: scratch too small (%zu < %zu)", scratch_bytes, act_bytes);
   if ((rc = FFN_ALIGNED(x, w_gu, w_down, residual, y, scratch))) return rc;
   SRT_REQUIRE((((uintptr_t)x_scale | (uintptr_t)w_scale) & 3) == 0, "gated_ffn: scales must be aligned to 4 bytes");
@@ -707,9 +715,8 @@ int gated_ffn_fwd(const srt_gated_ffn_desc* d, const void* x, const float* x_sca
 
 GatedFfnScratch gated_ffn_scratch(const srt_gated_ffn_desc& d, int grad_dtype) {
   GatedFfnScratch s;
-  const size_t TF = (size_t)d.tokens * d.hidden;
-  s.dgu = up256(TF * 2);
-  s.slots = s.dgu + up256(TF * 4);
+  s.dgu = up256((size_t)d.tokens * act_pitch(d) * 2);
+  s.slots = s.dgu + up256((size_t)d.tokens * dgu_pitch(d) * 2);
   s.total = s.slots + larger(balanced_gemm_scratch_bytes(dx_problem(d)),
                              larger(balanced_gemm_scratch_bytes(dw_problem(d, grad_dtype)), balanced_gemm_scratch_bytes(dd_problem(d, grad_dtype))));
   return s;
