@@ -62,7 +62,7 @@ def _build_binding(force: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}",
            "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", str(cuda / "include"), str(BINDING_SRC), "-o", str(BINDING), f"-L{torch_dir / 'lib'}",
-           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
