@@ -64,7 +64,8 @@ __device__ __forceinline__ void clear(V& v) { v.raw = {}; }
 
 struct RowShape {
   int64_t rows;
-  int C, W;  // W warps a row, a power of two
+  int C, W;     // W warps a row, a power of two
+  float inv_c;  // 1 / C
 };
 
 // NORM false: y = x, only quantised. OUT8: q and scale instead of y.
@@ -73,7 +74,7 @@ __global__ void __maxnreg__((NV * Vec16<T>::N > 16) ? 128 : 80)
 rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float* __restrict__ gamma, T* h_out, T* __restrict__ y,
                    uint8_t* __restrict__ q, float* __restrict__ scale, float* __restrict__ rstd, float eps) {
   constexpr int V = Vec16<T>::N;
-  constexpr bool AHEAD = NV <= 2;  // the next row's vectors beside the current one's
+  constexpr bool AHEAD = NV * V <= 16;  // the next row's vectors beside the current one's
   __shared__ float red[2][32];
   pdl_enter();
   const int W = s.W, groups = (int)(blockDim.x >> 5) / W, grp = (int)(threadIdx.x >> 5) / W;
@@ -90,23 +91,23 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
     }
   }
   Vec16<T> xv[NV], rv[NV];
-  auto fetch = [&](int64_t row) {
+  auto fetch = [&](int64_t row, int64_t at) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * W * 32;
       clear(xv[i]);
       clear(rv[i]);
-      if (row < s.rows && v < nv) {
-        xv[i].load(x + row * s.C + v * V);
-        if (residual) rv[i].load(residual + row * s.C + v * V);
+      if (row < s.rows && lane + i * W * 32 < nv) {
+        xv[i].load(x + at + i * W * 32 * V);
+        if (residual) rv[i].load(residual + at + i * W * 32 * V);
       }
     }
   };
   int64_t row = (int64_t)blockIdx.x * groups + grp;
-  if (AHEAD) fetch(row);
-  for (; row < s.rows; row += step) {
-    const int64_t at = row * s.C;
-    if (!AHEAD) fetch(row);
+  int64_t at = row * s.C + lane * V;  // of this lane's first vector
+  const int64_t step_at = step * s.C;
+  if (AHEAD) fetch(row, at);
+  for (; row < s.rows; row += step, at += step_at) {
+    if (!AHEAD) fetch(row, at);
     float f[NV][V], sq = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -120,7 +121,7 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
 #pragma unroll
       for (int e = 0; e < V; ++e) sq = fmaf(f[i][e], f[i][e], sq);
     }
-    if (AHEAD) fetch(row + step);
+    if (AHEAD) fetch(row + step, at + step_at);
     if (h_out) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -128,11 +129,11 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
         if (v >= nv) continue;
         Vec16<T> o;
         o.pack(f[i]);
-        o.store(h_out + at + v * V);
+        o.store(h_out + at + i * W * 32 * V);
       }
     }
     if constexpr (NORM) {
-      const float rs = rsqrtf(group_all<false>(sq, W, red, turn) / (float)s.C + eps);
+      const float rs = rsqrtf(group_all<false>(sq, W, red, turn) * s.inv_c + eps);
       if (rstd && lane == 0) rstd[row] = rs;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -155,8 +156,8 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
         uint32_t w[V / 4];
 #pragma unroll
         for (int e = 0; e < V; e += 4) w[e / 4] = four_e4m3(f[i][e] * inv, f[i][e + 1] * inv, f[i][e + 2] * inv, f[i][e + 3] * inv);
-        if constexpr (V == 8) *reinterpret_cast<uint2*>(q + at + v * V) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(q + at + v * V) = w[0];
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(q + at + i * W * 32 * V) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(q + at + i * W * 32 * V) = w[0];
       }
     } else {
 #pragma unroll
@@ -165,7 +166,7 @@ rmsnorm_fwd_kernel(const RowShape s, const T* x, const T* residual, const float*
         if (v >= nv) continue;
         Vec16<T> o;
         o.pack(f[i]);
-        o.store(y + at + v * V);
+        o.store(y + at + i * W * 32 * V);
       }
     }
   }
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(512, 1)
 rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const float* __restrict__ gamma,
                    const float* __restrict__ rstd, const T* dh, T* dx, float* __restrict__ partial) {
   constexpr int V = Vec16<T>::N;
-  constexpr bool AHEAD = NV <= 2;
+  constexpr bool AHEAD = NV * V <= 16;
   extern __shared__ float cols[];  // [row groups of the block][C]
   __shared__ float red[2][32];
   pdl_enter();
@@ -193,30 +194,31 @@ rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const
   }
   Vec16<T> gv[NV], hv[NV], av[NV];
   float rs_next = 0.f;
-  auto fetch = [&](int64_t row) {
+  auto fetch = [&](int64_t row, int64_t at) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * W * 32;
       clear(gv[i]);
       clear(hv[i]);
       clear(av[i]);
-      if (row < s.rows && v < nv) {
-        gv[i].load(dy + row * s.C + v * V);
-        hv[i].load(h + row * s.C + v * V);
-        if (dh) av[i].load(dh + row * s.C + v * V);
+      if (row < s.rows && lane + i * W * 32 < nv) {
+        gv[i].load(dy + at + i * W * 32 * V);
+        hv[i].load(h + at + i * W * 32 * V);
+        if (dh) av[i].load(dh + at + i * W * 32 * V);
       }
     }
     rs_next = row < s.rows ? rstd[row] : 0.f;
   };
   int64_t row = (int64_t)blockIdx.x * groups + grp;
-  if (AHEAD) fetch(row);
-  for (; row < s.rows; row += step) {
-    if (!AHEAD) fetch(row);
+  int64_t at = row * s.C + lane * V;  // of this lane's first vector
+  const int64_t step_at = step * s.C;
+  if (AHEAD) fetch(row, at);
+  for (; row < s.rows; row += step, at += step_at) {
+    if (!AHEAD) fetch(row, at);
     const float rs = rs_next;
     Vec16<T> g0[NV], h0[NV], a0[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) { g0[i] = gv[i]; h0[i] = hv[i]; a0[i] = av[i]; }
-    if (AHEAD) fetch(row + step);
+    if (AHEAD) fetch(row + step, at + step_at);
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -230,7 +232,7 @@ rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const
         dot = fmaf(p, gm[i][e], dot);
       }
     }
-    dot = group_all<false>(dot, W, red, turn) / (float)s.C;
+    dot = group_all<false>(dot, W, red, turn) * s.inv_c;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = lane + i * W * 32;
@@ -243,7 +245,7 @@ rmsnorm_bwd_kernel(const RowShape s, const T* dy, const T* __restrict__ h, const
       for (int e = 0; e < V; ++e) a[e] += rs * (g[e] * gm[i][e] - f[e] * rs * dot);
       Vec16<T> o;
       o.pack(a);
-      o.store(dx + row * s.C + v * V);
+      o.store(dx + at + i * W * 32 * V);
     }
   }
   // the groups of the block in order
@@ -289,8 +291,11 @@ rmsnorm_dgamma_kernel(const float* __restrict__ partial, int blocks, int C, floa
 // Warps a row: as few as hold it in 16 elements a lane, and more where the rows are too few to occupy the device; only bf16
 // rows beyond 8192 have more elements a lane. Three blocks of eight warps an SM in forward (80 registers a thread), one of
 // sixteen in backward.
-// 8192 rows of 896 in bf16, inputs out of memory: forward 13.7 us with one warp and four vectors a lane, without the next
-// row in flight; backward 28.6 us.
+// 8192 rows of 896 in bf16, out of memory: forward 12.3 us, 4.8 TB/s (13.7 with one warp and four vectors a lane, without the
+// next row in flight; 14.6 through a ring of bulk copies in shared memory; 13.3 with 32 bytes a lane and load), backward 15.9
+// (28.6; 19.2; 18.5). 777 fp32 rows of 2056 5.1 us. Both keep the issue slots 63 % busy at 36 % (25 % in backward) of the
+// warps an SM can hold, waiting for arithmetic as much as for memory: unpacking, summing and packing take 22 instructions an
+// element and lane, and more warps would need the registers that hold the rows.
 struct RowLaunch {
   RowShape s;
   int nv, threads;
@@ -302,7 +307,7 @@ RowLaunch row_launch(int64_t rows, int C, int vec, int warps, int per_sm) {
   while (W < 16 && C > W * 32 * 16) W *= 2;
   const int sms = sm_count();
   while (W < 16 && rows * W < 8ll * sms && ceil_div(C, W * 32 * vec) > 1) W *= 2;
-  l.s = {rows, C, W};
+  l.s = {rows, C, W, 1.f / (float)C};
   l.nv = ceil_div(C, W * 32 * vec);
   if (warps < W) warps = W;
   while (warps > W && rows * W < (int64_t)warps * sms) warps /= 2;  // one row a block before a second one
