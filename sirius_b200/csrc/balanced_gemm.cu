@@ -9,6 +9,11 @@
 //
 // Warps as in the gated kernels: 0 TMA, 1 MMA, 2-17 four epilogue groups that take the 32-column slabs of a tile in turn. The
 // accumulator is double-buffered in tensor memory, so the epilogue of a tile runs beside the products of the next.
+//
+// Of the feed-forward block of 8192 tokens x 896 x 4864: y 58 us, 1230 TFLOP/s (a join of 5 beside it); dx 98 us, 1460, tensor pipe
+// 80 % busy; dWg over dWu 94 us, 1520, 83 %; dWd 56 us, 1280, 70 % (133 tiles for 148 CTAs). Operands come out of L2 at 11 to
+// 15 TB/s, which is what single CTAs are bound by; pairs read half of B each. A library product of these sizes takes 57, 109, 123
+// and 57 us. Two slabs for the output of an epilogue group instead of one cost a stage: dWd 55 -> 67 us.
 #include <cuda.h>
 
 #include <atomic>

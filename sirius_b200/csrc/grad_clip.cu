@@ -22,9 +22,15 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int GC_THREADS = 512;
-constexpr int GC_CHUNK = 32768;       // elements
+// Elements of a chunk. The norm of 508 M fp32 in 169 tensors takes 353 us (5.8 TB/s), in chunks of 8192 elements 396 and of 16384
+// 390; scaling them takes 656 (6.2 TB/s), and 683 in chunks of 131072. The conversions to 64 bits are what keeps the norm from
+// the memory's rate: with squares added in fp32 16 at a time it reads 498 MB in 91 us instead of 102, but then its last bit is
+// no longer the sum's.
+constexpr int GC_CHUNK = 32768;
 constexpr int GC_MAX_BLOCKS = 1024;   // partial sums of a launch
-constexpr int GC_FEW = 32, GC_MANY = 1024;  // tensors in the parameters of a launch
+// Tensors in the parameters of a launch. They are copied whole, 0.6 or 20 KB: 30 tensors take 7.0 us of the host with the short
+// list and 9.5 with the long one; a hundred would take four launches a pass with the short one.
+constexpr int GC_FEW = 32, GC_MANY = 1024;
 
 template <int MAXT>
 struct TensorList {
@@ -175,7 +181,7 @@ inline unsigned blocks_for(int chunks) {
   return (unsigned)(chunks < room ? chunks : room);
 }
 
-// Up to MAXT tensors a launch, chosen by the caller: the parameters of a launch are copied whole, 20 KB for 1024 tensors.
+// Up to MAXT tensors a launch.
 template <typename T, int MAXT>
 int run(int tensors, void* const* grads, const int64_t* counts, float max_norm, int scale, float* clip, double* partial, cudaStream_t st) {
   TensorList<MAXT> l;
