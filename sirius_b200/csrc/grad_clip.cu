@@ -6,10 +6,10 @@
 // depend on how the sum is cut beyond its last bits. A NaN anywhere makes norm and coefficient NaN, an infinity a coefficient
 // of zero; nothing is skipped on the way.
 //
-// The list of tensors travels in the kernel's parameters (nothing to copy, so a call can be captured), cut into chunks that
-// blocks take in turn. Bound by memory: one read for the norm; clipping in place reads and writes once more. The second
-// launch walks the chunks backwards, so that what the first one read last comes out of L2, and every block adds the partial
-// sums for itself instead of waiting for a launch between.
+// The list of tensors travels in the kernel's parameters (nothing to copy, so a call can be captured), cut into chunks of which
+// every block takes an equal share. Bound by memory: one read for the norm; clipping in place reads and writes once more. The
+// second launch walks each share backwards, so that what the first one read last comes out of L2, and every block adds the
+// partial sums for itself instead of waiting for a launch between.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -22,11 +22,11 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int GC_THREADS = 512;
-// Elements of a chunk. The norm of 508 M fp32 in 169 tensors takes 353 us (5.8 TB/s), in chunks of 8192 elements 396 and of 16384
-// 390; scaling them takes 656 (6.2 TB/s), and 683 in chunks of 131072. The conversions to 64 bits are what keeps the norm from
-// the memory's rate: with squares added in fp32 16 at a time it reads 498 MB in 91 us instead of 102, but then its last bit is
-// no longer the sum's.
-constexpr int GC_CHUNK = 32768;
+// Elements of a chunk: one turn of a block's loop over fp32. Every block takes the same number of chunks, one after the other:
+// the norm of 508 M fp32 in 169 tensors takes 344 us (5.9 TB/s), scaling them 657 (6.2 TB/s); with chunks of 32768 dealt in
+// turn 353 and 675. The conversions to 64 bits are what keeps the norm from the memory's rate: with squares added in fp32 16 at
+// a time it reads 498 MB in 91 us instead of 100, but then its last bit is no longer the sum's.
+constexpr int GC_CHUNK = 8192;
 constexpr int GC_MAX_BLOCKS = 1024;   // partial sums of a launch
 // Tensors in the parameters of a launch. They are copied whole, 0.6 or 20 KB: 30 tensors take 7.0 us of the host with the short
 // list and 9.5 with the long one; a hundred would take four launches a pass with the short one.
@@ -52,19 +52,37 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
   return v;
 }
 
-// The tensor of a chunk, and the chunk's elements [begin, begin + n).
-template <int MAXT>
-__device__ __forceinline__ int find_chunk(const TensorList<MAXT>& l, int chunk, int64_t& begin, int& n) {
+// A block's share: as many chunks as any other's or one more, one after the other. f(tensor, first element, elements) for every tensor that
+// the share meets, in order or (BACK) in the opposite order.
+template <bool BACK, int MAXT, typename F>
+__device__ __forceinline__ void share_of_block(const TensorList<MAXT>& l, F&& f) {
+  constexpr int MOST = (1 << 28) / GC_CHUNK;  // chunks at a time, so that elements count in 32 bits
+  const int all = l.first[l.tensors], b = (int)blockIdx.x, each = all / (int)gridDim.x, over = all - each * (int)gridDim.x;
+  const int c0 = b * each + min(b, over), c1 = c0 + each + (b < over ? 1 : 0);  // the first `over` blocks have one more
+  if (c0 >= c1) return;
+  const int begin = BACK ? c1 - 1 : c0;
   int lo = 0, hi = l.tensors - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (l.first[mid] <= chunk) lo = mid;
+    if (l.first[mid] <= begin) lo = mid;
     else hi = mid - 1;
   }
-  begin = (int64_t)(chunk - l.first[lo]) * GC_CHUNK;
-  const int64_t left = l.n[lo] - begin;
-  n = left < GC_CHUNK ? (int)left : GC_CHUNK;
-  return lo;
+  for (int t = lo, c = BACK ? c1 : c0; BACK ? c > c0 : c < c1;) {
+    int from, to;  // chunks of tensor t
+    if (BACK) {
+      while (c <= l.first[t]) --t;
+      to = c;
+      from = max(max(c0, l.first[t]), c - MOST);
+      c = from;
+    } else {
+      while (c >= l.first[t + 1]) ++t;
+      from = c;
+      to = min(min(c1, l.first[t + 1]), c + MOST);
+      c = to;
+    }
+    const int64_t at = (int64_t)(from - l.first[t]) * GC_CHUNK, end = (int64_t)(to - l.first[t]) * GC_CHUNK;
+    f(t, at, (int)((end < l.n[t] ? end : l.n[t]) - at));
+  }
 }
 // Elements before the first 16-byte boundary.
 template <typename T>
@@ -80,10 +98,7 @@ grad_norm_partial_kernel(const __grid_constant__ TensorList<MAXT> l, double* __r
   __shared__ double sh[GC_THREADS / 32];
   pdl_enter();
   double acc = 0.0;
-  for (int chunk = blockIdx.x; chunk < l.first[l.tensors]; chunk += gridDim.x) {
-    int64_t begin;
-    int n;
-    const int t = find_chunk(l, chunk, begin, n);
+  share_of_block<false>(l, [&](int t, int64_t begin, int n) {
     const T* p = (const T*)l.ptr[t] + begin;
     const int head = head_of(p, n), nv = (n - head) / V;
     const T* pv = p + head;
@@ -106,7 +121,7 @@ grad_norm_partial_kernel(const __grid_constant__ TensorList<MAXT> l, double* __r
     if ((int)threadIdx.x < head) one(ElemTraits<T>::to_f(p[threadIdx.x]));
     const int tail = head + nv * V + (int)threadIdx.x;
     if (tail < n) one(ElemTraits<T>::to_f(p[tail]));
-  }
+  });
   acc = block_sum(acc, sh);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
@@ -135,14 +150,11 @@ grad_scale_kernel(const __grid_constant__ TensorList<MAXT> l, const double* __re
   __shared__ double sh[GC_THREADS / 32];
   pdl_enter();
   const float k = coefficient_of(partial, count, max_norm, sh, clip);
-  for (int chunk = l.first[l.tensors] - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
-    int64_t begin;
-    int n;
-    const int t = find_chunk(l, chunk, begin, n);
+  share_of_block<true>(l, [&](int t, int64_t begin, int n) {
     T* p = (T*)l.ptr[t] + begin;
     const int head = head_of(p, n), nv = (n - head) / V;
     T* pv = p + head;
-    for (int v = threadIdx.x; v < nv; v += U * GC_THREADS) {
+    for (int v = (nv - 1) / (U * GC_THREADS) * (U * GC_THREADS) + (int)threadIdx.x; v >= 0; v -= U * GC_THREADS) {
       Vec16<T> a[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -161,7 +173,7 @@ grad_scale_kernel(const __grid_constant__ TensorList<MAXT> l, const double* __re
     if ((int)threadIdx.x < head) p[threadIdx.x] = ElemTraits<T>::from_f(ElemTraits<T>::to_f(p[threadIdx.x]) * k);
     const int tail = head + nv * V + (int)threadIdx.x;
     if (tail < n) p[tail] = ElemTraits<T>::from_f(ElemTraits<T>::to_f(p[tail]) * k);
-  }
+  });
 }
 
 template <int MAXT>
@@ -253,7 +265,7 @@ int grad_norm(int dtype, int tensors, void* const* grads, const int64_t* counts,
     SRT_REQUIRE(counts[i] >= 0 && (counts[i] == 0 || grads[i]), "grad_norm: tensor %d has no memory or a negative count", i);
     SRT_REQUIRE(((uintptr_t)grads[i] & (dtype == SRT_F32 ? 3 : 1)) == 0, "grad_norm: tensor %d is not aligned to its elements", i);
     chunks += counts[i] / GC_CHUNK + 1;
-    SRT_REQUIRE(chunks < (1ll << 30), "grad_norm: more than 2^45 elements");
+    SRT_REQUIRE(chunks < (1ll << 30), "grad_norm: more than 2^43 elements");
   }
   if (scale) {
     const int twice = first_overlap(dtype == SRT_F32 ? 4 : 2, tensors, grads, counts);
