@@ -47,6 +47,7 @@ constexpr int epi_groups(bool pair) { return pair ? 4 : 2; }                  //
 constexpr int ffn_threads(bool pair) { return 64 + 128 * epi_groups(pair); }
 constexpr int F_MAX_STAGES = 16;
 constexpr int F_SLAB_BYTES = FM * 64;    // 128 x 32 bf16 on the way out, 64-byte swizzle
+constexpr int F_NARROW_BYTES = FM * 32;  // 128 x 16 bf16, 32-byte swizzle: three a group of a single CTA, in backward
 enum { W_FFN_LOAD = 0x31, W_FFN_FULL = 0x32, W_FFN_ACC = 0x33, W_FFN_EPI = 0x34, W_FFN_DRAIN = 0x35 };
 
 struct FfnParams {
@@ -58,8 +59,9 @@ struct FfnParams {
   uint32_t a_bytes;            // of a stage: with fewer than 128 tokens only their rows; the products read on into what
                                // follows, and the rows of the accumulators that this fills are not stored
   uint32_t gu_bytes, da_bytes; // what one CTA loads a k-block in either phase
-  bf16 *act, *dgu;             // outputs without a tensor map (single CTAs)
-  int act_pitch, dgu_pitch;    // of their rows
+  int slab_bytes;              // shared memory that outputs pass through on their way to TMA; 0: straight from registers to
+  bf16 *act, *dgu;             // these, rows so far apart
+  int act_pitch, dgu_pitch;
   const float *x_scale, *w_scale;
   int* status;
 };
@@ -95,8 +97,8 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int NS = p.stages;
-  uint8_t* sOut = base + NS * p.stage_bytes;  // a slab per epilogue group, pairs only
-  uint64_t* bars = (uint64_t*)(sOut + (PAIR ? epi_groups(true) * F_SLAB_BYTES : FM * 128 - (int)p.a_bytes));
+  uint8_t* sOut = base + NS * p.stage_bytes;
+  uint64_t* bars = (uint64_t*)(sOut + p.slab_bytes + (PAIR ? 0 : FM * 128 - (int)p.a_bytes));
   const uint32_t full = smem_u32(bars), empty = full + 8 * F_MAX_STAGES, acc_full = empty + 8 * F_MAX_STAGES, acc_empty = acc_full + 16;
   uint32_t* tmem_ptr = (uint32_t*)(bars + 2 * F_MAX_STAGES + 4);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -324,47 +326,91 @@ gated_ffn_kernel(const FfnParams p, const __grid_constant__ CUtensorMap tx, cons
           }
         }
       } else {
-        // eight channels at a time, dealt to the two groups in turn
-        if (m0 < p.T)
-          for (int c = grp * 8; c < g; c += 16) {
-            uint32_t gv[8], uv[8], dv[8];
-            tmem_ld_32x32b_x8(t_gu + (uint32_t)c, gv);
-            tmem_ld_32x32b_x8(t_gu + (uint32_t)(g + c), uv);
-            if constexpr (BWD) tmem_ld_32x32b_x8(t_da + (uint32_t)c, dv);
-            tmem_ld_wait();
-            const int f = n0 + c;
-            if (mrow < p.T && f < p.F) {
-              float a[8], dg[8], du[8];
+        if (BWD && p.slab_bytes) {
+          // sixteen channels at a time, dealt to the two groups in turn
+          const uint32_t slab = smem_u32(sOut) + (uint32_t)grp * 3 * F_NARROW_BYTES, mine = slab + (uint32_t)row * 32u;
+          const uint32_t flip = (uint32_t)(row >> 2) & 1u;
+          if (m0 < p.T)
+            for (int c = grp * 16; c < g && n0 + c < p.F; c += 32) {
+              uint32_t gv[16], uv[16], dv[16], w[3][8];
+              tmem_ld_32x32b_x16(t_gu + (uint32_t)c, gv);
+              tmem_ld_32x32b_x16(t_gu + (uint32_t)(g + c), uv);
+              tmem_ld_32x32b_x16(t_da + (uint32_t)c, dv);
+              tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                float gt = __uint_as_float(gv[e]), up = __uint_as_float(uv[e]);
-                if (E4M3) {
-                  gt *= xs * p.w_scale[f + e];
-                  up *= xs * p.w_scale[p.F + f + e];
+              for (int e = 0; e < 16; e += 2) {
+                float a[2], dg[2], du[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const float gt = __uint_as_float(gv[e + k]), up = __uint_as_float(uv[e + k]), da = __uint_as_float(dv[e + k]);
+                  const float sg = sigmoid_f(gt), silu = gt * sg;
+                  a[k] = silu * up;
+                  dg[k] = da * up * (sg + silu * (1.f - sg));
+                  du[k] = da * silu;
                 }
-                const float sg = sigmoid_f(gt), silu = gt * sg;
-                a[e] = silu * up;
-                if constexpr (BWD) {
-                  const float da = __uint_as_float(dv[e]);
-                  dg[e] = da * up * (sg + silu * (1.f - sg));
-                  du[e] = da * silu;
-                }
+                w[0][e / 2] = pack_bf16(a[0], a[1]);
+                w[1][e / 2] = pack_bf16(dg[0], dg[1]);
+                w[2][e / 2] = pack_bf16(du[0], du[1]);
               }
-              Vec16<bf16> o;
-              o.pack(a);
-              o.store(p.act + (size_t)mrow * p.act_pitch + f);
-              if constexpr (BWD) {
-                o.pack(dg);
-                o.store(p.dgu + (size_t)mrow * p.dgu_pitch + f);
-                o.pack(du);
-                o.store(p.dgu + (size_t)mrow * p.dgu_pitch + p.F + f);
+              if (issuer) bulk_wait_group_read<0>();  // the stores before have read the slabs
+              named_bar_sync(1 + grp, 128);
+#pragma unroll
+              for (int o = 0; o < 3; ++o)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+                  st_shared_v4(mine + (uint32_t)o * F_NARROW_BYTES + (((uint32_t)v ^ flip) << 4), w[o][4 * v], w[o][4 * v + 1], w[o][4 * v + 2], w[o][4 * v + 3]);
+              fence_proxy_async_smem();
+              named_bar_sync(1 + grp, 128);
+              if (issuer) {
+                tma_store_2d(&tact, slab, n0 + c, m0);
+                tma_store_2d(&tgate, slab + F_NARROW_BYTES, n0 + c, m0);
+                tma_store_2d(&tup, slab + 2 * F_NARROW_BYTES, n0 + c, m0);
+                bulk_commit_group();
               }
             }
-          }
+        } else {
+          // eight channels at a time, dealt to the two groups in turn
+          if (m0 < p.T)
+            for (int c = grp * 8; c < g; c += 16) {
+              uint32_t gv[8], uv[8], dv[8];
+              tmem_ld_32x32b_x8(t_gu + (uint32_t)c, gv);
+              tmem_ld_32x32b_x8(t_gu + (uint32_t)(g + c), uv);
+              if constexpr (BWD) tmem_ld_32x32b_x8(t_da + (uint32_t)c, dv);
+              tmem_ld_wait();
+              const int f = n0 + c;
+              if (mrow < p.T && f < p.F) {
+                float a[8], dg[8], du[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  float gt = __uint_as_float(gv[e]), up = __uint_as_float(uv[e]);
+                  if (E4M3) {
+                    gt *= xs * p.w_scale[f + e];
+                    up *= xs * p.w_scale[p.F + f + e];
+                  }
+                  const float sg = sigmoid_f(gt), silu = gt * sg;
+                  a[e] = silu * up;
+                  if constexpr (BWD) {
+                    const float da = __uint_as_float(dv[e]);
+                    dg[e] = da * up * (sg + silu * (1.f - sg));
+                    du[e] = da * silu;
+                  }
+                }
+                Vec16<bf16> o;
+                o.pack(a);
+                o.store(p.act + (size_t)mrow * p.act_pitch + f);
+                if constexpr (BWD) {
+                  o.pack(dg);
+                  o.store(p.dgu + (size_t)mrow * p.dgu_pitch + f);
+                  o.pack(du);
+                  o.store(p.dgu + (size_t)mrow * p.dgu_pitch + p.F + f);
+                }
+              }
+            }
+        }
         done();
       }
     }
-    if (PAIR && issuer) bulk_wait_group_read<0>();  // the slab outlives the last store's read
+    if ((PAIR || BWD) && issuer) bulk_wait_group_read<0>();  // the slab outlives the last store's read
   }
 
   tc_fence_before_sync();
@@ -426,7 +472,7 @@ template <bool PAIR, bool BWD, bool E4M3>
 int launch_ffn(FfnParams& p, const CUtensorMap (&tm)[7], cudaStream_t st) {
   const size_t budget = PAIR || p.cols > 256 ? 232448 : 113 * 1024;  // two single CTAs share an SM where tensor memory allows
   // a single CTA with few tokens reads up to 16 KB beyond a stage's rows
-  const size_t fixed = 1024 + (PAIR ? epi_groups(true) * F_SLAB_BYTES : FM * 128 - (int)p.a_bytes) + ffn_tail_bytes();
+  const size_t fixed = 1024 + (size_t)p.slab_bytes + (PAIR ? 0 : FM * 128 - (int)p.a_bytes) + ffn_tail_bytes();
   p.stages = (int)((budget - fixed) / p.stage_bytes);
   if (p.stages > F_MAX_STAGES) p.stages = F_MAX_STAGES;
   const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
@@ -489,6 +535,11 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   p.dgu = (bf16*)dgu;
   p.act_pitch = act_pitch(d);
   p.dgu_pitch = dgu_pitch(d);
+  // A warp that stores 16 bytes of each of its 32 rows takes 32 turns for it, three times in backward. Through slabs instead, single
+  // CTAs make a whole backward pass of 333 x 896 x 4864 take 44.7 us and not 45.5, of 777 tokens 71.5 and not 75.9; with fewer
+  // rows than a tile's the stages that the slabs cost weigh more: 64 tokens 35.0 and not 32.5.
+  const bool slabs = !plan.pair && bwd && T >= FM;
+  p.slab_bytes = plan.pair ? epi_groups(true) * F_SLAB_BYTES : slabs ? epi_groups(false) * 3 * F_NARROW_BYTES : 0;
   p.x_scale = x_scale;
   p.w_scale = w_scale;
   p.status = tc_status_device_ptr();
@@ -498,10 +549,11 @@ int gated_products(const srt_gated_ffn_desc& d, const void* x, const float* x_sc
   if ((rc = tmap_rows_128b(&tm[0], x, T, C, C, esz, a_rows)) || (rc = tmap_rows_128b(&tm[1], w_gu, 2ull * F, C, C, esz, b_rows))) return rc;
   for (int i = 2; i < 7; ++i) tm[i] = tm[0];
   if (bwd && ((rc = tmap_rows_128b(&tm[2], dy, T, C, C, 2, a_rows)) || (rc = tmap_rows_128b(&tm[3], w_down, C, F, F, 2, 64)))) return rc;
-  if (plan.pair && (rc = tmap_rows(&tm[4], act, T, F, p.act_pitch, 2, 32, FM))) return rc;
+  const int out_cols = plan.pair ? 32 : 16;
+  if ((plan.pair || slabs) && (rc = tmap_rows(&tm[4], act, T, F, p.act_pitch, 2, out_cols, FM))) return rc;
   // the two halves of dgu have maps of their own: a store that reaches beyond `hidden` is clipped in either
-  if (plan.pair && bwd && ((rc = tmap_rows(&tm[5], dgu, T, F, p.dgu_pitch, 2, 32, FM)) ||
-                           (rc = tmap_rows(&tm[6], (bf16*)dgu + F, T, F, p.dgu_pitch, 2, 32, FM))))
+  if (bwd && (plan.pair || slabs) && ((rc = tmap_rows(&tm[5], dgu, T, F, p.dgu_pitch, 2, out_cols, FM)) ||
+                                      (rc = tmap_rows(&tm[6], (bf16*)dgu + F, T, F, p.dgu_pitch, 2, out_cols, FM))))
     return rc;
   if (bwd) return plan.pair ? launch_ffn<true, true, false>(p, tm, st) : launch_ffn<false, true, false>(p, tm, st);
   if (e4m3) return plan.pair ? launch_ffn<true, false, true>(p, tm, st) : launch_ffn<false, false, true>(p, tm, st);

@@ -1744,8 +1744,8 @@ int tmap_batched_bf16(CUtensorMap* tm, const void* base, uint64_t kdim, uint64_t
   return make_tmap_4d(tm, base, kdim, rows, z1, z2, ld, s1, s2, box_rows);
 }
 
-// Row-major matrix of 1-byte, bf16 or fp32 elements, rows `pitch` elements apart. Boxes of 64 or 128 bytes x box_rows, swizzled
-// over that width.
+// Row-major matrix of 1-byte, bf16 or fp32 elements, rows `pitch` elements apart. Boxes of 32, 64 or 128 bytes x box_rows,
+// swizzled over that width.
 int tmap_rows(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, int elem_bytes, uint32_t box_cols, uint32_t box_rows) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) {
@@ -1761,7 +1761,10 @@ int tmap_rows(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, u
                                    : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = fn(tm, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  box_cols * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  box_cols * elem_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
+                  : box_cols * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
