@@ -566,9 +566,11 @@ split_gemm_kernel(const SplitParams p, const __grid_constant__ CUtensorMap ta, c
 // How a problem is cut: the cut with the least time by this model, in microseconds, of which the constants were measured (with
 // both forms, every tile width and all three operand orders, 74 pairs busy). A k-block takes 0.155 at least, 1.53 ns a column
 // of the tile for the products, and its bytes at 115 KB out of L2 (rows that do not begin on 128 bytes take half as much again),
-// or, where B is read only once, 40 KB out of memory. An epilogue takes 0.35 and 10 ns a column, in fp32 17, and runs beside the
-// next tile's products. Sharing the rest of the tiles takes a launch and the slots' way to memory and back, some 3.5 MB.
-// Against the best cut found by trying all: within 5 % for 13 of 16 problems of 8 to 8192 rows.
+// or, where B is read only once, 40 KB out of memory. An epilogue takes 0.7, a pair's 1.0, and 7 ns a column, in fp32 10, and runs beside
+// the next tile's products. Sharing the rest of the tiles takes a launch and the slots' way to memory and back, some 3.5 MB.
+// Against the best cut found by trying all: within 5 % for 13 of 16 problems of 8 to 8192 rows; for the weight gradients of 18
+// shapes and 1 to 2048 tokens, in both types, 2 % behind on the mean (8 with half the time for a tile's beginning and half as
+// much again a column: narrow tiles then look too good).
 //
 // A tile a cluster of c takes 3.6 to begin and end, 0.16 c and 0.195 ns an element of the tile to bring the parts together, and
 // a step of 128 along the reduction 0.28 at least, 2.8 ns a column, its bytes at 160 KB and 16.5 TB/s on all of them; where B is
@@ -670,7 +672,7 @@ GemmPlan plan_gemm(const GemmProblem& q, size_t room) {
       at_least(0.00153 * n);
       at_least((a_bytes + b_bytes) / 115e3);
       if (g.m_units == 1) at_least(b_bytes / 40e3 + 0.03);
-      const double t_epi = 0.35 + (q.out_dtype == SRT_F32 ? 0.017 : 0.010) * n;
+      const double t_epi = (pair ? 1.0 : 0.7) + (q.out_dtype == SRT_F32 ? 0.010 : 0.007) * n;
       for (int share = 0; share < 2; ++share) {
         const long long most = (long long)g.tiles * kb / LEAST;  // units that have something to do
         g.units = share && most > g.tiles ? (most < all ? (int)most : all) : (g.tiles < all ? g.tiles : all);
