@@ -348,26 +348,32 @@ int fwd_launch(int64_t rows, int C, const void* x, const void* residual, const f
     default: return go(rmsnorm_fwd_kernel<T, 4, NORM, OUT8>);
   }
 }
+// The columns of dgamma that a block adds up, one set a row group: at most 32 KB, and 64 where sixteen warps share a row. They come on
+// top of the kernel's static shared memory, so the limit is raised for every instance and not where they alone pass 48 KB.
+constexpr int RN_BWD_SMEM = 64 * 1024;
+template <typename T, int NV>
+int bwd_instance(const RowLaunch& l, int C, const void* dy, const void* h, const float* gamma, const float* rstd, const void* dh, void* dx,
+                 float* dgamma, float* partial, cudaStream_t st) {
+  const size_t smem = (size_t)(l.threads / 32 / l.s.W) * C * sizeof(float);
+  static SmemOptIn opt_in;
+  SRT_CHECK_CUDA(opt_in.set(rmsnorm_bwd_kernel<T, NV>, RN_BWD_SMEM));
+  SRT_CHECK_CUDA(launch_pdl(rmsnorm_bwd_kernel<T, NV>, dim3(l.blocks), dim3(l.threads), smem, st, l.s, (const T*)dy, (const T*)h, gamma, rstd,
+                            (const T*)dh, (T*)dx, partial));
+  SRT_LAUNCH_CHECK();
+  SRT_CHECK_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3(ceil_div(C, 16)), dim3(256), 0, st, (const float*)partial, (int)l.blocks, C, dgamma));
+  SRT_LAUNCH_CHECK();
+  return SRT_OK;
+}
 template <typename T>
 int bwd_launch(int64_t rows, int C, const void* dy, const void* h, const float* gamma, const float* rstd, const void* dh, void* dx,
                float* dgamma, float* partial, cudaStream_t st) {
   const RowLaunch l = row_launch(rows, C, Vec16<T>::N, 16, 1);
   SRT_REQUIRE(l.blocks <= RN_MAX_BLOCKS, "rmsnorm_bwd: %u partial rows", l.blocks);
-  const size_t smem = (size_t)(l.threads / 32 / l.s.W) * C * sizeof(float);
-  auto go = [&](auto kernel) -> int {
-    if (smem > 48 * 1024) SRT_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
-    SRT_CHECK_CUDA(launch_pdl(kernel, dim3(l.blocks), dim3(l.threads), smem, st, l.s, (const T*)dy, (const T*)h, gamma, rstd, (const T*)dh,
-                              (T*)dx, partial));
-    SRT_LAUNCH_CHECK();
-    SRT_CHECK_CUDA(launch_pdl(rmsnorm_dgamma_kernel, dim3(ceil_div(C, 16)), dim3(256), 0, st, (const float*)partial, (int)l.blocks, C, dgamma));
-    SRT_LAUNCH_CHECK();
-    return SRT_OK;
-  };
   switch (l.nv) {
-    case 1: return go(rmsnorm_bwd_kernel<T, 1>);
-    case 2: return go(rmsnorm_bwd_kernel<T, 2>);
-    case 3: return go(rmsnorm_bwd_kernel<T, 3>);
-    default: return go(rmsnorm_bwd_kernel<T, 4>);
+    case 1: return bwd_instance<T, 1>(l, C, dy, h, gamma, rstd, dh, dx, dgamma, partial, st);
+    case 2: return bwd_instance<T, 2>(l, C, dy, h, gamma, rstd, dh, dx, dgamma, partial, st);
+    case 3: return bwd_instance<T, 3>(l, C, dy, h, gamma, rstd, dh, dx, dgamma, partial, st);
+    default: return bwd_instance<T, 4>(l, C, dy, h, gamma, rstd, dh, dx, dgamma, partial, st);
   }
 }
 
