@@ -348,12 +348,15 @@ PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     count(n, 3, c.what);
     const float max_norm = (float)number(a[1]);
     if (!(max_norm > 0.f)) value_error(std::string(c.what) + ": max_norm (" + std::to_string(max_norm) + ") must be positive");
-    PyObject* list = PySequence_Fast(a[0], "the gradients are a list of tensors");
-    if (!list) throw PySet{};
     struct Release {
       PyObject* o;
-      ~Release() { Py_DECREF(o); }
-    } release{list};
+      ~Release() { Py_XDECREF(o); }
+    } given{PySequence_Fast(a[0], "the gradients are a list of tensors")};
+    if (!given.o) throw PySet{};
+    // The call's own references: a caller's list may change in another thread while the lock is given up, and its tensors go.
+    const Release held{PySequence_Tuple(given.o)};
+    PyObject* list = held.o;
+    if (!list) throw PySet{};
     const Py_ssize_t tensors = PySequence_Fast_GET_SIZE(list);
     if (tensors > INT32_MAX) value_error(std::string(c.what) + ": too many tensors");
     std::vector<void*> ptr((size_t)tensors);
