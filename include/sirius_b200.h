@@ -406,9 +406,11 @@ int srt_step_optimizer(srt_step* s);
 /* Clipping of the next optimizer step (of every executor; srt_step_*, srt_gpt2_*, srt_swin_*, srt_qwen2_*): the norm of the
  * gradients that step would consume (accumulated ones where there are any) and the coefficient min(1, max_norm / (norm +
  * 1e-6)), which the step multiplies them by on their way in; the gradient buffer stays as it is. Call it after the
- * gradient exchange; a later forward_backward or accumulate takes it back. _grad_norm waits for the norm and reads it. */
+ * gradient exchange; a later forward_backward or accumulate takes it back. _grad_norm waits for the norm and reads it.
+ * _clip_pending: 1 while the next optimizer step has a coefficient to take. */
 int srt_step_clip_grad_norm(srt_step* s, float max_norm);
 int srt_step_grad_norm(srt_step* s, float* host_norm);
+int srt_step_clip_pending(srt_step* s);
 /* Scaled loss of the last micro-batch; synchronises the stream (loss.item()). */
 int srt_step_loss(srt_step* s, float* host_loss);
 int srt_step_logits(srt_step* s, float* host, int B);
@@ -467,6 +469,7 @@ int srt_gpt2_forward_only(srt_gpt2* g, int B);
 int srt_gpt2_optimizer(srt_gpt2* g);
 int srt_gpt2_clip_grad_norm(srt_gpt2* g, float max_norm); /* as srt_step_clip_grad_norm */
 int srt_gpt2_grad_norm(srt_gpt2* g, float* host_norm);
+int srt_gpt2_clip_pending(srt_gpt2* g);
 int srt_gpt2_loss(srt_gpt2* g, float* host_loss);        /* synchronises; loss of the last micro-batch */
 int srt_gpt2_logits(srt_gpt2* g, float* host, int B);    /* [B*seq][vocab], after forward_only */
 int srt_gpt2_synchronize(srt_gpt2* g);
@@ -576,6 +579,7 @@ int srt_swin_forward_only(srt_swin* s, int B);
 int srt_swin_optimizer(srt_swin* s);
 int srt_swin_clip_grad_norm(srt_swin* s, float max_norm); /* as srt_step_clip_grad_norm */
 int srt_swin_grad_norm(srt_swin* s, float* host_norm);
+int srt_swin_clip_pending(srt_swin* s);
 int srt_swin_loss(srt_swin* s, float* host_loss);
 int srt_swin_logits(srt_swin* s, float* host, int B);
 int srt_swin_synchronize(srt_swin* s);
@@ -619,6 +623,7 @@ int srt_qwen2_forward_only(srt_qwen2* g, int B);
 int srt_qwen2_optimizer(srt_qwen2* g);
 int srt_qwen2_clip_grad_norm(srt_qwen2* g, float max_norm); /* as srt_step_clip_grad_norm */
 int srt_qwen2_grad_norm(srt_qwen2* g, float* host_norm);
+int srt_qwen2_clip_pending(srt_qwen2* g);
 int srt_qwen2_loss(srt_qwen2* g, float* host_loss);
 int srt_qwen2_logits(srt_qwen2* g, float* host, int B);
 int srt_qwen2_synchronize(srt_qwen2* g);

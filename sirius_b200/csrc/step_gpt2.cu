@@ -617,6 +617,7 @@ int srt_gpt2_grad_norm(srt_gpt2* h, float* host_norm) {
   SRT_REQUIRE(g, "gpt2_grad_norm: null handle");
   return g->clip.read(host_norm, g->stream);
 }
+int srt_gpt2_clip_pending(srt_gpt2* h) { return h && ((Gpt2*)h)->clip.armed ? 1 : 0; }
 
 // Mean next-token loss of the last micro-batch over its own targets (what the reference's model returns).
 int srt_gpt2_loss(srt_gpt2* h, float* host_loss) {

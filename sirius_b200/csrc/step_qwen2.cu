@@ -629,6 +629,7 @@ int srt_qwen2_grad_norm(srt_qwen2* h, float* host_norm) {
   SRT_REQUIRE(g, "qwen2_grad_norm: null handle");
   return g->clip.read(host_norm, g->stream);
 }
+int srt_qwen2_clip_pending(srt_qwen2* h) { return h && ((Qwen2*)h)->clip.armed ? 1 : 0; }
 
 int srt_qwen2_recompute_mlp(srt_qwen2* h, int on) {
   Qwen2* g = (Qwen2*)h;

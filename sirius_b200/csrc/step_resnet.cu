@@ -1237,6 +1237,7 @@ int srt_step_grad_norm(srt_step* h, float* host_norm) {
   SRT_REQUIRE(s, "grad_norm: null handle");
   return s->clip.read(host_norm, s->stream);
 }
+int srt_step_clip_pending(srt_step* h) { return h && ((Step*)h)->clip.armed ? 1 : 0; }
 
 int srt_step_optimizer(srt_step* h) {
   Step* s = (Step*)h;

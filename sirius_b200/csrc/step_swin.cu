@@ -593,6 +593,7 @@ int srt_swin_grad_norm(srt_swin* h, float* host_norm) {
   SRT_REQUIRE(g, "swin_grad_norm: null handle");
   return g->clip.read(host_norm, g->stream);
 }
+int srt_swin_clip_pending(srt_swin* h) { return h && ((Swin*)h)->clip.armed ? 1 : 0; }
 
 // Mean cross-entropy of the last micro-batch.
 int srt_swin_loss(srt_swin* h, float* host_loss) {

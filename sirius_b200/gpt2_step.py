@@ -46,6 +46,7 @@ register({
     "srt_gpt2_forward_only": (None, [_vp, _i]),
     "srt_gpt2_clip_grad_norm": (None, [_vp, _f]),
     "srt_gpt2_grad_norm": (None, [_vp, C.POINTER(_f)]),
+    "srt_gpt2_clip_pending": (_i, [_vp]),
     "srt_gpt2_optimizer": (None, [_vp]),
     "srt_gpt2_loss": (None, [_vp, _pf]),
     "srt_gpt2_logits": (None, [_vp, _vp, _i]),
@@ -167,7 +168,9 @@ class Gpt2Step(GradBucketsMixin):
         call("srt_gpt2_forward_only", self._h, self._B)
 
     def clip_grad_norm(self, max_norm: float) -> None:
-        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them)."""
+        """The next optimizer_step scales the gradients (the accumulated ones, if there are any) by min(1, max_norm / norm of all of
+        them). Call it directly before that step, behind the gradient exchange: a later forward_backward or accumulate takes it
+        back. Loops of torch_col pass max_norm to MicroBatchManager.optimizer_step or GradAccumulator.step instead."""
         call("srt_gpt2_clip_grad_norm", self._h, max_norm)
 
     def grad_norm(self) -> float:
@@ -175,6 +178,11 @@ class Gpt2Step(GradBucketsMixin):
         v = C.c_float()
         call("srt_gpt2_grad_norm", self._h, C.byref(v))
         return v.value
+
+    @property
+    def clip_pending(self) -> bool:
+        """Whether the next optimizer_step has a coefficient of clip_grad_norm to take."""
+        return bool(_lib.lib().srt_gpt2_clip_pending(self._h))
 
     def optimizer_step(self) -> None:
         call("srt_gpt2_optimizer", self._h)

@@ -37,6 +37,7 @@ register({
     "srt_step_accumulate": (None, [_vp]),
     "srt_step_clip_grad_norm": (None, [_vp, C.c_float]),
     "srt_step_grad_norm": (None, [_vp, C.POINTER(C.c_float)]),
+    "srt_step_clip_pending": (_i, [_vp]),
     "srt_step_optimizer": (None, [_vp]),
     "srt_step_loss": (None, [_vp, C.POINTER(C.c_float)]),
     "srt_step_logits": (None, [_vp, _vp, _i]),
@@ -165,7 +166,9 @@ class ResNetStep:
         call("srt_step_accumulate", self._h)
 
     def clip_grad_norm(self, max_norm: float) -> None:
-        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them)."""
+        """The next optimizer_step scales the gradients (the accumulated ones, if there are any) by min(1, max_norm / norm of all of
+        them). Call it directly before that step, behind the gradient exchange: a later forward_backward or accumulate takes it
+        back. Loops of torch_col pass max_norm to MicroBatchManager.optimizer_step or GradAccumulator.step instead."""
         call("srt_step_clip_grad_norm", self._h, max_norm)
 
     def grad_norm(self) -> float:
@@ -173,6 +176,11 @@ class ResNetStep:
         v = C.c_float()
         call("srt_step_grad_norm", self._h, C.byref(v))
         return v.value
+
+    @property
+    def clip_pending(self) -> bool:
+        """Whether the next optimizer_step has a coefficient of clip_grad_norm to take."""
+        return bool(_lib.lib().srt_step_clip_pending(self._h))
 
     def optimizer_step(self) -> None:
         call("srt_step_optimizer", self._h)

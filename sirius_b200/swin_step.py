@@ -34,6 +34,7 @@ register({
     "srt_swin_forward_only": (None, [_vp, _i]),
     "srt_swin_clip_grad_norm": (None, [_vp, _f]),
     "srt_swin_grad_norm": (None, [_vp, C.POINTER(_f)]),
+    "srt_swin_clip_pending": (_i, [_vp]),
     "srt_swin_optimizer": (None, [_vp]),
     "srt_swin_loss": (None, [_vp, C.POINTER(_f)]),
     "srt_swin_logits": (None, [_vp, _vp, _i]),
@@ -104,7 +105,8 @@ class SwinStep(GradBucketsMixin):
         call("srt_swin_forward_only", self._h, self._B)
 
     def clip_grad_norm(self, max_norm: float) -> None:
-        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them)."""
+        """The next optimizer_step scales the gradients by min(1, max_norm / norm of all of them). Call it directly before that
+        step, behind the gradient exchange: a later forward_backward takes it back."""
         call("srt_swin_clip_grad_norm", self._h, max_norm)
 
     def grad_norm(self) -> float:
@@ -112,6 +114,11 @@ class SwinStep(GradBucketsMixin):
         v = C.c_float()
         call("srt_swin_grad_norm", self._h, C.byref(v))
         return v.value
+
+    @property
+    def clip_pending(self) -> bool:
+        """Whether the next optimizer_step has a coefficient of clip_grad_norm to take."""
+        return bool(_lib.lib().srt_swin_clip_pending(self._h))
 
     def optimizer_step(self) -> None:
         call("srt_swin_optimizer", self._h)

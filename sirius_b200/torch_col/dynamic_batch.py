@@ -15,6 +15,7 @@ import torch
 
 from . import _C
 from ._C import CtrlEvent, TrainMode, _DynamicBatchDistirbutor, _PerfModel
+from .accumulate import clip_module_grads
 from .colocate_ctrl import ColocateCtrl, CtrlBase, DummyCtrl, get_colocate_ctrl
 from .util import EventManager, MemoryPool
 
@@ -103,14 +104,18 @@ class MicroBatchManager:
             loss /= _DynamicBatchDistirbutor.get_global_batch_size() / self._dynamic_dataset.get_batch_size(batch)
         return loss
 
-    def optimizer_step(self, batch: Batch, optimizer=None, amp_scaler=None, grad_accumulator=None):
+    def optimizer_step(self, batch: Batch, optimizer=None, amp_scaler=None, grad_accumulator=None, max_norm=None):
+        """max_norm: the gradients of an update are scaled by min(1, max_norm / norm of all of them). Of micro-batches
+        that accumulate it is their sum that counts, so the norm is taken behind the last of them."""
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError(f"max_norm ({max_norm}) must be positive")
         if self._should_checkpoint_micro_batch():
             assert grad_accumulator is not None
             with get_colocate_ctrl().steps_no_interrupt():
                 ev = EventManager.record_event('optimizer_step')
                 grad_accumulator.accumulate()
                 if batch.should_update_param():
-                    grad_accumulator.step(optimizer, amp_scaler)
+                    grad_accumulator.step(optimizer, amp_scaler, **({} if max_norm is None else {'max_norm': max_norm}))
                     ev.tag = 'global'
                 else:
                     ev.tag = 'local'
@@ -118,8 +123,13 @@ class MicroBatchManager:
         else:
             def _step():
                 if hasattr(optimizer, 'optimizer_step'):   # a sirius_b200 step object
+                    if max_norm is not None:
+                        optimizer.clip_grad_norm(max_norm)
                     optimizer.optimizer_step()
-                elif amp_scaler is not None:
+                    return
+                if max_norm is not None:
+                    clip_module_grads([p for g in optimizer.param_groups for p in g['params']], max_norm, optimizer, amp_scaler)
+                if amp_scaler is not None:
                     amp_scaler.step(optimizer)
                     amp_scaler.update()
                     optimizer.zero_grad()
