@@ -202,7 +202,10 @@ int srt_adamw(float* p, const float* g, float* m, float* v, void* p_bf16, int64_
 /* Clipping by the norm of all gradients together (torch.nn.utils.clip_grad_norm_): clip[0] = sqrt(sum of squares, in 64 bits)
  * over `tensors` device arrays of one dtype, clip[1] = min(1, max_norm / (clip[0] + 1e-6)). srt_clip_grad_norm also multiplies
  * the arrays by clip[1] in place; the clipped optimizer steps take it from `clip` instead, which saves that pass. grads and
- * counts are host arrays and are read before the call returns. srt_clip_grad_norm refuses arrays that share memory. */
+ * counts are host arrays and are read before the call returns. srt_clip_grad_norm refuses arrays that share memory.
+ * srt_adamw_clipped forms 1 - beta and the bias corrections in 64 bits and rounds them once. srt_adamw, and the executors' steps
+ * with or without clipping, form them in fp32 from the rounded betas, so 1 - beta is off by up to 2^-25 / (1 - beta) of itself
+ * there (3e-5 for 0.999): with a coefficient of one the two agree to that, and the moments bit for bit where fp32 holds the betas exactly. */
 size_t srt_grad_norm_scratch_bytes(int tensors);
 int srt_grad_norm(int dtype, int tensors, const void* const* grads, const int64_t* counts, float max_norm, float* clip, void* scratch,
                   size_t scratch_bytes, void* stream);

@@ -603,7 +603,8 @@ int adamw(float* p, const float* g, float* m, float* v, void* pb, int64_t n, flo
   const float bc2 = 1.f - powf(b2, (float)step);
   return launch_adamw(p, g, m, v, pb, n, lr, b1, b2, 1.f - b1, 1.f - b2, eps, wd, bc1, sqrtf(bc2), coefficient, st);
 }
-// The constants in 64 bits: 1 - beta2 of a beta2 that was rounded to fp32 first is off by 1e-5.
+// The constants in 64 bits: 1 - beta2 of a beta2 that was rounded to fp32 first is off by 1e-5. adamw() above keeps its fp32
+// constants all the same, with a coefficient too: the executors' updates keep their bits.
 int adamw_clipped(float* p, const float* g, float* m, float* v, void* pb, int64_t n, double lr, double b1, double b2, double eps, double wd,
                   int step, const float* clip, cudaStream_t st) {
   if (n == 0) return SRT_OK;

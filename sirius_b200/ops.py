@@ -253,7 +253,12 @@ def sgd_momentum(p, g, m, lr, mu, wd, first_step, p_bf16=None, clip=None):
 
 
 def adamw(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16=None, clip=None):
-    """`clip`: what grad_norm returned; the gradients are multiplied by its coefficient on the way in."""
+    """`clip`: what grad_norm returned; the gradients are multiplied by its coefficient on the way in.
+
+    With `clip` the constants (1 - b1, 1 - b2, the bias corrections) are formed in 64 bits and rounded once. Without it, and in the
+    executors' steps in either case, they are formed in fp32 from the rounded betas, which training runs of before depend on bit
+    for bit: 1 - b is then off by up to 2^-25 / (1 - b) of itself (3e-5 for 0.999, nothing for betas that fp32 holds), and a
+    coefficient of one changes the update by as much."""
     if clip is not None:
         (_ops_native or _native()).adamw_clipped(p, g, m, v, lr, b1, b2, eps, wd, step, p_bf16, clip)
         return
