@@ -51,22 +51,31 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
 
 
 def _build_binding(force: bool) -> None:
-    """The native front ends of ops.py, against the torch of this interpreter (found, not imported)."""
+    """The native front ends of ops.py, against the torch of this interpreter (found, not imported). A stamp keeps what they were
+    built for, so that another torch, interpreter or command builds them again."""
+    import importlib.metadata
     import importlib.util
     import sysconfig
-    torch_dir = Path(next(iter(importlib.util.find_spec("torch").submodule_search_locations)))
-    newest = max(BINDING_SRC.stat().st_mtime, *(h.stat().st_mtime for h in (PKG.parent / "include").glob("*.h")))
-    if not force and BINDING.exists() and BINDING.stat().st_mtime >= newest:
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        sys.stderr.write("sirius_b200: torch is not installed, so the native front ends of sirius_b200.ops are left out\n")
         return
+    torch_dir = Path(next(iter(spec.submodule_search_locations)))
     cuda = Path(NVCC).resolve().parent.parent
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{sysconfig.get_paths()['include']}",
            "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", str(cuda / "include"), str(BINDING_SRC), "-o", str(BINDING), f"-L{torch_dir / 'lib'}",
            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+    stamp = BUILD / "_ops_native.stamp"
+    built_for = "\n".join(["torch " + importlib.metadata.version("torch"), str(sysconfig.get_config_var("SOABI")), *cmd]) + "\n"
+    newest = max(p.stat().st_mtime for p in (BINDING_SRC, *(PKG.parent / "include").glob("*.h")))
+    if (not force and BINDING.exists() and BINDING.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == built_for):
+        return
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"g++ failed on {BINDING_SRC.name}")
+    stamp.write_text(built_for)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -83,13 +92,13 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=max(1, min(8, len(jobs) + 1))) as ex:
         binding = ex.submit(_build_binding, force)
         list(ex.map(lambda j: _compile(j[0], j[1], verbose), jobs))
-        binding.result()
-    if jobs or not LIB.exists():
-        cmd = [NVCC, "-shared", "-o", str(LIB), *map(str, objs), "-lpthread", "-lrt", "-ldl"]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            sys.stderr.write(res.stdout + res.stderr)
-            raise RuntimeError("link failed")
+        if jobs or not LIB.exists():
+            cmd = [NVCC, "-shared", "-o", str(LIB), *map(str, objs), "-lpthread", "-lrt", "-ldl"]
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            if res.returncode != 0:
+                sys.stderr.write(res.stdout + res.stderr)
+                raise RuntimeError("link failed")
+        binding.result()  # the library is there whatever becomes of the front ends
     return LIB
 
 
