@@ -607,6 +607,9 @@ int srt_qwen2_create(const srt_qwen2_config* cfg, srt_qwen2** out);
  * SRT_ERR_ABORTED at the next layer boundary (kill batch); accumulate adds the micro-batch gradients to the
  * global-batch sum that the optimizer then consumes (pytorch/torch_col/accumulate.py:7-49). */
 int srt_qwen2_create_with_pool(const srt_qwen2_config* cfg, struct srt_pool* pool, srt_qwen2** out);
+/* pool may be null; recompute_mlp as srt_qwen2_recompute_mlp, but the activations are laid out once, in that mode: the larger set
+ * of the other one need not fit. */
+int srt_qwen2_create_with_options(const srt_qwen2_config* cfg, struct srt_pool* pool, int recompute_mlp, srt_qwen2** out);
 int srt_qwen2_accumulate(srt_qwen2* g);
 int srt_qwen2_release_activations(srt_qwen2* g, size_t* released_bytes);
 int srt_qwen2_shrink_activations(srt_qwen2* g, int B, size_t* released_bytes);

@@ -497,10 +497,15 @@ extern "C" {
 int srt_qwen2_create(const srt_qwen2_config* cfg, srt_qwen2** out) { return srt_qwen2_create_with_pool(cfg, nullptr, out); }
 
 int srt_qwen2_create_with_pool(const srt_qwen2_config* cfg, srt_pool* pool, srt_qwen2** out) {
+  return srt_qwen2_create_with_options(cfg, pool, 0, out);
+}
+
+int srt_qwen2_create_with_options(const srt_qwen2_config* cfg, srt_pool* pool, int recompute_mlp, srt_qwen2** out) {
   SRT_REQUIRE(cfg && out, "qwen2_create: null argument");
   Qwen2* g = new Qwen2();
   g->cfg = *cfg;
   g->pool = pool;
+  g->recompute_mlp = recompute_mlp != 0;
   int rc = g->build();
   if (rc == SRT_OK) rc = cudaStreamSynchronize(g->stream) == cudaSuccess ? SRT_OK : SRT_ERR_CUDA;
   if (rc != SRT_OK) { delete g; return rc; }

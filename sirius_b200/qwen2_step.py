@@ -22,6 +22,7 @@ class Qwen2ConfigC(C.Structure):
 register({
     "srt_qwen2_create": (None, [C.POINTER(Qwen2ConfigC), C.POINTER(_vp)]),
     "srt_qwen2_create_with_pool": (None, [C.POINTER(Qwen2ConfigC), _vp, C.POINTER(_vp)]),
+    "srt_qwen2_create_with_options": (None, [C.POINTER(Qwen2ConfigC), _vp, _i, C.POINTER(_vp)]),
     "srt_qwen2_accumulate": (None, [_vp]),
     "srt_qwen2_release_activations": (None, [_vp, C.POINTER(C.c_size_t)]),
     "srt_qwen2_shrink_activations": (None, [_vp, _i, C.POINTER(C.c_size_t)]),
@@ -66,9 +67,7 @@ class Qwen2Step(GradBucketsMixin):
         self.cfg, self.seq, self.vocab, self.max_batch = cfg, seq, vocab, max_batch
         self._h = _vp()
         self.pool = pool
-        call("srt_qwen2_create_with_pool", C.byref(cfg), pool if pool else None, C.byref(self._h))
-        if recompute_mlp:
-            self.recompute_mlp()
+        call("srt_qwen2_create_with_options", C.byref(cfg), pool if pool else None, int(recompute_mlp), C.byref(self._h))
         self.params = {}
         name, shape, ndim = C.create_string_buffer(256), (_i64 * 2)(), _i()
         for i in range(_lib.lib().srt_qwen2_num_params(self._h)):
