@@ -644,7 +644,8 @@ int srt_qwen2_recompute_mlp(srt_qwen2* h, int on) {
   int rc = g->free_activation_blocks();
   if (rc) return rc;
   g->recompute_mlp = on != 0;
-  return B > 0 ? g->alloc_activations(B) : (int)SRT_OK;
+  if (B > 0 && (rc = g->alloc_activations(B))) return rc;
+  return g->pool ? srt_pool_empty_cache(g->pool, SRT_POOL_TRAIN, nullptr) : (int)SRT_OK;  // what the mode saves goes back
 }
 
 int srt_qwen2_loss(srt_qwen2* h, float* host_loss) {

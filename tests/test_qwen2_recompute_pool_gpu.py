@@ -1,4 +1,5 @@
-"""recompute_mlp on a page pool: a pool that holds the mode's own activations is enough to create the step."""
+"""recompute_mlp on a page pool: a pool that holds the mode's own activations is enough to create the step, and switching the mode on
+hands the pages that it saves back to the pool."""
 from contextlib import ExitStack
 
 import numpy as np
@@ -54,3 +55,18 @@ def test_a_pool_that_holds_the_modes_own_activations_is_enough():
         got = gradients(step, state, ids)
         assert got[0] == want[0] and all(np.array_equal(got[1][n], want[1][n]) for n in want[1])
     assert ops.tc_status() == 0
+
+def test_switching_hands_the_saved_pages_back():
+    plain, recompute = sizes()
+    with ExitStack() as ends:
+        pool = PagePool((plain + (256 << 20)) / 2 ** 30, page_mb=2)
+        ends.callback(pool.close)
+        step = Qwen2Step(**CFG, max_batch=B, seq=S, pool=pool.handle)
+        ends.callback(step.close)
+        before = pool.stat("free_pages")
+        step.recompute_mlp()
+        gained = (pool.stat("free_pages") - before) * pool.stat("page_nbytes")
+        # whole pages of 2 MB, of which every block may share its first and its last with a neighbour
+        assert gained >= 0.9 * (plain - recompute), (gained, plain - recompute)
+        step.recompute_mlp(False)
+        assert pool.stat("free_pages") <= before + 8
