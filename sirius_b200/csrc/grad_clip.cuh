@@ -19,13 +19,14 @@ struct GradClip {
   GradClip() = default;
   GradClip(const GradClip&) = delete;
   GradClip& operator=(const GradClip&) = delete;
+  // With the step's other buffers: a step that runs takes no memory.
+  int prepare() {
+    SRT_CHECK_CUDA(cudaMalloc((void**)&clip, 256 + grad_norm_scratch_bytes(1)));
+    scratch = (char*)clip + 256;
+    return SRT_OK;
+  }
   int measure(float* grad, int64_t n, float max_norm, cudaStream_t st) {
     SRT_REQUIRE(max_norm > 0.f, "clip_grad_norm: max_norm (%g) must be positive", (double)max_norm);
-    if (!clip) {
-      const size_t need = 256 + grad_norm_scratch_bytes(1);
-      SRT_CHECK_CUDA(cudaMalloc((void**)&clip, need));
-      scratch = (char*)clip + 256;
-    }
     void* g = grad;
     int rc = grad_norm(SRT_F32, 1, &g, &n, max_norm, 0, clip, scratch, grad_norm_scratch_bytes(1), st);
     if (rc) return rc;

@@ -259,6 +259,7 @@ int Gpt2::build() {
   int rc;
   if ((rc = dalloc(&P, n_flat * 4, true))) return rc;
   if ((rc = dalloc(&G, n_flat * 4, true))) return rc;
+  if ((rc = clip.prepare())) return rc;
   if ((rc = dalloc(&M1, n_flat * 4, true))) return rc;
   if ((rc = dalloc(&M2, n_flat * 4, true))) return rc;
   if ((rc = dalloc(&Pw, n_flat * 2, true))) return rc;

@@ -272,6 +272,7 @@ int Qwen2::build() {
   if ((rc = dalloc(&P, n_flat * 4, true)) || (rc = dalloc(&G, n_flat * 4, true)) || (rc = dalloc(&M1, n_flat * 4, true)) ||
       (rc = dalloc(&M2, n_flat * 4, true)) || (rc = dalloc(&Pw, n_flat * 2, true)))
     return rc;
+  if ((rc = clip.prepare())) return rc;
   if ((rc = dalloc(&ACC, n_flat * 4, true)) || (rc = dalloc(&loss_acc, 256, true))) return rc;
   if ((rc = dalloc(&rope, (size_t)S * D * 4))) return rc;
   const size_t T = (size_t)cfg.max_batch * S;

@@ -457,6 +457,7 @@ int Step::build() {
   int rc;
   if ((rc = dalloc((void**)&P, n_flat * 4, true))) return rc;
   if ((rc = dalloc((void**)&G, n_flat * 4, true))) return rc;
+  if ((rc = clip.prepare())) return rc;
   if ((rc = dalloc((void**)&M, n_flat * 4, true))) return rc;
   if ((rc = dalloc((void**)&ACC, n_flat * 4, true))) return rc;
   if ((rc = dalloc((void**)&BUF, n_buf * 4, true))) return rc;

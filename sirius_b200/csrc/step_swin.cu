@@ -219,6 +219,7 @@ int Swin::build() {
   if ((rc = dalloc(&P, n_flat * 4, true)) || (rc = dalloc(&G, n_flat * 4, true)) || (rc = dalloc(&M1, n_flat * 4, true)) ||
       (rc = dalloc(&M2, n_flat * 4, true)) || (rc = dalloc(&Pw, n_flat * 2, true)))
     return rc;
+  if ((rc = clip.prepare())) return rc;
   const size_t B = cfg.max_batch, I = cfg.image;
   auto act = [&](__nv_bfloat16** p, size_t elems) { return dalloc(p, elems * 2, true); };
   if ((rc = dalloc(&stage_images, B * 3 * I * I * 4)) || (rc = dalloc(&stage_labels, B * 8))) return rc;
