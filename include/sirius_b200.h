@@ -525,8 +525,9 @@ int srt_lm_cross_entropy(void* logits, const int32_t* labels, int64_t rows, int 
 /* Root-mean-square norm of rows of C elements (C a multiple of 8, at most 32 KB a row), dtype SRT_F32 or SRT_BF16:
  *   h = x + residual (residual may be null), rstd = 1 / sqrt(mean(h^2) + eps), y = gamma h rstd.
  * h and rstd may be null; h may be x or residual. y is formed from the fp32 sum and rounded once. The e4m3 form writes q and
- * one scale a row instead of y: scale = max(max |y| / 448, 2^-126), q = e4m3(y / scale); srt_quantize_rows_e4m3 does the same
- * to rows as they are (weights). Backward: dx = dh + the norm's gradient (the gradient of x and of residual alike; dh, the
+ * one scale a row instead of y: scale = max(max |y| / 448, 2^-126), q = e4m3(y * (1 / scale)) with the reciprocal rounded to
+ * fp32 (next to a rounding border q may be the other neighbour of y / scale); srt_quantize_rows_e4m3 does the same to rows as
+ * they are (weights). Backward: dx = dh + the norm's gradient (the gradient of x and of residual alike; dh, the
  * gradient that reaches h by other ways, may be null; dx may be dy or dh), dgamma = sum over the rows in a fixed order,
  * overwritten. Operands are 16-byte aligned. Without rows nothing is written but dgamma = 0. */
 int srt_rmsnorm_fwd(int dtype, const void* x, const void* residual, const float* gamma, void* h, void* y, float* rstd, int64_t rows,
@@ -541,7 +542,8 @@ int srt_rmsnorm_bwd(int dtype, const void* dy, const void* h, const float* gamma
 /* Gated feed-forward block: act = silu(x Wg^T) * (x Wu^T), y = residual + act Wd^T, for x [tokens][width],
  * w_gate_up = Wg over Wu [2 hidden][width], w_down = Wd [width][hidden], all bf16, fp32 accumulation; width and hidden are
  * multiples of 8, operands and scratch 16-byte aligned, matrices below 2^31 elements. residual may be null. The gate and up
- * projections never reach memory. Backward forms them again from x: dx, dw_gate_up and dw_down (each may be null; the weights'
+ * projections never reach memory; act, and in backward the gradients of gate and up, are rounded to bf16 once, as operands of the
+ * next product, and the sigmoid is good to (4 + 1.2 |gate|) 2^-23 of itself. Backward forms them again from x: dx, dw_gate_up and dw_down (each may be null; the weights'
  * gradients are of type grad_dtype and overwritten). scratch: what the _scratch_bytes calls say. Outputs and
  * scratch overlap nothing else. A call repeats bit for bit; the order of its sums depends on the sizes and on the SMs at hand,
  * so a token beside others may differ from the same token alone in the last bits. The e4m3 form takes x and w_gate_up in 8 bits with

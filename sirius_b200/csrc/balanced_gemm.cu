@@ -3,16 +3,18 @@
 // The output is cut into tiles; a unit (a CTA, or a CTA pair with cta_group::2) takes whole tiles while there are enough for
 // all, and what is left over, fewer tiles than units, is cut along the reduction into as many equal ranges as there are units.
 // A unit that has only a part of a tile's reduction leaves fp32 sums in a slot of its own, and a second, small launch adds the
-// slots of every such tile in the order of the reduction. So 152 tiles on 74 pairs take 2.05 rounds and not three, a few rows
-// against a long reduction occupy the device, no CTA waits for another, and the sums have a fixed order. With few tiles a
-// cluster shares each, and the parts meet in its shared memory instead (split_gemm_kernel).
+// slots of every such tile in the order of the reduction. So the 152 tiles of a weight gradient take 74 pairs 2.05 rounds and not
+// three, a few rows against a long reduction occupy the device, no CTA waits for another, and the sums have a fixed order. With
+// few tiles a cluster shares each, and the parts meet in its shared memory instead (split_gemm_kernel).
 //
 // Warps as in the gated kernels: 0 TMA, 1 MMA, 2-17 four epilogue groups that take the 32-column slabs of a tile in turn. The
 // accumulator is double-buffered in tensor memory, so the epilogue of a tile runs beside the products of the next.
 //
-// Of the feed-forward block of 8192 tokens x 896 x 4864: y 58 us, 1230 TFLOP/s (a join of 5 beside it); dx 98 us, 1460, tensor pipe
-// 80 % busy; dWg over dWu 94 us, 1520, 83 %; dWd 56 us, 1280, 70 % (133 tiles for 148 CTAs). Operands come out of L2 at 11 to
-// 15 TB/s, which is what single CTAs are bound by; pairs read half of B each. A library product of these sizes takes 57, 109, 123
+// Of the feed-forward block of 8192 tokens x 896 x 4864: y 56 us, 1270 TFLOP/s, tensor pipe 65 % busy (128 tiles on 74 pairs, two
+// rounds for 1.73 of work; sharing the rest would cost more in slots and a second launch); dx 97 us, 1480, 80 % (one round of whole
+// tiles, 54 shared by all pairs, a join of 5 behind it); dWg over dWu 94 us, 1520, 83 % (two rounds, 4 tiles shared, a join); dWd
+// 54 us, 1320, 70 % (133 tiles for 148 CTAs). Operands come out of L2 at 11 to 15 TB/s, which is what single CTAs are bound by;
+// pairs read half of B each. A library product of these sizes takes 57, 109, 123
 // and 57 us. Two slabs for the output of an epilogue group instead of one cost a stage: dWd 55 -> 67 us.
 #include <cuda.h>
 

@@ -1,10 +1,11 @@
 // Root-mean-square norm with the residual's addition, its 8-bit output, its backward pass, and rows quantised as they are.
 //
 //   forward    h = x + residual,  rstd = 1 / sqrt(mean(h^2) + eps),  y = gamma h rstd
-//   8 bits     scale = max(max |y| / 448, 2^-126) of a row, q = e4m3(y / scale)
+//   8 bits     scale = max(max |y| / 448, 2^-126) of a row, q = e4m3(y (1 / scale)): a product with the rounded reciprocal, so a
+//              quotient within 2^-23 of itself of a rounding border may go to the other neighbour
 //   backward   xhat = h rstd,  g = gamma dy:  dx = dh + rstd (g - xhat mean(g xhat)),  dgamma = sum over rows of dy xhat
 //
-// bf16 or fp32 rows, fp32 parameters and statistics. y comes from the fp32 sum, not from the rounded h that is stored: one
+// bf16 or fp32 rows, fp32 parameters and statistics, the root by rsqrtf. y comes from the fp32 sum, not from the rounded h that is stored: one
 // rounding on the way to y instead of two.
 //
 // All of it is bound by memory: a row is read once, sits in the registers of one to sixteen warps (16 elements a lane, 32 in

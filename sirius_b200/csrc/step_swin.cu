@@ -86,8 +86,8 @@ struct Swin {
     SRT_CHECK_CUDA(cudaStreamWaitEvent(stream, ev_join, 0));
     return SRT_OK;
   }
-  GradBuckets buckets;
-  GradClip clip;  // norm of the gradients, and the coefficient of the next optimizer step      // units: the blocks in forward order, each stage's patch merging counted with its last block
+  GradBuckets buckets;      // units: the blocks in forward order, each stage's patch merging counted with its last block
+  GradClip clip;            // norm of the gradients, and the coefficient of the next optimizer step
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
   std::vector<void*> allocs;
