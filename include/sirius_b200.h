@@ -259,7 +259,8 @@ int srt_conv_plan_override(int gather, int tile_n, int pair);
 /* Process-wide: whether filter gradients may use the CTA-pair kernel (256 x 256 tiles, clusters of two) where the
  * shape allows, or always the single-CTA kernel. on = 1 / 0 sets it, -1 only reads; returns the previous setting.
  * srt_conv_wgrad_scratch_bytes covers both, so the switch may change between sizing and launch. Default 1; the
- * gradient exchange (srt_ddp_create) turns it off for data-parallel runs. */
+ * gradient exchange (srt_ddp_create) turns it off for data-parallel runs. The GPT-2, Swin and Qwen2 steps take the single-CTA
+ * kernel for the gradients that they queue on their second stream, whatever the switch says. */
 int srt_conv_wgrad_pairs(int on);
 
 /* ---- training-step executor (replaces the body of the reference's training loop:

@@ -136,6 +136,15 @@ struct PdlOff {  // scope guard
   explicit PdlOff(bool o) : off(o) { if (off) set_pdl_enabled(false); }
   ~PdlOff() { if (off) set_pdl_enabled(true); }
 };
+// Per thread: filter gradients launched while this lives take the kernel without CTA pairs. For executors that queue them on a
+// second stream beside attention, norms and products of the first: the stalls on record (a step that never returned, the device
+// still answering) were all steps of such an executor with pairs on that stream, and no cause was found.
+void set_wgrad_beside(bool on);
+struct WgradBeside {  // scope guard
+  bool on;
+  explicit WgradBeside(bool o) : on(o) { if (on) set_wgrad_beside(true); }
+  ~WgradBeside() { if (on) set_wgrad_beside(false); }
+};
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl_if(bool early, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                                  cudaStream_t st, Args&&... args) {

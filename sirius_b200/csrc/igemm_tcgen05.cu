@@ -1655,6 +1655,7 @@ struct WgradPlan {
   bool pair;  // 256 x 256 tiles on CTA pairs
 };
 
+static thread_local bool tl_wgrad_beside = false;
 static int g_wgrad_pair = getenv("SIRIUS_B200_WGRAD_PAIR") ? atoi(getenv("SIRIUS_B200_WGRAD_PAIR")) : 1;
 
 // sizing = true asks what the plan would be with every process-wide switch (pair kernel, plan override, im2col) in
@@ -1664,7 +1665,7 @@ WgradPlan plan_wgrad(const GatherGeom& g, bool allow_pair = true, bool sizing = 
   const bool plain = g.R == 1 && g.S == 1 && g.stride == 1 && g.pad == 0;
   w.b_tma = g_force_gather ? 0 : plain ? 1 : (im2col_ok(g) && g_im2col_enabled) ? 2 : 0;
   const bool by_tma = sizing ? (plain || im2col_ok(g)) : w.b_tma != 0;
-  const bool switched_on = sizing || (g_wgrad_pair && g_force_pair != 0);
+  const bool switched_on = sizing || (g_wgrad_pair && g_force_pair != 0 && !tl_wgrad_beside);
   // CTA pairs where both operands come by TMA and the tile is not mostly padding: at least 256 filters (ragged
   // beyond that is fine) and 192 columns
   w.pair = allow_pair && switched_on && by_tma && g.Nout >= 256 && g.Kg >= 192 && g.src_c % 64 == 0 && sm_count() >= 2;
@@ -1834,6 +1835,7 @@ int tc_status_fetch(int* out) {
 //   pair    0: one CTA per tile, 1: CTA pairs wherever the shape allows, -1: heuristic
 static int g_force_bn = 0;
 static int g_gather_lag = getenv("SIRIUS_B200_GATHER_LAG") ? atoi(getenv("SIRIUS_B200_GATHER_LAG")) : 0;  // 0 = stage count - 2
+void set_wgrad_beside(bool on) { tl_wgrad_beside = on; }
 void tc_set_wgrad_pairs(bool on) { g_wgrad_pair = on ? 1 : 0; }
 bool tc_wgrad_pairs() { return g_wgrad_pair != 0; }
 

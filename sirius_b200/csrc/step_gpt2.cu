@@ -221,6 +221,7 @@ struct Gpt2 {
     }
     {
       PdlOff no_early_launch(ws != stream);
+      WgradBeside single_ctas(ws != stream);
       if ((rc = colsum_bf16(dy, T, l.out, gf(l.b), wscratch, scratch_bytes, ws))) return rc;
       if ((rc = conv_wgrad(lin_desc(T, l.in, l.out), SRT_BF16, SRT_IMPL_AUTO, dy, x, gf(l.w), wscratch, scratch_bytes, ws)))
         return rc;
@@ -419,6 +420,7 @@ int Gpt2::backward(int B, int global_batch) {
     SRT_CHECK_CUDA(cudaStreamWaitEvent(side, ev_fork, 0));
     side_dirty = true;
     PdlOff no_early_launch(true);
+    WgradBeside single_ctas(true);
     if ((rc = conv_wgrad(lin_desc(T, C, Vpad), SRT_BF16, SRT_IMPL_AUTO, logits, lnfo, gf(wte), scratch_side, scratch_bytes, side)))
       return rc;
   } else if ((rc = conv_wgrad(lin_desc(T, C, Vpad), SRT_BF16, SRT_IMPL_AUTO, logits, lnfo, gf(wte), scratch, scratch_bytes,

@@ -223,6 +223,7 @@ struct Qwen2 {
     }
     {
       PdlOff no_early_launch(ws != stream);
+      WgradBeside single_ctas(ws != stream);
       if (l.b_off >= 0 && (rc = colsum_bf16(dy, T, l.out, G + l.b_off, wscratch, scratch_bytes, ws))) return rc;
       if ((rc = conv_wgrad(lin_desc(T, l.in, l.out), SRT_BF16, SRT_IMPL_AUTO, dy, x, G + l.w_off, wscratch, scratch_bytes, ws)))
         return rc;
@@ -446,6 +447,7 @@ int Qwen2::backward(int B, int global_batch) {
     SRT_CHECK_CUDA(cudaStreamWaitEvent(side, ev_fork, 0));
     side_dirty = true;
     PdlOff no_early_launch(true);
+    WgradBeside single_ctas(true);
     if ((rc = conv_wgrad(lin_desc(T, C, Vpad), SRT_BF16, SRT_IMPL_AUTO, logits, nfo, gf(emb), scratch_side, scratch_bytes, side)))
       return rc;
   } else if ((rc = conv_wgrad(lin_desc(T, C, Vpad), SRT_BF16, SRT_IMPL_AUTO, logits, nfo, gf(emb), scratch, scratch_bytes,

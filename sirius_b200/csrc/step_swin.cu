@@ -150,6 +150,7 @@ struct Swin {
     }
     {
       PdlOff no_early_launch(ws != stream);
+      WgradBeside single_ctas(ws != stream);
       if (l.b >= 0 && (rc = colsum_bf16(dy, T, l.out, gf(l.b), wscratch, scratch_bytes, ws))) return rc;
       if ((rc = conv_wgrad(lin_desc(T, l.in, l.out), SRT_BF16, SRT_IMPL_AUTO, dy, x, gf(l.w), wscratch, scratch_bytes, ws)))
         return rc;
