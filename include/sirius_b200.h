@@ -205,7 +205,8 @@ int srt_adamw(float* p, const float* g, float* m, float* v, void* p_bf16, int64_
  * counts are host arrays and are read before the call returns. srt_clip_grad_norm refuses arrays that share memory.
  * srt_adamw_clipped forms 1 - beta and the bias corrections in 64 bits and rounds them once. srt_adamw, and the executors' steps
  * with or without clipping, form them in fp32 from the rounded betas, so 1 - beta is off by up to 2^-25 / (1 - beta) of itself
- * there (3e-5 for 0.999): with a coefficient of one the two agree to that, and the moments bit for bit where fp32 holds the betas exactly. */
+ * there (3e-5 for 0.999): with a coefficient of one the two agree to that, and the moments bit for bit where fp32 holds the
+ * betas exactly. */
 size_t srt_grad_norm_scratch_bytes(int tensors);
 int srt_grad_norm(int dtype, int tensors, const void* const* grads, const int64_t* counts, float max_norm, float* clip, void* scratch,
                   size_t scratch_bytes, void* stream);
@@ -544,7 +545,8 @@ int srt_rmsnorm_bwd(int dtype, const void* dy, const void* h, const float* gamma
  * w_gate_up = Wg over Wu [2 hidden][width], w_down = Wd [width][hidden], all bf16, fp32 accumulation; width and hidden are
  * multiples of 8, operands and scratch 16-byte aligned, matrices below 2^31 elements. residual may be null. The gate and up
  * projections never reach memory; act, and in backward the gradients of gate and up, are rounded to bf16 once, as operands of the
- * next product, and the sigmoid is good to (4 + 1.2 |gate|) 2^-23 of itself. Backward forms them again from x: dx, dw_gate_up and dw_down (each may be null; the weights'
+ * next product, and the sigmoid is good to (4 + 1.2 |gate|) 2^-23 of itself. Backward forms the projections again from x: dx,
+ * dw_gate_up and dw_down (each may be null; the weights'
  * gradients are of type grad_dtype and overwritten). scratch: what the _scratch_bytes calls say. Outputs and
  * scratch overlap nothing else. A call repeats bit for bit; the order of its sums depends on the sizes and on the SMs at hand,
  * so a token beside others may differ from the same token alone in the last bits. The e4m3 form takes x and w_gate_up in 8 bits with

@@ -67,7 +67,11 @@ def _build_binding(force: bool) -> None:
            "-isystem", str(cuda / "include"), str(BINDING_SRC), "-o", str(BINDING), f"-L{torch_dir / 'lib'}",
            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
     stamp = BUILD / "_ops_native.stamp"
-    built_for = "\n".join(["torch " + importlib.metadata.version("torch"), str(sysconfig.get_config_var("SOABI")), *cmd]) + "\n"
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:   # a source tree on the path
+        version = (torch_dir / "version.py").read_text()
+    built_for = "\n".join(["torch " + version, str(sysconfig.get_config_var("SOABI")), *cmd]) + "\n"
     newest = max(p.stat().st_mtime for p in (BINDING_SRC, *(PKG.parent / "include").glob("*.h")))
     if (not force and BINDING.exists() and BINDING.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == built_for):
         return

@@ -14,8 +14,8 @@
 // rounds for 1.73 of work; sharing the rest would cost more in slots and a second launch); dx 97 us, 1480, 80 % (one round of whole
 // tiles, 54 shared by all pairs, a join of 5 behind it); dWg over dWu 94 us, 1520, 83 % (two rounds, 4 tiles shared, a join); dWd
 // 54 us, 1320, 70 % (133 tiles for 148 CTAs). Operands come out of L2 at 11 to 15 TB/s, which is what single CTAs are bound by;
-// pairs read half of B each. A library product of these sizes takes 57, 109, 123
-// and 57 us. Two slabs for the output of an epilogue group instead of one cost a stage: dWd 55 -> 67 us.
+// pairs read half of B each. A library product of these sizes takes 57, 109, 123 and 57 us. Two slabs for the output of an epilogue
+// group instead of one cost a stage: dWd 55 -> 67 us.
 #include <cuda.h>
 
 #include <atomic>

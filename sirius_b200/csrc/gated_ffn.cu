@@ -17,8 +17,8 @@
 //
 // act, dgate and dup are rounded to bf16 once: they are operands of tensor-core products. Everything before that is fp32, the
 // sigmoid from __expf and __fdividef (off by 2 + 1.17 |gate| and by 2 units in the last place: 2^-18 of itself up to a gate of 20,
-// far below bf16's 2^-9). Against 64 bits the rounding of act takes y of 1237 x 1544 x 8936 from 0.0017 of its 2-norm, which is y's own rounding, to 0.0019; the gradients of 8192 x 896
-// x 4864, with that of dgate and dup, to 0.0023.
+// far below bf16's 2^-9). Against 64 bits the rounding of act takes y of 1237 x 1544 x 8936 from 0.0017 of its 2-norm, which is
+// y's own rounding, to 0.0019; the gradients of 8192 x 896 x 4864, with that of dgate and dup, to 0.0023.
 //
 // 8192 tokens x 896 x 4864, one launch each. Forward 92 us, 1550 TFLOP/s, tensor pipe 85 % busy, operands out of L2 at 12.1 TB/s,
 // 49 % of its rate; the rest is the epilogue of a last, partly filled round. Backward 158 us, 1360 TFLOP/s, tensor pipe 73 %: its

@@ -5,8 +5,8 @@
 //              quotient within 2^-23 of itself of a rounding border may go to the other neighbour
 //   backward   xhat = h rstd,  g = gamma dy:  dx = dh + rstd (g - xhat mean(g xhat)),  dgamma = sum over rows of dy xhat
 //
-// bf16 or fp32 rows, fp32 parameters and statistics, the root by rsqrtf. y comes from the fp32 sum, not from the rounded h that is stored: one
-// rounding on the way to y instead of two.
+// bf16 or fp32 rows, fp32 parameters and statistics, the root by rsqrtf. y comes from the fp32 sum, not from the rounded h that
+// is stored: one rounding on the way to y instead of two.
 //
 // All of it is bound by memory: a row is read once, sits in the registers of one to sixteen warps (16 elements a lane, 32 in
 // the longest rows) until its statistics are known, and is written once; the next row's loads are in flight meanwhile.
